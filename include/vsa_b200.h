@@ -446,6 +446,30 @@ int vsa_sparse_bwd_dkdv_raster(const void* dout, const void* q, const void* k, c
                                int64_t BH, int64_t Lq, int64_t Lkv, int D, int be, int topk,
                                float scale, int dtype, void* stream);
 
+/* ---- rotary positions ---------------------------------------------------------------------------------------
+ * y[b, h, l] = x[b, h, l] with the pairs of its first rotary_dim dims turned by the angles of the token's table row:
+ * (a, b) -> (a cos - b sin, b cos + a sin); inverse = 1 turns the other way, which is the gradient.  Pairs are neighbours
+ * (2i, 2i+1) where interleaved, else halves (i, i + rotary_dim/2); the other dims are copied.  Two tensors (q and k, any
+ * numbers of heads, heads[i] = 0: absent) in one launch; x and y do not overlap; strides in elements, head dim contiguous.
+ *   cos_table, sin_table  [table_rows, rotary_dim/2] fp32
+ *   positions             table row of token l of batch b at positions[b * positions_stride + l]; NULL: l.  A row outside
+ *                         the table leaves the token as it is.
+ *   src_map               NULL, or the source row of destination row l ([rows], values outside [0, src_rows): zeros are
+ *                         written): raster <-> tile order on the way.
+ * Head dims up to 256; 16-byte aligned rows are the fast path.  No reference counterpart. */
+typedef struct VsaRotary {
+  const void* x[2];
+  void* y[2];
+  const float *cos_table, *sin_table;
+  const int32_t *positions, *src_map;
+  int64_t B, rows, src_rows, table_rows, positions_stride;
+  int64_t x_stride[2][3], y_stride[2][3];      /* batch, head, token */
+  int heads[2];
+  int D, rotary_dim, interleaved, inverse, dtype;
+} VsaRotary;
+
+int vsa_rotary(const VsaRotary* a, void* stream);
+
 /* out = out_s + out_c[block] * gate (gate may be NULL) in fp32, one rounding.
  * Replaces _combine_forward_kernel: vsa/fused_common.py:175-199,259-295. */
 int vsa_combine_fwd(const void* out_s, const void* out_c, const void* gate, void* out,

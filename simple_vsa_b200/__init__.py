@@ -8,7 +8,12 @@ Drop-in names (same positional order as ``vsa/__init__.py`` of the reference):
 * ``b200_sparse_attention(q, k, v, selected, variable_block_sizes, *, block_size,
   sm_scale=None)`` and its aliases ``triton_sparse_attention``,
   ``helion_sparse_attention`` -- the fine branch on caller-supplied routes;
-* ``block_mean``, ``topk_block_mask``, ``CompressionGate``.
+* ``block_mean``, ``topk_block_mask``, ``CompressionGate``;
+
+and what a video transformer's layer has around the operator:
+
+* ``video_rotary(q, k, rotary, positions=None)`` / ``video_rotary_raster`` with ``build_rotary_metadata`` -- rotary
+  positions, also on the way into tile order (``tile_heads``, ``video_sparse_attn_raster``).
 
 Everything runs in hand-written CUDA kernels for sm_100a loaded from
 ``libvsa_b200.so``; importing this package without that library raises.
@@ -24,6 +29,7 @@ from torch import Tensor, nn
 from . import _lib  # noqa: F401  (fails loudly when the CUDA library is absent)
 from .tiling import build_vsa_metadata, tile, tile_with, untile, untile_with
 from .raster import tile_heads, untile_heads, video_sparse_attn_raster
+from .rotary import build_rotary_metadata, video_rotary, video_rotary_raster
 from .ops import (
     BlockSize,
     as_block_elements,
@@ -41,6 +47,7 @@ __all__ = [
     "as_block_elements", "validate_vsa_inputs",
     "build_vsa_metadata", "tile", "untile", "tile_with", "untile_with",
     "video_sparse_attn_raster", "tile_heads", "untile_heads",
+    "build_rotary_metadata", "video_rotary", "video_rotary_raster",
 ]
 
 

@@ -37,6 +37,14 @@ class OperatorBwd(ctypes.Structure):
                [("scale", F), ("dtype", I)]
 
 
+class Rotary(ctypes.Structure):
+    """``VsaRotary`` of the header."""
+    _fields_ = [("x", P * 2), ("y", P * 2)] + [(n, P) for n in ("cos_table", "sin_table", "positions", "src_map")] + \
+               [(n, L) for n in ("B", "rows", "src_rows", "table_rows", "positions_stride")] + \
+               [("x_stride", (L * 3) * 2), ("y_stride", (L * 3) * 2), ("heads", I * 2)] + \
+               [(n, I) for n in ("D", "rotary_dim", "interleaved", "inverse", "dtype")]
+
+
 # name -> argument types, in the order of include/vsa_b200.h
 SIGNATURES = {
     "vsa_block_mean3_fwd": [P, P, P, P, P, P, P, P, L, L, L, I, I, I, P],
@@ -76,6 +84,7 @@ SIGNATURES = {
     "vsa_combine_bwd": [P, P, P, P, P, L, L, I, I, I, P],
     "vsa_operator_fwd": [ctypes.POINTER(OperatorFwd), P],
     "vsa_operator_bwd": [ctypes.POINTER(OperatorBwd), P],
+    "vsa_rotary": [ctypes.POINTER(Rotary), P],
 }
 PLAIN = {"vsa_last_error_string": ([], c_char_p), "vsa_version": ([], c_int),
          "vsa_launch_count": ([], c_int64),

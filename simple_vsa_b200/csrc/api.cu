@@ -631,6 +631,19 @@ int vsa_combine_bwd(const void* dout, const void* gate, const void* out_c, void*
   return combine_bwd(dout, gate, out_c, d_out_c, dgate, BH, Lq, D, be, dtype, (cudaStream_t)stream);
 }
 
+int vsa_rotary(const VsaRotary* a, void* stream) {
+  VSA_REQUIRE(a, "rotary: null pointer");
+  int rc = check_dtype(a->dtype);
+  if (rc) return rc;
+  VSA_REQUIRE(a->B >= 0 && a->rows >= 0 && a->src_rows >= 0 && a->table_rows >= 0 && a->heads[0] >= 0 && a->heads[1] >= 0 && a->D >= 0,
+              "rotary: negative extent");
+  VSA_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim % 2 == 0 && a->rotary_dim <= a->D, "rotary: rotary_dim must be even and at most the head dim");
+  VSA_REQUIRE(a->rotary_dim == 0 || a->table_rows == 0 || (a->cos_table && a->sin_table), "rotary: null table");
+  for (int t = 0; t < 2; ++t)
+    VSA_REQUIRE(a->heads[t] == 0 || a->B == 0 || a->rows == 0 || a->D == 0 || (a->y[t] && (a->x[t] || a->src_rows == 0)), "rotary: null pointer");
+  return rotary(*a, (cudaStream_t)stream);
+}
+
 int vsa_operator_fwd(const VsaOperatorFwd* a, void* stream) {
   VSA_REQUIRE(a, "operator forward: null pointer");
   int rc = check_sparse(a->BH, a->Lq, a->Lkv, a->D, a->be, a->topk, a->dtype);

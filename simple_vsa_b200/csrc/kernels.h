@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/vsa_b200.h"
+
 namespace vsa {
 
 // ---- scalar kernels (generic_kernels.cu) -------------------------------------------------
@@ -52,6 +54,9 @@ int sparse_dkdv_scalar(const void* dout, const void* q, const void* k, const voi
                        const float* delta, const int32_t* counts, const int32_t* offsets, const int32_t* inverse,
                        const int32_t* kv_sizes, void* dk, void* dv, int64_t BH, int64_t Lq, int64_t Lkv, int D, int be,
                        int topk, float scale, int dtype, cudaStream_t st);
+
+// ---- rotary positions (rotary.cu) --------------------------------------------------------
+int rotary(const VsaRotary& a, cudaStream_t st);
 
 // ---- fp32 on 64 x 64 tiles, head dim 64 or 128, block volume 64, 128 or 256 (sparse_f32.cu) --------------------
 // operands: every tensor of the call that is read or written in 16-byte pieces
