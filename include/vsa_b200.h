@@ -470,6 +470,41 @@ typedef struct VsaRotary {
 
 int vsa_rotary(const VsaRotary* a, void* stream);
 
+/* ---- cross attention -------------------------------------------------------------------------------------------
+ * out[b, h, i] = sum_j p_ij v[b, h', j], p_i = softmax over the live keys j of scale * q[b, h, i] . k[b, h', j]; the H / Hkv query
+ * heads from h' * H / Hkv on share key head h'.  Key j of sample b is live where j < kv_lengths[b] (NULL: all) and, with
+ * key_bits, where its bit is set.  A row without a live key gets zeros, and passes no gradient; keys that are not live are not
+ * looked at (they may hold anything) and receive zeros.  Strides in elements: batch, head, token; head dims contiguous.
+ *   key_bits  [B, vsa_cross_words(Lkv)] from vsa_cross_key_bits (which folds kv_lengths in), or NULL
+ *   lse2      [B * H, Lq rounded up to 128] fp32: base-2 log-sum-exp of the scaled scores, +inf for rows without a live key and
+ *             for the padding; written by the forward, read by the backward
+ *   delta     the same shape, scratch of the backward
+ *   workspace vsa_cross_workspace_bytes(backward, ...) bytes (0: may be NULL), 16-byte aligned, free again after the call
+ * bf16 and fp16 with head dims that are multiples of 8 up to 128, 16-byte aligned pointers and strides of multiples of 8 run on
+ * tcgen05 kernels (vsa_cross_on_tensor_cores), everything else up to head dim 256 on CUDA cores in fp32.  Results do not
+ * depend on the order in which blocks run.  No reference counterpart (its operator is self-attention over one token grid). */
+typedef struct VsaCross {
+  const void *q, *k, *v, *dout;
+  void *out, *dq, *dk, *dv;                    /* dout, dq, dk, dv, delta: backward only */
+  float *lse2, *delta;
+  const int32_t* kv_lengths;
+  const uint32_t* key_bits;
+  void* workspace;
+  int64_t B, H, Hkv, Lq, Lkv;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+  float scale;
+  int D, dtype;
+} VsaCross;
+
+int vsa_cross_fwd(const VsaCross* a, void* stream);
+int vsa_cross_bwd(const VsaCross* a, void* stream);
+int vsa_cross_on_tensor_cores(const VsaCross* a, int backward);
+int64_t vsa_cross_workspace_bytes(int backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype);
+int64_t vsa_cross_words(int64_t Lkv);
+/* mask [B, Lkv] bytes, rows mask_stride apart: non-zero = live. */
+int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* kv_lengths, uint32_t* key_bits, int64_t B, int64_t Lkv,
+                       void* stream);
+
 /* out = out_s + out_c[block] * gate (gate may be NULL) in fp32, one rounding.
  * Replaces _combine_forward_kernel: vsa/fused_common.py:175-199,259-295. */
 int vsa_combine_fwd(const void* out_s, const void* out_c, const void* gate, void* out,

@@ -13,7 +13,9 @@ Drop-in names (same positional order as ``vsa/__init__.py`` of the reference):
 and what a video transformer's layer has around the operator:
 
 * ``video_rotary(q, k, rotary, positions=None)`` / ``video_rotary_raster`` with ``build_rotary_metadata`` -- rotary
-  positions, also on the way into tile order (``tile_heads``, ``video_sparse_attn_raster``).
+  positions, also on the way into tile order (``tile_heads``, ``video_sparse_attn_raster``);
+* ``video_cross_attn(q, k, v, kv_lengths=None, kv_mask=None)`` / ``video_cross_attn_raster`` -- attention to an
+  encoder's states of another length.
 
 Everything runs in hand-written CUDA kernels for sm_100a loaded from
 ``libvsa_b200.so``; importing this package without that library raises.
@@ -29,6 +31,7 @@ from torch import Tensor, nn
 from . import _lib  # noqa: F401  (fails loudly when the CUDA library is absent)
 from .tiling import build_vsa_metadata, tile, tile_with, untile, untile_with
 from .raster import tile_heads, untile_heads, video_sparse_attn_raster
+from .cross import video_cross_attn, video_cross_attn_raster
 from .rotary import build_rotary_metadata, video_rotary, video_rotary_raster
 from .ops import (
     BlockSize,
@@ -47,6 +50,7 @@ __all__ = [
     "as_block_elements", "validate_vsa_inputs",
     "build_vsa_metadata", "tile", "untile", "tile_with", "untile_with",
     "video_sparse_attn_raster", "tile_heads", "untile_heads",
+    "video_cross_attn", "video_cross_attn_raster",
     "build_rotary_metadata", "video_rotary", "video_rotary_raster",
 ]
 

@@ -45,6 +45,15 @@ class Rotary(ctypes.Structure):
                [(n, I) for n in ("D", "rotary_dim", "interleaved", "inverse", "dtype")]
 
 
+class Cross(ctypes.Structure):
+    """``VsaCross`` of the header."""
+    _fields_ = [(n, P) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "lse2", "delta", "kv_lengths", "key_bits",
+                                 "workspace")] + \
+               [(n, L) for n in ("B", "H", "Hkv", "Lq", "Lkv")] + \
+               [(n + "_stride", L * 3) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + \
+               [("scale", F), ("D", I), ("dtype", I)]
+
+
 # name -> argument types, in the order of include/vsa_b200.h
 SIGNATURES = {
     "vsa_block_mean3_fwd": [P, P, P, P, P, P, P, P, L, L, L, I, I, I, P],
@@ -85,6 +94,9 @@ SIGNATURES = {
     "vsa_operator_fwd": [ctypes.POINTER(OperatorFwd), P],
     "vsa_operator_bwd": [ctypes.POINTER(OperatorBwd), P],
     "vsa_rotary": [ctypes.POINTER(Rotary), P],
+    "vsa_cross_fwd": [ctypes.POINTER(Cross), P],
+    "vsa_cross_bwd": [ctypes.POINTER(Cross), P],
+    "vsa_cross_key_bits": [P, L, P, P, L, L, P],
 }
 PLAIN = {"vsa_last_error_string": ([], c_char_p), "vsa_version": ([], c_int),
          "vsa_launch_count": ([], c_int64),
@@ -94,7 +106,10 @@ PLAIN = {"vsa_last_error_string": ([], c_char_p), "vsa_version": ([], c_int),
          "vsa_sparse_raster_supported": ([I, I, I, I], c_int),
          "vsa_sparse_kernel_family": ([I, I, I, I], c_int),
          "vsa_sparse_pass_kernels": ([I, L, L, I, I, I, I], c_int),
-         "vsa_sparse_bwd_ds_workspace_bytes": ([L, L, I, I], c_int64)}
+         "vsa_sparse_bwd_ds_workspace_bytes": ([L, L, I, I], c_int64),
+         "vsa_cross_on_tensor_cores": ([ctypes.POINTER(Cross), I], c_int),
+         "vsa_cross_workspace_bytes": ([I, L, L, L, L, L, I, I], c_int64),
+         "vsa_cross_words": ([L], c_int64)}
 
 
 class VsaError(RuntimeError):

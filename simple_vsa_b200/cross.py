@@ -1,0 +1,158 @@
+"""Cross attention of the video tokens to an encoder's states: every query attends to all live keys of its sample.
+
+Beside the sparse self-attention of a video transformer's layer stands a dense attention to the states of a prompt (or an image)
+encoder: queries by the ten thousand, keys by the hundred, of another length per sample.  ``video_cross_attn`` takes
+``[batch, heads, seq_len, dim]`` tensors, ``video_cross_attn_raster`` the ``[batch, seq_len, heads, head_dim]`` that the
+projections leave; both read and write any strides with a contiguous head dim in place.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _lib, ops
+from ._lib import call
+
+
+def _usable(x: Tensor) -> Tensor:
+    """The tensor itself where its rows can be read in place, else a dense copy: head dim contiguous, and in 16-bit types with
+    head dims of whole 16-byte pieces everything on 16-byte boundaries (other rows run on CUDA cores, element by element)."""
+    if x.shape[3] > 1 and x.stride(3) != 1:
+        return x.contiguous()
+    if x.element_size() == 2 and x.shape[3] % 8 == 0:
+        steps = [s for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1]
+        if x.data_ptr() % 16 or any(s % 8 or s <= 0 for s in steps):
+            return ops._dense(x)
+    return x
+
+
+def _arguments(q, k, v, kv_lengths, key_bits, scale: float, dt: int) -> _lib.Cross:
+    a = _lib.Cross()
+    a.B, a.H, a.Lq, a.D = q.shape
+    a.Hkv, a.Lkv = k.shape[1], k.shape[2]
+    a.scale, a.dtype = scale, dt
+    a.kv_lengths, a.key_bits = ops._ptr(kv_lengths), ops._ptr(key_bits)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _operand(a, name, t)
+    return a
+
+
+def _operand(a: _lib.Cross, name: str, t: Tensor) -> None:
+    setattr(a, name, t.data_ptr())
+    getattr(a, name + "_stride")[:] = t.stride()[:3]
+
+
+def _workspace(a: _lib.Cross, backward: int, device) -> Optional[Tensor]:
+    n = _lib.lib.vsa_cross_workspace_bytes(backward, a.B, a.H, a.Hkv, a.Lq, a.Lkv, a.D, a.dtype)
+    if n <= 0:
+        return None
+    ws = torch.empty(n, device=device, dtype=torch.uint8)
+    a.workspace = ws.data_ptr()
+    return ws
+
+
+def _key_bits(kv_mask: Tensor, kv_lengths: Optional[Tensor]) -> Tensor:
+    """The mask packed to a bit per key, whole tiles of 128 keys, the lengths folded in."""
+    B, T = kv_mask.shape
+    bits = torch.empty((B, _lib.lib.vsa_cross_words(T)), device=kv_mask.device, dtype=torch.int32)
+    call("vsa_cross_key_bits", kv_mask.data_ptr(), kv_mask.stride(0), ops._ptr(kv_lengths), bits.data_ptr(), B, T,
+         ops._stream(kv_mask.device))
+    return bits
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lengths, key_bits, scale, need_grad):
+        B, H, L, D = q.shape
+        dt = ops._check_device_dtype(q, k, v)
+        out = torch.empty_like(q)
+        lse = torch.empty((B * H, -(-L // 128) * 128), device=q.device, dtype=torch.float32)
+        a = _arguments(q, k, v, kv_lengths, key_bits, scale, dt)
+        _operand(a, "out", out)
+        a.lse2 = lse.data_ptr()
+        ws = _workspace(a, 0, q.device)  # noqa: F841  alive until the launch
+        call("vsa_cross_fwd", a, ops._stream(q.device))
+        if need_grad:
+            ctx.save_for_backward(q, k, v, out, lse, kv_lengths, key_bits)
+            ctx.scale = scale
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, kv_lengths, key_bits = ctx.saved_tensors
+        with torch.cuda.device(q.device):
+            dt = ops._check_device_dtype(q, k, v)
+            dout = _usable(dout)
+            a = _arguments(q, k, v, kv_lengths, key_bits, ctx.scale, dt)
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+            delta = torch.empty_like(lse)
+            for name, t in (("out", out), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+                _operand(a, name, t)
+            a.lse2, a.delta = lse.data_ptr(), delta.data_ptr()
+            ws = _workspace(a, 1, q.device)  # noqa: F841
+            call("vsa_cross_bwd", a, ops._stream(q.device))
+        return dq, dk, dv, None, None, None, None
+
+
+def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
+    layout = "[batch, seq_len, heads, head_dim]" if raster else "[batch, heads, seq_len, dim]"
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError(f"q, k, and v must have shape {layout}")
+    if raster:
+        q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+    B, H, L, D = q.shape
+    T = k.shape[2]
+    if k.shape[0] != B or v.shape[0] != B:
+        raise ValueError("q, k, and v must share the batch dimension")
+    if v.shape[1] != k.shape[1] or v.shape[2] != T:
+        raise ValueError("k and v must have the same heads and sequence length")
+    if k.shape[1] == 0 and H or k.shape[1] and H % k.shape[1]:
+        raise ValueError(f"the {H} query heads must be a multiple of the {k.shape[1]} key heads")
+    if k.shape[3] != D or v.shape[3] != D:
+        raise ValueError("q, k, and v must have the same head dimension")
+    if not 1 <= D <= 256:
+        raise ValueError(f"cross attention supports head dimensions from 1 to 256, got {D}")
+    ops._check_device_dtype(q, k, v)
+    if kv_lengths is not None and (kv_lengths.is_floating_point() or kv_lengths.dtype == torch.bool or tuple(kv_lengths.shape) != (B,)):
+        raise ValueError(f"kv_lengths must hold {B} integers, one per sample")
+    if kv_mask is not None and (kv_mask.dtype != torch.bool or tuple(kv_mask.shape) != (B, T)):
+        raise ValueError(f"kv_mask must be a bool tensor of shape [{B}, {T}], True where a key takes part")
+    scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D)
+    if not math.isfinite(scale):
+        raise ValueError("sm_scale must be finite")
+    with torch.cuda.device(q.device):
+        if kv_lengths is not None:
+            if kv_lengths.dtype == torch.int64:
+                kv_lengths = kv_lengths.clamp(0, T)
+            kv_lengths = ops._sizes(kv_lengths, q.device)
+        key_bits = None
+        if kv_mask is not None:
+            kv_mask = kv_mask.to(q.device)
+            key_bits = _key_bits(kv_mask if T <= 1 or kv_mask.stride(1) == 1 else kv_mask.contiguous(), kv_lengths)
+        q, k, v = _usable(q), _usable(k), _usable(v)
+        need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+        out = _CrossAttention.apply(q, k, v, kv_lengths, key_bits, scale, need_grad)
+    return out.transpose(1, 2) if raster else out
+
+
+def video_cross_attn(q: Tensor, k: Tensor, v: Tensor, kv_lengths: Optional[Tensor] = None, *, kv_mask: Optional[Tensor] = None,
+                     sm_scale: Optional[float] = None) -> Tensor:
+    """Attention of ``q [batch, heads, seq_len, dim]`` to ``k, v [batch, kv_heads, kv_len, dim]`` of another length.
+
+    ``heads`` is a multiple of ``kv_heads``; neighbouring query heads share a key head.  Key j of sample b takes part where
+    ``j < kv_lengths[b]`` (None: all; lengths beyond kv_len are kv_len) and ``kv_mask[b, j]`` (bool, None: all).  What stands in
+    the other keys and values does not matter, NaN included; a sample without a key that takes part gives zeros and zero
+    gradients.  Scale ``1/sqrt(dim)`` unless ``sm_scale`` says otherwise.  bf16, fp16 or fp32; head dims up to 256, in 16-bit types
+    multiples of 8 up to 128 on the tensor cores.  Differentiable in q, k and v."""
+    return _attend(q, k, v, kv_lengths, kv_mask, sm_scale, False)
+
+
+def video_cross_attn_raster(q: Tensor, k: Tensor, v: Tensor, kv_lengths: Optional[Tensor] = None, *,
+                            kv_mask: Optional[Tensor] = None, sm_scale: Optional[float] = None) -> Tensor:
+    """:func:`video_cross_attn` for ``[batch, seq_len, heads, head_dim]`` activations, as the projections leave them; no tensor is
+    re-laid, and the output comes in the same layout."""
+    return _attend(q, k, v, kv_lengths, kv_mask, sm_scale, True)

@@ -631,6 +631,105 @@ int vsa_combine_bwd(const void* dout, const void* gate, const void* out_c, void*
   return combine_bwd(dout, gate, out_c, d_out_c, dgate, BH, Lq, D, be, dtype, (cudaStream_t)stream);
 }
 
+// ---- cross attention ----------------------------------------------------------------------------------------
+// Parts that a pass is cut into: `units` blocks of work of `steps` steps each; a part more costs a block's set-up, taken as
+// `setup` steps.  The smallest time of whole waves over the SMs wins, the fewest parts among equals.
+static int cross_parts(int64_t units, int64_t steps, int64_t setup, int64_t most) {
+  const int64_t sms = 148;
+  int best = 1;
+  int64_t best_time = -1;
+  for (int64_t s = 1; s <= steps && s <= most; ++s) {
+    const int64_t per = (steps + s - 1) / s;
+    if ((steps + per - 1) / per != s) continue;      // the same cut as with fewer parts
+    const int64_t time = (units * s + sms - 1) / sms * (per + setup);
+    if (best_time < 0 || time < best_time) best_time = time, best = (int)s;
+    if (units * s > 16 * sms) break;
+  }
+  return best;
+}
+static int cross_fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  const int tile = cross_generic_tile(D);
+  (void)dtype;
+  return cross_parts(B * H * ((Lq + tile - 1) / tile), (Lkv + tile - 1) / tile, 2, 64);
+}
+static int cross_bwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  const int tile = cross_generic_tile(D);
+  (void)dtype;
+  return cross_parts(B * Hkv * ((Lkv + tile - 1) / tile), (H / Hkv) * ((Lq + tile - 1) / tile), 2, 64);
+}
+static bool cross_extents_fine(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D) {
+  return B >= 0 && H >= 0 && Hkv >= 0 && Lq >= 0 && Lkv >= 0 && D >= 1 && D <= 256 && (Hkv == 0 ? H == 0 : H % Hkv == 0) && B <= 65535 &&
+         H <= 65535 && Lq <= 0x3fffffff && Lkv <= 0x3fffffff;
+}
+
+int64_t vsa_cross_words(int64_t Lkv) { return Lkv < 0 ? -1 : cross_words(Lkv); }
+
+int64_t vsa_cross_workspace_bytes(int backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  if (!cross_extents_fine(B, H, Hkv, Lq, Lkv, D) || (dtype != VSA_BF16 && dtype != VSA_F32 && dtype != VSA_F16)) return -1;
+  if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return 0;
+  if (!backward) {
+    const int64_t s = cross_fwd_splits(B, H, Lq, Lkv, D, dtype);
+    return s == 1 ? 0 : s * B * H * Lq * (D + 1) * 4;
+  }
+  const int64_t s = cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype);
+  return s == 1 ? 0 : s * 2 * B * Hkv * Lkv * D * 4;
+}
+
+static int check_cross(const VsaCross* a, bool backward, const char* what) {
+  VSA_REQUIRE(a, "%s: null pointer", what);
+  int rc = check_dtype(a->dtype);
+  if (rc) return rc;
+  VSA_REQUIRE(a->H >= 0 && a->Hkv >= 0 && (a->Hkv == 0 ? a->H == 0 : a->H % a->Hkv == 0), "%s: the query heads must be a multiple of the key heads", what);
+  VSA_REQUIRE(a->B >= 0 && a->Lq >= 0 && a->Lkv >= 0 && a->D >= 1, "%s: negative extent", what);
+  if (!cross_extents_fine(a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D))
+    return fail(VSA_ERR_UNSUPPORTED, "%s: head dims up to 256, batches and heads up to 65535, 2^30 tokens", what);
+  if (a->B == 0 || a->Hkv == 0) return VSA_OK;
+  const bool rows = a->H > 0 && a->Lq > 0, keys = a->Lkv > 0;
+  VSA_REQUIRE(!rows || (a->q && a->out && a->lse2), "%s: null pointer", what);
+  VSA_REQUIRE(!rows || !keys || (a->k && a->v), "%s: null pointer", what);
+  VSA_REQUIRE(!backward || !rows || (a->dout && a->dq && a->delta), "%s: null pointer", what);
+  VSA_REQUIRE(!backward || !keys || (a->dk && a->dv), "%s: null pointer", what);
+  VSA_REQUIRE(a->workspace || vsa_cross_workspace_bytes(backward, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype) == 0,
+              "%s: a workspace is needed", what);
+  VSA_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "%s: the workspace is not 16-byte aligned", what);
+  return VSA_OK;
+}
+
+int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* kv_lengths, uint32_t* key_bits, int64_t B, int64_t Lkv,
+                       void* stream) {
+  VSA_REQUIRE(B >= 0 && Lkv >= 0, "cross attention key mask: negative extent");
+  VSA_REQUIRE(B == 0 || Lkv == 0 || (mask && key_bits), "cross attention key mask: null pointer");
+  if (B > 65535 || Lkv > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention key mask: batches up to 65535, 2^30 keys");
+  return cross_key_bits(mask, mask_stride, kv_lengths, key_bits, B, Lkv, (cudaStream_t)stream);
+}
+
+int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) {
+  (void)a;
+  (void)backward;
+  return 0;
+}
+
+int vsa_cross_fwd(const VsaCross* a, void* stream) {
+  int rc = check_cross(a, false, "cross attention forward");
+  if (rc || a->B == 0 || a->H == 0 || a->Lq == 0) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  const int splits = a->Lkv == 0 ? 1 : cross_fwd_splits(a->B, a->H, a->Lq, a->Lkv, a->D, a->dtype);
+  float* part_out = (float*)a->workspace;
+  float* part_lse = part_out + (splits == 1 ? 0 : splits * a->B * a->H * a->Lq * a->D);
+  if ((rc = cross_fwd_generic(*a, splits, part_out, part_lse, st))) return rc;
+  return splits == 1 ? VSA_OK : cross_join(*a, splits, part_out, part_lse, st);
+}
+
+int vsa_cross_bwd(const VsaCross* a, void* stream) {
+  int rc = check_cross(a, true, "cross attention backward");
+  if (rc || a->B == 0 || a->Hkv == 0) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (a->Lq == 0 || a->H == 0) return a->Lkv == 0 ? VSA_OK : cross_sum(*a, 0, nullptr, st);       // no query: zeros
+  const int splits = a->Lkv == 0 ? 1 : cross_bwd_splits(a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype);
+  if ((rc = cross_bwd_generic(*a, splits, (float*)a->workspace, st))) return rc;
+  return splits == 1 ? VSA_OK : cross_sum(*a, splits, (const float*)a->workspace, st);
+}
+
 int vsa_rotary(const VsaRotary* a, void* stream) {
   VSA_REQUIRE(a, "rotary: null pointer");
   int rc = check_dtype(a->dtype);

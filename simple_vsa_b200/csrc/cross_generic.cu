@@ -1,0 +1,488 @@
+// Cross attention on CUDA cores: fp32, head dims up to 256 of any alignment, any strides.  Also the small kernels that both families of
+// cross attention share: the packed key mask, the join of a forward split over the keys, the sum of partial dK and dV.
+//
+// out_i = sum_j p_ij v_j with p_i the softmax of scale q_i.k_j over the live keys j of the sample; a row without one gets zeros.
+// Tiles of 64 query rows x 64 keys (32 x 32 above head dim 128), 256 threads, a 4 x 4 patch of scores each, everything in fp32 and one
+// rounding at the end.  Bound by the FP32 pipe and by shared-memory reads (a 16-byte read feeds 8 to 16 multiply-adds).
+#include "common.cuh"
+#include "kernels.h"
+
+namespace vsa {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T> __device__ __forceinline__ float to_f(T x) { return Elem<T>::to(x); }
+template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <typename T> __device__ __forceinline__ T from_f(float x) { return Elem<T>::from(x); }
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+
+// DP: head dim rounded up; KT: tile edge; P: patch edge
+template <int DP_>
+struct Tile {
+  static constexpr int DP = DP_, KT = DP_ > 128 ? 32 : 64, P = KT / 16, PITCH = DP_ + 4, SPITCH = KT + 4;
+  static constexpr int floats = KT * PITCH, score_floats = KT * SPITCH;
+};
+
+// Rows row0 .. of one (batch, head) slice, converted; rows from `rows` on, rows that `live` says no to and dims from D on are zeros.
+template <typename T, typename TL, typename LIVE>
+__device__ __forceinline__ void load_tile(float* sm, const T* __restrict__ g, long long stride, int D, bool vec, LIVE live) {
+  constexpr int C = TL::DP / 4;
+  for (int e = threadIdx.x; e < TL::KT * C; e += kThreads) {
+    const int r = e / C, c = (e % C) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live(r) && c < D) {
+      const T* p = g + r * stride + c;
+      if (sizeof(T) == 4 && vec) {
+        x = *reinterpret_cast<const float4*>(p);
+      } else {
+        x.x = to_f<T>(p[0]);
+        if (c + 1 < D) x.y = to_f<T>(p[1]);
+        if (c + 2 < D) x.z = to_f<T>(p[2]);
+        if (c + 3 < D) x.w = to_f<T>(p[3]);
+      }
+    }
+    *reinterpret_cast<float4*>(sm + r * TL::PITCH + c) = x;
+  }
+}
+
+// s[i][j] = a[P ty + i] . b[tx + 16 j], in pieces of 16 products (a chain of 16 + D/16 roundings instead of D)
+template <typename TL>
+__device__ __forceinline__ void scores(float (&s)[TL::P][TL::P], const float* a, const float* b, int tx, int ty) {
+#pragma unroll
+  for (int i = 0; i < TL::P; ++i)
+#pragma unroll
+    for (int j = 0; j < TL::P; ++j) s[i][j] = 0.f;
+#pragma unroll 1
+  for (int d0 = 0; d0 < TL::DP; d0 += 16) {
+    float t[TL::P][TL::P] = {};
+#pragma unroll
+    for (int d = d0; d < d0 + 16; d += 4) {
+      float4 x[TL::P], y[TL::P];
+#pragma unroll
+      for (int i = 0; i < TL::P; ++i) x[i] = *reinterpret_cast<const float4*>(a + (TL::P * ty + i) * TL::PITCH + d);
+#pragma unroll
+      for (int j = 0; j < TL::P; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * TL::PITCH + d);
+#pragma unroll
+      for (int i = 0; i < TL::P; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::P; ++j)
+          t[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, t[i][j]))));
+    }
+#pragma unroll
+    for (int i = 0; i < TL::P; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::P; ++j) s[i][j] += t[i][j];
+  }
+}
+
+// acc[i][4 h + e] += sum_n p[P ty + i][n] * b[n][64 h + 4 tx + e]
+template <typename TL>
+__device__ __forceinline__ void product(float (&acc)[TL::P][TL::DP / 16], const float* p, const float* b, int tx, int ty) {
+#pragma unroll 2
+  for (int n = 0; n < TL::KT; n += 4) {
+    float4 w[TL::P];
+#pragma unroll
+    for (int i = 0; i < TL::P; ++i) w[i] = *reinterpret_cast<const float4*>(p + (TL::P * ty + i) * TL::SPITCH + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int h = 0; h < TL::DP / 64; ++h) {
+        const float4 x = *reinterpret_cast<const float4*>(b + (n + e) * TL::PITCH + 64 * h + 4 * tx);
+#pragma unroll
+        for (int i = 0; i < TL::P; ++i) {
+          const float f = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+          acc[i][4 * h + 0] = fmaf(f, x.x, acc[i][4 * h + 0]);
+          acc[i][4 * h + 1] = fmaf(f, x.y, acc[i][4 * h + 1]);
+          acc[i][4 * h + 2] = fmaf(f, x.z, acc[i][4 * h + 2]);
+          acc[i][4 * h + 3] = fmaf(f, x.w, acc[i][4 * h + 3]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, typename TL>
+__device__ __forceinline__ void store_rows(T* __restrict__ g, long long stride, int D, int rows, const float (&acc)[TL::P][TL::DP / 16],
+                                           const float (&mul)[TL::P], int tx, int ty) {
+#pragma unroll
+  for (int i = 0; i < TL::P; ++i) {
+    const int r = TL::P * ty + i;
+    if (r >= rows) continue;
+#pragma unroll
+    for (int h = 0; h < TL::DP / 64; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 64 * h + 4 * tx + e;
+        if (d < D) g[r * stride + d] = from_f<T>(mul[i] == 0.f ? 0.f : acc[i][4 * h + e] * mul[i]);
+      }
+  }
+}
+
+__device__ __forceinline__ float lanes16_max(float x) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+__device__ __forceinline__ float lanes16_sum(float x) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+struct Ctx {                   // what a CTA knows about its sample's keys
+  int len;
+  const uint32_t* bits;
+  __device__ __forceinline__ bool live(int key) const { return key < len && (bits == nullptr || (bits[key >> 5] >> (key & 31) & 1u)); }
+};
+__device__ __forceinline__ Ctx keys_of(const VsaCross& a, int b) {
+  Ctx c;
+  c.len = cross_length(a, b);
+  c.bits = a.key_bits == nullptr ? nullptr : a.key_bits + (long long)b * cross_words(a.Lkv);
+  return c;
+}
+
+template <typename T> __device__ __forceinline__ const T* slice(const void* p, const int64_t (&st)[3], int b, int h) {
+  return (const T*)p + b * st[0] + h * st[1];
+}
+template <typename T> __device__ __forceinline__ T* slice(void* p, const int64_t (&st)[3], int b, int h) {
+  return (T*)p + b * st[0] + h * st[1];
+}
+
+// ---- forward: one tile of query rows, one range of key tiles ----------------------------------------------------
+template <typename T, typename TL>
+__global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __grid_constant__ VsaCross a, int splits, float* part_out, float* part_lse,
+                                                                     bool vec) {
+  extern __shared__ __align__(16) float sm[];
+  float *sq = sm, *sk = sq + TL::floats, *sv = sk + TL::floats, *ss = sv + TL::floats;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int split = blockIdx.x % splits, qt = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
+  const int row0 = qt * TL::KT, rows = (int)min((long long)TL::KT, (long long)a.Lq - row0);
+  const Ctx keys = keys_of(a, b);
+  const int tiles = (keys.len + TL::KT - 1) / TL::KT, per = (tiles + splits - 1) / splits;
+  const int t0 = split * per, t1 = min(tiles, t0 + per);
+  const float c = a.scale * kLog2e;
+  load_tile<T, TL>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, [&](int r) { return r < rows; });
+  float m[TL::P], l[TL::P], acc[TL::P][TL::DP / 16];
+#pragma unroll
+  for (int i = 0; i < TL::P; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < TL::DP / 16; ++d) acc[i][d] = 0.f;
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int k0 = t * TL::KT;
+    __syncthreads();
+    auto live = [&](int r) { return keys.live(k0 + r); };
+    load_tile<T, TL>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
+    load_tile<T, TL>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+    __syncthreads();
+    float s[TL::P][TL::P];
+    scores<TL>(s, sq, sk, tx, ty);
+    bool on[TL::P];
+#pragma unroll
+    for (int j = 0; j < TL::P; ++j) on[j] = live(tx + 16 * j);
+#pragma unroll
+    for (int i = 0; i < TL::P; ++i) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < TL::P; ++j)
+        if (on[j]) top = fmaxf(top, s[i][j] * c);
+      const float mn = fmaxf(m[i], lanes16_max(top)), shift = mn == -INFINITY ? 0.f : mn;
+      const float keep = exp2f(m[i] - shift);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < TL::P; ++j) {
+        const float p = on[j] ? exp2f(fmaf(s[i][j], c, -shift)) : 0.f;
+        sum += p;
+        ss[(TL::P * ty + i) * TL::SPITCH + tx + 16 * j] = p;
+      }
+      l[i] = l[i] * keep + lanes16_sum(sum);
+      m[i] = mn;
+#pragma unroll
+      for (int d = 0; d < TL::DP / 16; ++d) acc[i][d] *= keep;
+    }
+    __syncthreads();
+    product<TL>(acc, ss, sv, tx, ty);
+  }
+  float mul[TL::P];
+#pragma unroll
+  for (int i = 0; i < TL::P; ++i) mul[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+  const long long bh = (long long)b * a.H + h, lp = cross_rows(a.Lq);
+  if (splits == 1) {
+    store_rows<T, TL>(slice<T>(a.out, a.out_stride, b, h) + row0 * a.out_stride[2], a.out_stride[2], a.D, rows, acc, mul, tx, ty);
+  } else {
+    const long long at = (split * (long long)a.B * a.H + bh) * a.Lq + row0;
+    store_rows<float, TL>(part_out + at * a.D, a.D, a.D, rows, acc, mul, tx, ty);
+  }
+  if (tx == 0) {
+#pragma unroll
+    for (int i = 0; i < TL::P; ++i) {
+      const int r = TL::P * ty + i;
+      const float lse = l[i] == 0.f ? (splits == 1 ? INFINITY : -INFINITY) : m[i] + log2f(l[i]);
+      if (splits > 1) {
+        if (r < rows) part_lse[(split * (long long)a.B * a.H + bh) * a.Lq + row0 + r] = lse;
+      } else if (row0 + r < lp) {
+        a.lse2[bh * lp + row0 + r] = r < rows ? lse : INFINITY;
+      }
+    }
+  }
+  if (splits == 1 && row0 + TL::KT >= a.Lq)
+    for (long long r = row0 + TL::KT + tid; r < lp; r += kThreads) a.lse2[bh * lp + r] = INFINITY;
+}
+
+// ---- backward: dQ (and delta) of one tile of query rows -----------------------------------------------------------
+template <typename T, typename TL>
+__global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid_constant__ VsaCross a, bool vec) {
+  extern __shared__ __align__(16) float sm[];
+  float *sq = sm, *sdo = sq + TL::floats, *sk = sdo + TL::floats, *sv = sk + TL::floats, *ss = sv + TL::floats;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int qt = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
+  const int row0 = qt * TL::KT, rows = (int)min((long long)TL::KT, (long long)a.Lq - row0);
+  const Ctx keys = keys_of(a, b);
+  const int tiles = (keys.len + TL::KT - 1) / TL::KT;
+  const float c = a.scale * kLog2e;
+  const long long bh = (long long)b * a.H + h, lp = cross_rows(a.Lq);
+  auto there = [&](int r) { return r < rows; };
+  load_tile<T, TL>(sk, slice<T>((const void*)a.out, a.out_stride, b, h) + row0 * a.out_stride[2], a.out_stride[2], a.D, vec, there);
+  load_tile<T, TL>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, there);
+  load_tile<T, TL>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
+  __syncthreads();
+  float lse[TL::P], delta[TL::P], acc[TL::P][TL::DP / 16], mul[TL::P];
+#pragma unroll
+  for (int i = 0; i < TL::P; ++i) {
+    const int r = TL::P * ty + i;
+    float d = 0.f;
+    for (int e = tx; e < TL::DP; e += 16) d = fmaf(sk[r * TL::PITCH + e], sdo[r * TL::PITCH + e], d);
+    delta[i] = lanes16_sum(d);
+    lse[i] = row0 + r < lp ? a.lse2[bh * lp + row0 + r] : INFINITY;
+    if (tx == 0 && row0 + r < lp) a.delta[bh * lp + row0 + r] = r < rows ? delta[i] : 0.f;
+    mul[i] = a.scale;
+#pragma unroll
+    for (int e = 0; e < TL::DP / 16; ++e) acc[i][e] = 0.f;
+  }
+  for (int t = 0; t < tiles; ++t) {
+    const int k0 = t * TL::KT;
+    __syncthreads();
+    auto live = [&](int r) { return keys.live(k0 + r); };
+    load_tile<T, TL>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
+    load_tile<T, TL>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+    __syncthreads();
+    float s[TL::P][TL::P], dp[TL::P][TL::P];
+    scores<TL>(s, sq, sk, tx, ty);
+    scores<TL>(dp, sdo, sv, tx, ty);
+#pragma unroll
+    for (int j = 0; j < TL::P; ++j) {
+      const bool on = live(tx + 16 * j);
+#pragma unroll
+      for (int i = 0; i < TL::P; ++i)
+        ss[(TL::P * ty + i) * TL::SPITCH + tx + 16 * j] = on ? exp2f(fmaf(s[i][j], c, -lse[i])) * (dp[i][j] - delta[i]) : 0.f;
+    }
+    __syncthreads();
+    product<TL>(acc, ss, sk, tx, ty);
+  }
+  if (row0 + TL::KT >= a.Lq)
+    for (long long r = row0 + TL::KT + tid; r < lp; r += kThreads) a.delta[bh * lp + r] = 0.f;
+  store_rows<T, TL>(slice<T>(a.dq, a.dq_stride, b, h) + row0 * a.dq_stride[2], a.dq_stride[2], a.D, rows, acc, mul, tx, ty);
+}
+
+// ---- backward: dK, dV of one tile of keys, one range of the query tiles of all heads that share them ------------------
+template <typename T, typename TL>
+__global__ void __launch_bounds__(kThreads) cross_dkdv_generic_kernel(const __grid_constant__ VsaCross a, int splits, float* part, bool vec) {
+  extern __shared__ __align__(16) float sm[];
+  float *sk = sm, *sv = sk + TL::floats, *sq = sv + TL::floats, *sdo = sq + TL::floats, *sp = sdo + TL::floats, *sds = sp + TL::score_floats;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int split = blockIdx.x % splits, kt = blockIdx.x / splits, hk = blockIdx.y, b = blockIdx.z, group = (int)(a.H / a.Hkv);
+  const int k0 = kt * TL::KT, krows = (int)min((long long)TL::KT, (long long)a.Lkv - k0);
+  const Ctx keys = keys_of(a, b);
+  const float c = a.scale * kLog2e;
+  auto live = [&](int r) { return keys.live(k0 + r); };
+  load_tile<T, TL>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
+  load_tile<T, TL>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+  float dk[TL::P][TL::DP / 16], dv[TL::P][TL::DP / 16], mul_k[TL::P], mul_v[TL::P];
+#pragma unroll
+  for (int i = 0; i < TL::P; ++i) {
+    const bool on = live(TL::P * ty + i);
+    mul_k[i] = on ? a.scale : 0.f;
+    mul_v[i] = on ? 1.f : 0.f;
+#pragma unroll
+    for (int e = 0; e < TL::DP / 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+  }
+  const int qtiles = (int)((a.Lq + TL::KT - 1) / TL::KT);
+  const long long total = (long long)qtiles * group, per = (total + splits - 1) / splits;
+  const long long t1 = k0 < keys.len ? min(total, (split + 1) * per) : 0, lp = cross_rows(a.Lq);
+  for (long long t = split * per; t < t1; ++t) {
+    const int h = hk * group + (int)(t / qtiles), row0 = (int)(t % qtiles) * TL::KT;
+    const int rows = (int)min((long long)TL::KT, (long long)a.Lq - row0);
+    const long long stat = ((long long)b * a.H + h) * lp + row0;
+    auto there = [&](int r) { return r < rows; };
+    __syncthreads();
+    load_tile<T, TL>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, there);
+    load_tile<T, TL>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
+    __syncthreads();
+    float s[TL::P][TL::P], dp[TL::P][TL::P];
+    scores<TL>(s, sk, sq, tx, ty);
+    scores<TL>(dp, sv, sdo, tx, ty);
+#pragma unroll
+    for (int j = 0; j < TL::P; ++j) {
+      const int r = tx + 16 * j;
+      const float lse = there(r) ? a.lse2[stat + r] : INFINITY, delta = there(r) ? a.delta[stat + r] : 0.f;
+#pragma unroll
+      for (int i = 0; i < TL::P; ++i) {
+        const int at = (TL::P * ty + i) * TL::SPITCH + r;
+        const float p = exp2f(fmaf(s[i][j], c, -lse));
+        sp[at] = p;
+        sds[at] = p * (dp[i][j] - delta);
+      }
+    }
+    __syncthreads();
+    product<TL>(dv, sp, sdo, tx, ty);
+    product<TL>(dk, sds, sq, tx, ty);
+  }
+  if (splits == 1) {
+    store_rows<T, TL>(slice<T>(a.dk, a.dk_stride, b, hk) + k0 * a.dk_stride[2], a.dk_stride[2], a.D, krows, dk, mul_k, tx, ty);
+    store_rows<T, TL>(slice<T>(a.dv, a.dv_stride, b, hk) + k0 * a.dv_stride[2], a.dv_stride[2], a.D, krows, dv, mul_v, tx, ty);
+  } else {
+    const long long one = (long long)a.B * a.Hkv * a.Lkv * a.D, at = (((long long)b * a.Hkv + hk) * a.Lkv + k0) * a.D;
+    store_rows<float, TL>(part + (2 * split) * one + at, a.D, a.D, krows, dk, mul_k, tx, ty);
+    store_rows<float, TL>(part + (2 * split + 1) * one + at, a.D, a.D, krows, dv, mul_v, tx, ty);
+  }
+}
+
+// ---- shared: joins and the key mask ------------------------------------------------------------------------------------
+// One warp per query row: the parts' weights are 2^(lse - max), their outputs already normalised.
+template <typename T>
+__global__ void __launch_bounds__(256) cross_join_kernel(const __grid_constant__ VsaCross a, int splits, const float* __restrict__ part_out,
+                                                         const float* __restrict__ part_lse) {
+  const long long rows = (long long)a.B * a.H * a.Lq, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), lp = cross_rows(a.Lq);
+  const int lane = threadIdx.x & 31;
+  if (row < rows) {
+    const long long bh = row / a.Lq, l = row - bh * a.Lq;
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + row]);
+    top = warp_max(top);
+    float sum = 0.f;
+    for (int s = lane; s < splits; s += 32) sum += top == -INFINITY ? 0.f : exp2f(part_lse[s * rows + row] - top);
+    sum = warp_sum(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = (T*)a.out + (bh / a.H) * a.out_stride[0] + (bh % a.H) * a.out_stride[1] + l * a.out_stride[2];
+    for (int d = lane; d < a.D; d += 32) {
+      float x = 0.f;
+      for (int s = 0; s < splits; ++s) {
+        const float ls = part_lse[s * rows + row];
+        // a part without a live key holds zeros; its weight is zero too
+        x = fmaf(top == -INFINITY ? 0.f : exp2f(ls - top), part_out[(s * rows + row) * a.D + d], x);
+      }
+      out[d] = from_f<T>(x * inv);
+    }
+    if (lane == 0) a.lse2[bh * lp + l] = top == -INFINITY ? INFINITY : top + log2f(sum);
+  }
+  // the padding behind each slice's rows, which the backward reads
+  const long long pad = lp - a.Lq, pads = (long long)a.B * a.H * pad, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long step = (long long)gridDim.x * 256;
+  for (long long i = at; i < pads; i += step) a.lse2[(i / pad) * lp + a.Lq + i % pad] = INFINITY;
+}
+
+// dK and dV: the parts are added in the order of the splits, whatever ran first.
+template <typename T>
+__global__ void __launch_bounds__(256) cross_sum_kernel(const __grid_constant__ VsaCross a, int splits, const float* __restrict__ part) {
+  const long long one = (long long)a.B * a.Hkv * a.Lkv * a.D;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < 2 * one; i += (long long)gridDim.x * 256) {
+    const bool is_v = i >= one;
+    const long long e = is_v ? i - one : i, row = e / a.D, bh = row / a.Lkv, l = row - bh * a.Lkv;
+    float x = 0.f;
+    for (int s = 0; s < splits; ++s) x += part[(2 * s + is_v) * one + e];
+    const int64_t(&st)[3] = is_v ? a.dv_stride : a.dk_stride;
+    ((T*)(is_v ? a.dv : a.dk))[(bh / a.Hkv) * st[0] + (bh % a.Hkv) * st[1] + l * st[2] + (e - row * a.D)] = from_f<T>(x);
+  }
+}
+
+__global__ void __launch_bounds__(256) cross_bits_kernel(const uint8_t* __restrict__ mask, long long stride, const int32_t* __restrict__ lengths,
+                                                         uint32_t* __restrict__ bits, long long Lkv, long long words) {
+  const int b = blockIdx.y;
+  const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), key = w * 32 + (threadIdx.x & 31);
+  if (w >= words) return;
+  long long len = Lkv;
+  if (lengths != nullptr) len = min(len, (long long)max(0, lengths[b]));
+  const unsigned word = __ballot_sync(0xffffffffu, key < len && mask[b * stride + key] != 0);
+  if ((threadIdx.x & 31) == 0) bits[b * words + w] = word;
+}
+
+bool vec4(const VsaCross& a, bool backward) {      // 16-byte reads of fp32 rows
+  if (a.dtype != VSA_F32 || a.D % 4) return false;
+  auto fine = [](const void* p, const int64_t (&s)[3]) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0;
+  };
+  return fine(a.q, a.q_stride) && fine(a.k, a.k_stride) && fine(a.v, a.v_stride) &&
+         (!backward || (fine(a.out, a.out_stride) && fine(a.dout, a.dout_stride)));
+}
+
+template <typename Kern>
+int reserve(Kern kern, int bytes, const char* what) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? VSA_OK : fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
+}
+
+template <typename T, typename TL>
+int fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
+  const int bytes = (3 * TL::floats + TL::score_floats) * 4;
+  int rc = reserve(cross_fwd_generic_kernel<T, TL>, bytes, "cross attention forward");
+  if (rc) return rc;
+  const int64_t tiles = (a.Lq + TL::KT - 1) / TL::KT;
+  cross_fwd_generic_kernel<T, TL><<<dim3((unsigned)(tiles * splits), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
+      a, splits, part_out, part_lse, vec4(a, false));
+  return check_launch("cross_fwd_generic_kernel");
+}
+template <typename T, typename TL>
+int bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  int bytes = (4 * TL::floats + TL::score_floats) * 4;
+  int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
+  if (rc) return rc;
+  cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::KT - 1) / TL::KT), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
+      a, vec4(a, true));
+  if ((rc = check_launch("cross_dq_generic_kernel"))) return rc;
+  if (a.Lkv == 0) return VSA_OK;
+  bytes = (4 * TL::floats + 2 * TL::score_floats) * 4;
+  if ((rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV"))) return rc;
+  cross_dkdv_generic_kernel<T, TL><<<dim3((unsigned)((a.Lkv + TL::KT - 1) / TL::KT * splits), (unsigned)a.Hkv, (unsigned)a.B), kThreads, bytes,
+                                     st>>>(a, splits, part, vec4(a, true));
+  return check_launch("cross_dkdv_generic_kernel");
+}
+
+}  // namespace
+
+#define VSA_CROSS_BY_DIM(T_, call_) (a.D <= 64 ? call_<T_, Tile<64>> : a.D <= 128 ? call_<T_, Tile<128>> : call_<T_, Tile<256>>)
+#define VSA_CROSS_BY_TYPE(call_) \
+  (a.dtype == VSA_F32 ? VSA_CROSS_BY_DIM(float, call_) : a.dtype == VSA_F16 ? VSA_CROSS_BY_DIM(__half, call_) : VSA_CROSS_BY_DIM(__nv_bfloat16, call_))
+
+int cross_generic_tile(int D) { return D > 128 ? 32 : 64; }
+
+int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
+  return VSA_CROSS_BY_TYPE(fwd)(a, splits, part_out, part_lse, st);
+}
+int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st) { return VSA_CROSS_BY_TYPE(bwd)(a, splits, part, st); }
+
+int cross_join(const VsaCross& a, int splits, const float* part_out, const float* part_lse, cudaStream_t st) {
+  const unsigned blocks = (unsigned)((a.B * a.H * a.Lq + 7) / 8);
+  if (a.dtype == VSA_F32) cross_join_kernel<float><<<blocks, 256, 0, st>>>(a, splits, part_out, part_lse);
+  else if (a.dtype == VSA_F16) cross_join_kernel<__half><<<blocks, 256, 0, st>>>(a, splits, part_out, part_lse);
+  else cross_join_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, splits, part_out, part_lse);
+  return check_launch("cross_join_kernel");
+}
+int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st) {
+  const int64_t n = 2 * a.B * a.Hkv * a.Lkv * a.D;
+  const unsigned blocks = (unsigned)(n / 256 + 1 < 148 * 8 ? n / 256 + 1 : 148 * 8);
+  if (a.dtype == VSA_F32) cross_sum_kernel<float><<<blocks, 256, 0, st>>>(a, splits, part);
+  else if (a.dtype == VSA_F16) cross_sum_kernel<__half><<<blocks, 256, 0, st>>>(a, splits, part);
+  else cross_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, splits, part);
+  return check_launch("cross_sum_kernel");
+}
+int cross_key_bits(const uint8_t* mask, int64_t stride, const int32_t* lengths, uint32_t* bits, int64_t B, int64_t Lkv, cudaStream_t st) {
+  const int64_t words = cross_words(Lkv);
+  if (B == 0 || words == 0) return VSA_OK;
+  cross_bits_kernel<<<dim3((unsigned)((words + 7) / 8), (unsigned)B), 256, 0, st>>>(mask, stride, lengths, bits, Lkv, words);
+  return check_launch("cross_bits_kernel");
+}
+
+}  // namespace vsa

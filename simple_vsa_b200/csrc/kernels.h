@@ -58,6 +58,31 @@ int sparse_dkdv_scalar(const void* dout, const void* q, const void* k, const voi
 // ---- rotary positions (rotary.cu) --------------------------------------------------------
 int rotary(const VsaRotary& a, cudaStream_t st);
 
+// ---- cross attention (cross_generic.cu) ---------------------------------------------------
+#ifdef __CUDACC__
+#define VSA_HD __host__ __device__ __forceinline__
+#else
+#define VSA_HD inline
+#endif
+// rows of lse2 and delta per slice; 32-bit words of a sample's packed key mask (whole tiles of 128 keys)
+VSA_HD int64_t cross_rows(int64_t Lq) { return (Lq + 127) / 128 * 128; }
+VSA_HD int64_t cross_words(int64_t Lkv) { return (Lkv + 127) / 128 * 4; }
+#ifdef __CUDACC__
+__device__ __forceinline__ int cross_length(const VsaCross& a, int b) {
+  if (a.kv_lengths == nullptr) return (int)a.Lkv;
+  const int n = a.kv_lengths[b];
+  return n < 0 ? 0 : n > a.Lkv ? (int)a.Lkv : n;
+}
+#endif
+int cross_generic_tile(int D);
+// splits > 1: partial outputs [splits][B*H][Lq][D] and statistics [splits][B*H][Lq] (-inf: no live key), for cross_join
+int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
+// splits > 1: partial dK and dV [splits][2][B*Hkv][Lkv][D], for cross_sum
+int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st);
+int cross_join(const VsaCross& a, int splits, const float* part_out, const float* part_lse, cudaStream_t st);
+int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st);
+int cross_key_bits(const uint8_t* mask, int64_t stride, const int32_t* lengths, uint32_t* bits, int64_t B, int64_t Lkv, cudaStream_t st);
+
 // ---- fp32 on 64 x 64 tiles, head dim 64 or 128, block volume 64, 128 or 256 (sparse_f32.cu) --------------------
 // operands: every tensor of the call that is read or written in 16-byte pieces
 bool sparse_f32_eligible(int D, int be, int dtype, int64_t BH, std::initializer_list<const void*> operands);
