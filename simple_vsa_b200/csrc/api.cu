@@ -648,8 +648,8 @@ static int cross_parts(int64_t units, int64_t steps, int64_t setup, int64_t most
   return best;
 }
 static int cross_fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  if (cross_umma_shape(D, dtype)) return cross_parts(B * H * ((Lq + 255) / 256), (Lkv + 127) / 128, 4, 64);
   const int tile = cross_generic_tile(D);
-  (void)dtype;
   return cross_parts(B * H * ((Lq + tile - 1) / tile), (Lkv + tile - 1) / tile, 2, 64);
 }
 static int cross_bwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
@@ -703,11 +703,9 @@ int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* 
   return cross_key_bits(mask, mask_stride, kv_lengths, key_bits, B, Lkv, (cudaStream_t)stream);
 }
 
-int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) {
-  (void)a;
-  (void)backward;
-  return 0;
-}
+static bool cross_on_umma(const VsaCross& a, bool backward) { return !scalar_forced() && !backward && cross_umma_eligible(a, backward); }
+
+int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) { return a != nullptr && cross_on_umma(*a, backward != 0) ? 1 : 0; }
 
 int vsa_cross_fwd(const VsaCross* a, void* stream) {
   int rc = check_cross(a, false, "cross attention forward");
@@ -716,7 +714,8 @@ int vsa_cross_fwd(const VsaCross* a, void* stream) {
   const int splits = a->Lkv == 0 ? 1 : cross_fwd_splits(a->B, a->H, a->Lq, a->Lkv, a->D, a->dtype);
   float* part_out = (float*)a->workspace;
   float* part_lse = part_out + (splits == 1 ? 0 : splits * a->B * a->H * a->Lq * a->D);
-  if ((rc = cross_fwd_generic(*a, splits, part_out, part_lse, st))) return rc;
+  rc = cross_on_umma(*a, false) ? cross_fwd_umma(*a, splits, part_out, part_lse, st) : cross_fwd_generic(*a, splits, part_out, part_lse, st);
+  if (rc) return rc;
   return splits == 1 ? VSA_OK : cross_join(*a, splits, part_out, part_lse, st);
 }
 

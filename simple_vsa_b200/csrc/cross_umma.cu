@@ -1,0 +1,518 @@
+// Cross attention on the Blackwell tensor path: bf16 and fp16, head dims that are multiples of 8 up to 128 (tiles of 64 or 128 dims, the
+// rest of a box lies outside the tensor and is zero-filled), any lengths, strides of multiples of 16 bytes read in place by TMA.
+//
+// Unlike the sparse kernels a query tile meets few key tiles (an encoder's states: four tiles of 128 at 512 keys), so set-up, first
+// loads and epilogue must not be paid per tile: the CTAs are persistent, and every role runs ahead of the others from one piece of
+// work to the next.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "umma.cuh"
+
+namespace vsa {
+namespace {
+
+using namespace umma;
+
+constexpr int kRows = 128;                 // rows of a tile: queries or keys
+constexpr int kHalf = kRows * 128;         // 64 head dims of a tile: 128 rows x 128 bytes
+constexpr uint32_t kTmemCols = 512;
+
+template <typename T> constexpr uint32_t kFmt = 1u;
+template <> constexpr uint32_t kFmt<__half> = 0u;
+
+#define CROSS_WAIT(bar_, parity_) warp_wait((bar_), (parity_), status)
+
+// D[128 x N] = A[128 x HD] B[N x HD]^T, both K-major; halves of 64 head dims kHalf / B_HALF bytes apart.
+template <typename T, int HD, int N, int B_HALF>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint32_t a_tile, uint32_t b_tile) {
+  constexpr uint32_t idesc = instr_desc(128, N, 0, 0, kFmt<T>);
+  constexpr uint32_t hi = desc_hi(1024);
+  const uint32_t a0 = desc_lo(a_tile, 16), b0 = desc_lo(b_tile, 16);
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks)
+    mma_ss(d_tmem, desc_pack(a0 + (uint32_t)(((ks >> 2) * kHalf + (ks & 3) * 32) >> 4), hi),
+           desc_pack(b0 + (uint32_t)(((ks >> 2) * B_HALF + (ks & 3) * 32) >> 4), hi), idesc, ks > 0 ? 1u : 0u);
+}
+// D[128 x HD] (+)= A[128 x ROWS] (tensor memory, 16-bit) B[ROWS x HD] (dims contiguous, TILE rows a half).  The A columns were written
+// by groups of GROUP scores each, every group packing its half-width result at the start of its own columns.
+template <typename T, int HD, int ROWS, int GROUP, int TILE>
+__device__ __forceinline__ void issue_product(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_tile, bool accumulate) {
+  constexpr uint32_t idesc = instr_desc(128, HD, 0, 1, kFmt<T>);
+  constexpr uint32_t hi = desc_hi(1024);
+  const uint32_t b0 = desc_lo(b_tile, TILE * 128);
+  const uint32_t acc0 = accumulate ? 1u : 0u;
+#pragma unroll
+  for (int ks = 0; ks < ROWS / 16; ++ks)
+    mma_ts(d_tmem, a_tmem + (uint32_t)((ks * 16 / GROUP) * GROUP + (ks * 16 % GROUP) / 2), desc_pack(b0 + (uint32_t)(ks * 128), hi), idesc,
+           ks > 0 ? 1u : acc0);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const uint32_t* r) {
+  return make_uint4(Elem<T>::pack(__uint_as_float(r[0]), __uint_as_float(r[1])), Elem<T>::pack(__uint_as_float(r[2]), __uint_as_float(r[3])),
+                    Elem<T>::pack(__uint_as_float(r[4]), __uint_as_float(r[5])), Elem<T>::pack(__uint_as_float(r[6]), __uint_as_float(r[7])));
+}
+// HD/64 boxes of rows x 64 dims of one (batch, head) slice on one barrier, whose bytes the caller has announced
+template <int HD>
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, int batch, uint32_t half_bytes, uint32_t bar) {
+#pragma unroll
+  for (int h = 0; h < HD / 64; ++h) tma_load_4d(dst + h * half_bytes, map, h * 64, row, head, batch, bar);
+}
+
+// Live keys of tile j of a sample: a bit each.
+struct TileKeys {
+  uint32_t w[4];
+  __device__ __forceinline__ bool full() const { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
+  __device__ __forceinline__ bool bit(int key) const {
+    const uint32_t x = key < 64 ? (key < 32 ? w[0] : w[1]) : (key < 96 ? w[2] : w[3]);
+    return x >> (key & 31) & 1u;
+  }
+};
+__device__ __forceinline__ TileKeys tile_keys(const VsaCross& a, int b, int len, int j) {
+  TileKeys t;
+  if (a.key_bits != nullptr) {
+    const uint4 x = *reinterpret_cast<const uint4*>(a.key_bits + (long long)b * cross_words(a.Lkv) + j * 4);
+    t.w[0] = x.x, t.w[1] = x.y, t.w[2] = x.z, t.w[3] = x.w;
+  } else {
+    const int left = len - j * kRows;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = left - 32 * i;
+      t.w[i] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+    }
+  }
+  return t;
+}
+
+// ------------------------------------------------------------------------------------------------------
+// forward
+// ------------------------------------------------------------------------------------------------------
+// A piece of work is 256 query rows of one head (two tiles of 128, which are the M dimension) against the key tiles of one split.  Both
+// tiles take every K and V tile from the same buffers; a softmax group of four warps owns a tile, a thread owns a row, and while one
+// group exponentiates the tensor cores form the other tile's products.  P goes over the scores it came from in tensor memory.
+// Per 128 x 128 scores at D = 128: 1024 tensor cycles, 1024 cycles of exponentials, 128 KB of shared-memory traffic at 128 B/clk.
+// The tensor cores run the MMAs of a CTA in the order of their issue: S(j+1) of a tile is issued behind its O += P(j) V(j) and
+// overwrites that P after it has been read.
+// The softmax keeps a running maximum, but moves the accumulated row only when the maximum has grown by more than 2^8: P stays below
+// 2^8 (fp16 holds 2^16, the sums are fp32), and moving O through registers is rare.
+constexpr int kFwdThreads = 384;
+template <int HD>
+struct FwdSmem {
+  static constexpr uint32_t tile = HD * 256;                      // 128 rows
+  static constexpr int stages = HD == 128 ? 4 : 8;                // K and V tiles in turn
+  static constexpr uint32_t q = 0;                                // two tiles
+  static constexpr uint32_t kv = q + 2 * tile;
+  static constexpr uint32_t stage = kv + stages * tile;           // 32 rows x 128 bytes a softmax warp
+  static constexpr uint32_t bars = stage + 8 * 4096;
+  static constexpr uint32_t misc = bars + 40 * 8;
+  static constexpr uint32_t total = misc + 16;
+};
+static_assert(FwdSmem<128>::total <= 232448 && FwdSmem<64>::total <= 232448, "shared memory of the cross attention forward");
+enum FwdBar { F_Q_FULL = 0, F_Q_EMPTY = 2, F_S_FULL = 4, F_P_FULL = 6, F_P2_FULL = 8, F_O_FULL = 10, F_KV_FULL = 12, F_KV_EMPTY = 20 };
+
+struct FwdWork {
+  int pairs, splits, items;       // pairs of query tiles per head, splits of the keys, all pieces
+  float *part_out, *part_lse;
+};
+struct FwdItem {
+  int b, h, row0, tiles, len, j0, j1, split;    // tiles: 1 or 2 live query tiles; key tiles j0 .. j1
+  __device__ __forceinline__ FwdItem(const VsaCross& a, const FwdWork& w, int item) {
+    const int rest = item / w.splits, bh = rest / w.pairs;
+    split = item - rest * w.splits;
+    b = bh / (int)a.H;
+    h = bh - b * (int)a.H;
+    row0 = (rest - bh * w.pairs) * 2 * kRows;
+    tiles = row0 + kRows < a.Lq ? 2 : 1;
+    len = cross_length(a, b);
+    const int n = (len + kRows - 1) / kRows, per = (n + w.splits - 1) / w.splits;
+    j0 = split * per;
+    j1 = min(n, j0 + per);
+  }
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ VsaCross a, const FwdWork w, int* status) {
+  using Sm = FwdSmem<HD>;
+  extern __shared__ __align__(1024) uint8_t cross_smem[];
+  if (*(volatile int*)status != 0) return;
+  uint8_t* sm = cross_smem;
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {                              // the operand layouts need it
+    if (threadIdx.x == 0) atomicCAS(status, 0, 70);
+    return;
+  }
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sm + Sm::misc);
+  auto bar = [&](int i) -> uint32_t { return base + Sm::bars + 8u * i; };
+  if (tid == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(bar(F_Q_FULL + t), 1);
+      mbar_init(bar(F_Q_EMPTY + t), 1);
+      mbar_init(bar(F_S_FULL + t), 1);
+      mbar_init(bar(F_P_FULL + t), 4);
+      mbar_init(bar(F_P2_FULL + t), 4);
+      mbar_init(bar(F_O_FULL + t), 1);
+    }
+    for (int i = 0; i < Sm::stages; ++i) {
+      mbar_init(bar(F_KV_FULL + i), 1);
+      mbar_init(bar(F_KV_EMPTY + i), 1);
+    }
+    fence_barrier_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == 2) {
+    tmem_alloc(base + Sm::misc, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+  const uint32_t tmem_o = tmem + 256;              // S of the two tiles, then O of the two tiles
+  const int group_heads = (int)(a.H / a.Hkv);
+  bool ok = true;
+
+  if (warp >= 4) {                                 // 2 x 208 + 80 registers are within the three groups' 168 at launch
+    registers_inc<208>();
+    const int quarter = warp & 3, t = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + 128 * t + lane_addr, o_addr = tmem_o + HD * t + lane_addr;
+    const float c = a.scale * kLog2e, c_abs = fabsf(c);
+    uint32_t s_uses = 0, o_uses = 0, steps = 0;    // phases of this tile's barriers; K/V pairs so far
+    for (int item = blockIdx.x; item < w.items && ok; item += gridDim.x) {
+      const FwdItem it(a, w, item);
+      if (t >= it.tiles) {
+        if (it.j1 > it.j0) steps += it.j1 - it.j0;
+        continue;
+      }
+      float m = -INFINITY;
+      float2 lsum = make_float2(0.f, 0.f);
+      for (int j = it.j0; j < it.j1; ++j, ++steps) {
+        const TileKeys keys = tile_keys(a, it.b, it.len, j);
+        const bool full = keys.full();
+        ok = CROSS_WAIT(bar(F_S_FULL + t), s_uses & 1);
+        if (!ok) break;
+        ++s_uses;
+        tc_fence_after();
+        uint32_t sv[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld(s_addr + 32 * i, sv[i]);
+        tmem_ld_wait();
+        float top;
+        {
+          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (full && c >= 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) x[q] = fmaxf(x[q], __uint_as_float(sv[q][i]));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float s = c >= 0.f ? __uint_as_float(sv[q][i]) : -__uint_as_float(sv[q][i]);
+                x[q] = fmaxf(x[q], keys.w[q] >> i & 1u ? s : -INFINITY);
+              }
+          }
+          top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          top = top == -INFINITY ? top : top * c_abs;
+        }
+        if (j == it.j0) {
+          m = top;
+        } else {
+          const bool up = top > m + 8.f;
+          if (__any_sync(0xffffffffu, up)) {       // O holds P V of every tile before this one: S came behind it in the pipe
+            const float keep = up ? fast_exp2(m - top) : 1.f;
+            if (up) m = top;
+            lsum = mul2(lsum, make_float2(keep, keep));
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 16) {
+              uint32_t ov[16];
+              tmem_ld(o_addr + d, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * keep);
+              tmem_st(o_addr + d, ov);
+            }
+          }
+        }
+        if (!full && t == 0) {                     // rows of V that no key takes part with meet P = 0: they must be finite
+          const uint32_t r = 2 * steps + 1, s = r % Sm::stages;
+          ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1);
+          if (!ok) break;
+          if (!keys.bit(row)) {
+            uint8_t* vrow = sm + Sm::kv + s * Sm::tile + row * 128;
+#pragma unroll
+            for (int ch = 0; ch < HD / 8; ++ch)
+              *reinterpret_cast<uint4*>(vrow + (ch >> 3) * kHalf + ((ch ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        const float shift = m == -INFINITY ? 0.f : m;
+        const float2 c2 = make_float2(c, c), m2 = make_float2(-shift, -shift);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = fma2(word_pair(sv[q] + 2 * i), c2, m2);
+            float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            if (!full) {                           // what stands in a key that takes no part may be anything: select
+              if (!(keys.w[q] >> (2 * i) & 1u)) e.x = 0.f;
+              if (!(keys.w[q] >> (2 * i + 1) & 1u)) e.y = 0.f;
+            }
+            lsum = add2(lsum, e);
+            pk[i] = Elem<T>::pack(e.x, e.y);
+          }
+          tmem_st(s_addr + 16 * q, pk);
+          if (q & 1) {                             // the product of the first 64 keys starts under the others
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar((q == 1 ? F_P_FULL : F_P2_FULL) + t));
+          }
+        }
+      }
+      if (!ok) break;
+      const float l = lsum.x + lsum.y, inv = l == 0.f ? 0.f : 1.f / l;
+      const bool any = it.j1 > it.j0;
+      if (any) {
+        ok = CROSS_WAIT(bar(F_O_FULL + t), o_uses & 1);
+        if (!ok) break;
+        ++o_uses;
+        tc_fence_after();
+      }
+      const int row_w = it.row0 + t * kRows + quarter * 32;         // first row of this warp
+      const long long bh = (long long)it.b * a.H + it.h;
+      if (w.splits == 1) {
+        a.lse2[bh * cross_rows(a.Lq) + row_w + lane] = l == 0.f || row_w + lane >= a.Lq ? INFINITY : m + log2f(l);
+        T* out = (T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1];
+        uint8_t* stage = sm + Sm::stage + (warp - 4) * 4096;
+#pragma unroll
+        for (int hh = 0; hh < HD / 64; ++hh) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t ov[32];
+            if (any) {
+              tmem_ld(o_addr + hh * 64 + half * 32, ov);
+              tmem_ld_wait();
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] = any ? __float_as_uint(__uint_as_float(ov[i]) * inv) : 0u;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * half + q) ^ (lane & 7)) << 4)) = pack8<T>(ov + 8 * q);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3), ch = lane & 7, d = hh * 64 + ch * 8;
+            if (row_w + r < a.Lq && d < a.D)
+              *reinterpret_cast<uint4*>(out + (row_w + r) * a.out_stride[2] + d) =
+                  *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+          }
+          __syncwarp();
+        }
+      } else {
+        const long long at = (it.split * (long long)a.B * a.H + bh) * a.Lq + row_w + lane;
+        const bool there = row_w + lane < a.Lq;
+        if (there) w.part_lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+#pragma unroll
+        for (int d = 0; d < HD; d += 32) {
+          uint32_t ov[32];
+          if (any) {
+            tmem_ld(o_addr + d, ov);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            if (there && d + i < a.D)
+              *reinterpret_cast<float4*>(w.part_out + at * a.D + d + i) =
+                  any ? make_float4(__uint_as_float(ov[i]) * inv, __uint_as_float(ov[i + 1]) * inv, __uint_as_float(ov[i + 2]) * inv,
+                                    __uint_as_float(ov[i + 3]) * inv)
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 71);
+  } else {
+    registers_dec<80>();
+    if (warp == 0) {
+      uint32_t q_phase = 3, r = 0;                 // a bit per tile
+      auto load_q = [&](const FwdItem& it, int t) {
+        ok = CROSS_WAIT(bar(F_Q_EMPTY + t), q_phase >> t & 1);
+        if (!ok) return;
+        q_phase ^= 1u << t;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(F_Q_FULL + t), Sm::tile);
+          load_rows<HD>(base + Sm::q + t * Sm::tile, &map_q, it.row0 + t * kRows, it.h, it.b, kHalf, bar(F_Q_FULL + t));
+        }
+        __syncwarp();
+      };
+      auto load_kv = [&](const FwdItem& it, const CUtensorMap* map, int j) {
+        const uint32_t s = r % Sm::stages;
+        ok = CROSS_WAIT(bar(F_KV_EMPTY + s), ((r / Sm::stages) & 1) ^ 1);
+        if (!ok) return;
+        ++r;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(F_KV_FULL + s), Sm::tile);
+          load_rows<HD>(base + Sm::kv + s * Sm::tile, map, j * kRows, it.h / group_heads, it.b, kHalf, bar(F_KV_FULL + s));
+        }
+        __syncwarp();
+      };
+      for (int item = blockIdx.x; item < w.items && ok; item += gridDim.x) {
+        const FwdItem it(a, w, item);
+        if (it.j1 <= it.j0) continue;
+        load_q(it, 0);
+        for (int j = it.j0; j < it.j1 && ok; ++j) {
+          load_kv(it, &map_k, j);
+          if (j == it.j0 && it.tiles == 2 && ok) load_q(it, 1);
+          if (ok) load_kv(it, &map_v, j);
+        }
+      }
+      if (!ok && lane == 0) atomicCAS(status, 0, 72);
+    } else if (warp == 1) {
+      // step n: key tile j of a piece, K in buffer 2n and V in buffer 2n+1 of the ring
+      struct Cursor {
+        int item, tiles, j, j0, j1;
+      };
+      auto settle = [&](Cursor& x) {               // the first piece from x.item on that has a key tile
+        for (; x.item < w.items; x.item += gridDim.x) {
+          const FwdItem it(a, w, x.item);
+          if (it.j1 > it.j0) {
+            x.tiles = it.tiles;
+            x.j = x.j0 = it.j0;
+            x.j1 = it.j1;
+            return;
+          }
+        }
+      };
+      uint32_t q_phase = 0, p_phase = 0;           // a bit per tile
+      auto issue_s = [&](const Cursor& x, uint32_t n, int t) {
+        const uint32_t r = 2 * n, s = r % Sm::stages;
+        if (x.j == x.j0) {
+          ok = CROSS_WAIT(bar(F_Q_FULL + t), q_phase >> t & 1);
+          if (!ok) return;
+          q_phase ^= 1u << t;
+        }
+        ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_scores<T, HD, 128, kHalf>(tmem + 128 * t, base + Sm::q + t * Sm::tile, base + Sm::kv + s * Sm::tile);
+          mma_commit(bar(F_S_FULL + t));
+          if (x.j == x.j1 - 1) mma_commit(bar(F_Q_EMPTY + t));
+          if (t == x.tiles - 1) mma_commit(bar(F_KV_EMPTY + s));
+        }
+        __syncwarp();
+      };
+      Cursor next{(int)blockIdx.x, 0, 0, 0, 0};
+      settle(next);
+      if (next.item < w.items)
+        for (int t = 0; t < next.tiles && ok; ++t) issue_s(next, 0, t);
+      for (uint32_t n = 0; ok && next.item < w.items; ++n) {
+        const Cursor cur = next;
+        if (++next.j == next.j1) {
+          next.item += gridDim.x;
+          settle(next);
+        }
+        const bool more = next.item < w.items;
+        const uint32_t r = 2 * n + 1, s = r % Sm::stages;
+        const uint32_t v_tile = base + Sm::kv + s * Sm::tile;
+#pragma unroll 1
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (t < cur.tiles) {
+            ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1) && CROSS_WAIT(bar(F_P_FULL + t), p_phase >> t & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one())
+              issue_product<T, HD, 64, 128, 128>(tmem_o + HD * t, tmem + 128 * t, v_tile, cur.j > cur.j0);
+            __syncwarp();
+            ok = CROSS_WAIT(bar(F_P2_FULL + t), p_phase >> t & 1);
+            if (!ok) break;
+            p_phase ^= 1u << t;
+            tc_fence_after();
+            if (elect_one()) {
+              issue_product<T, HD, 64, 128, 128>(tmem_o + HD * t, tmem + 128 * t + 32, v_tile + 64 * 128, true);
+              if (cur.j == cur.j1 - 1) mma_commit(bar(F_O_FULL + t));
+              if (t == cur.tiles - 1) mma_commit(bar(F_KV_EMPTY + s));
+            }
+            __syncwarp();
+          }
+          if (more && t < next.tiles) issue_s(next, n + 1, t);
+        }
+      }
+      if (!ok && lane == 0) atomicCAS(status, 0, 73);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------
+template <typename Kern>
+int reserve(Kern kern, int bytes, const char* what) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? VSA_OK : fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
+}
+
+int map_of(CUtensorMap* map, const VsaCross& a, const void* p, const int64_t (&stride)[3], int64_t heads, int64_t rows, int box, const char* what) {
+  return make_map_rows(map, a.dtype == VSA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, a.D, rows, heads, a.B,
+                       stride[2], stride[1], stride[0], box, what);
+}
+
+template <typename T, int HD>
+int launch_fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  int rc, *status;
+  if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention forward (q)"))) return rc;
+  if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (k)"))) return rc;
+  if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (v)"))) return rc;
+  if ((rc = device_status_word(&status))) return rc;
+  if ((rc = reserve(cross_fwd_umma_kernel<T, HD>, FwdSmem<HD>::total, "cross attention forward"))) return rc;
+  const int64_t pairs = (a.Lq + 2 * kRows - 1) / (2 * kRows), items = a.B * a.H * pairs * splits;
+  if (items > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention forward: too many query rows");
+  const FwdWork w{(int)pairs, splits, (int)items, part_out, part_lse};
+  const int64_t sms = device_sms();
+  cross_fwd_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kFwdThreads, FwdSmem<HD>::total, st>>>(mq, mk, mv, a, w, status);
+  return check_launch("cross_fwd_umma_kernel");
+}
+
+bool aligned(const void* p, const int64_t (&s)[3], int64_t heads, int64_t rows, int64_t batch) {
+  const int64_t n[3] = {batch, heads, rows};
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] <= 0 || s[i] % 8 || s[i] >= (1LL << 38))) return false;
+  return true;
+}
+
+}  // namespace
+
+bool cross_umma_shape(int D, int dtype) { return (dtype == VSA_BF16 || dtype == VSA_F16) && D % 8 == 0 && D >= 8 && D <= 128; }
+
+bool cross_umma_eligible(const VsaCross& a, bool backward) {
+  if (!cross_umma_shape(a.D, a.dtype) || a.Lkv < 1 || a.Lq < 1) return false;
+  if (!aligned(a.q, a.q_stride, a.H, a.Lq, a.B) || !aligned(a.k, a.k_stride, a.Hkv, a.Lkv, a.B) || !aligned(a.v, a.v_stride, a.Hkv, a.Lkv, a.B) ||
+      !aligned(a.out, a.out_stride, a.H, a.Lq, a.B))
+    return false;
+  return !backward || (aligned(a.dout, a.dout_stride, a.H, a.Lq, a.B) && aligned(a.dq, a.dq_stride, a.H, a.Lq, a.B) &&
+                       aligned(a.dk, a.dk_stride, a.Hkv, a.Lkv, a.B) && aligned(a.dv, a.dv_stride, a.Hkv, a.Lkv, a.B));
+}
+
+int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
+  if (a.dtype == VSA_F16)
+    return a.D <= 64 ? launch_fwd<__half, 64>(a, splits, part_out, part_lse, st) : launch_fwd<__half, 128>(a, splits, part_out, part_lse, st);
+  return a.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(a, splits, part_out, part_lse, st)
+                   : launch_fwd<__nv_bfloat16, 128>(a, splits, part_out, part_lse, st);
+}
+
+}  // namespace vsa

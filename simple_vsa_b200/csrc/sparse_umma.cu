@@ -424,6 +424,37 @@ int wait_timeout_selftest(unsigned long long limit_ns, int* gave_up, cudaStream_
   return check_launch("wait_timeout_selftest_kernel");
 }
 
+int make_map_rows(CUtensorMap* map, CUtensorMapDataType elem, const void* ptr, int64_t dim, int64_t rows, int64_t heads, int64_t batch,
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(VSA_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled is not available from the driver", what);
+  if (reinterpret_cast<uintptr_t>(ptr) % 16) return fail(VSA_ERR_BAD_ARGUMENT, "%s: pointer is not 16-byte aligned", what);
+  // the stride of an extent of one is never used, but has to be a legal one
+  const int64_t n[3] = {rows, heads, batch}, step[3] = {row_stride, head_stride, batch_stride};
+  cuuint64_t gstride[3];
+  for (int i = 0; i < 3; ++i) {
+    const int64_t s = n[i] > 1 ? step[i] : (dim + 7) / 8 * 8;
+    if (s <= 0 || s % 8) return fail(VSA_ERR_BAD_ARGUMENT, "%s: strides are not positive multiples of 16 bytes", what);
+    gstride[i] = (cuuint64_t)s * 2;
+  }
+  const cuuint64_t gdim[4] = {(cuuint64_t)dim, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, elem, 4, const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VSA_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed with code %d", what, (int)r);
+  return VSA_OK;
+}
+
+int device_status_word(int** word) {
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, g_device_status);
+  if (e != cudaSuccess) return fail(VSA_ERR_LAUNCH, "device status: %s", cudaGetErrorString(e));
+  *word = static_cast<int*>(p);
+  return VSA_OK;
+}
+
+int device_sms() { return sm_count(); }
+
 int device_status_fetch_and_clear(int* status) {
   int zero = 0;
   cudaError_t e = cudaMemcpyFromSymbol(status, g_device_status, sizeof(int));

@@ -7,6 +7,14 @@
 #include "common.cuh"
 
 namespace vsa {
+
+// Host side, sparse_umma.cu: a [batch, heads, rows, dim] operand of a 16-bit type with any strides (in elements, multiples of 8), boxes of
+// box_rows rows x 64 dims of one slice, 128-byte swizzle; the address of the status word on the current device.
+int make_map_rows(CUtensorMap* map, CUtensorMapDataType elem, const void* ptr, int64_t dim, int64_t rows, int64_t heads, int64_t batch,
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows, const char* what);
+int device_status_word(int** word);
+int device_sms();
+
 namespace umma {
 
 // ---- mbarrier --------------------------------------------------------------------------------
@@ -114,6 +122,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
