@@ -653,8 +653,9 @@ static int cross_fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D
   return cross_parts(B * H * ((Lq + tile - 1) / tile), (Lkv + tile - 1) / tile, 2, 64);
 }
 static int cross_bwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  // a step of the tensor path is 64 query rows; a CTA's set-up and epilogue and its share of the sum weigh about ten
+  if (cross_umma_shape(D, dtype)) return cross_parts(B * Hkv * ((Lkv + 127) / 128), (H / Hkv) * ((Lq + 63) / 64), 10, 64);
   const int tile = cross_generic_tile(D);
-  (void)dtype;
   return cross_parts(B * Hkv * ((Lkv + tile - 1) / tile), (H / Hkv) * ((Lq + tile - 1) / tile), 2, 64);
 }
 static bool cross_extents_fine(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D) {
@@ -703,7 +704,7 @@ int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* 
   return cross_key_bits(mask, mask_stride, kv_lengths, key_bits, B, Lkv, (cudaStream_t)stream);
 }
 
-static bool cross_on_umma(const VsaCross& a, bool backward) { return !scalar_forced() && !backward && cross_umma_eligible(a, backward); }
+static bool cross_on_umma(const VsaCross& a, bool backward) { return !scalar_forced() && cross_umma_eligible(a, backward); }
 
 int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) { return a != nullptr && cross_on_umma(*a, backward != 0) ? 1 : 0; }
 
@@ -725,7 +726,8 @@ int vsa_cross_bwd(const VsaCross* a, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   if (a->Lq == 0 || a->H == 0) return a->Lkv == 0 ? VSA_OK : cross_sum(*a, 0, nullptr, st);       // no query: zeros
   const int splits = a->Lkv == 0 ? 1 : cross_bwd_splits(a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype);
-  if ((rc = cross_bwd_generic(*a, splits, (float*)a->workspace, st))) return rc;
+  rc = cross_on_umma(*a, true) ? cross_bwd_umma(*a, splits, (float*)a->workspace, st) : cross_bwd_generic(*a, splits, (float*)a->workspace, st);
+  if (rc) return rc;
   return splits == 1 ? VSA_OK : cross_sum(*a, splits, (const float*)a->workspace, st);
 }
 

@@ -458,6 +458,637 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   if (warp == 2) tmem_dealloc(tmem, kTmemCols);
 }
 
+// ------------------------------------------------------------------------------------------------------
+// dQ (and delta)
+// ------------------------------------------------------------------------------------------------------
+// A piece of work is 128 query rows of one head: S = Q K^T, dP = dO V^T, dQ += dS K per key tile.  All sixteen elementwise warps
+// share a tile, 32 score columns a thread; S (later dS) in two accumulators, dP in one that is free again as soon as it has been read.
+// Per 128 x 128 scores at D = 128: 1536 tensor cycles, 1024 of exponentials.  delta = rowsum(out * dout) takes dout from its tile in
+// shared memory and out from registers that were filled while the piece before was finished.
+constexpr int kDqCols = 32;
+constexpr int kDqGroups = kRows / kDqCols;
+constexpr int kDqEwThreads = 128 * kDqGroups;
+constexpr int kDqThreads = 128 + kDqEwThreads;
+template <int HD>
+struct DqSmem {
+  static constexpr uint32_t tile = HD * 256;
+  static constexpr int k_stages = 3, v_stages = 2;
+  static constexpr uint32_t q = 0;
+  static constexpr uint32_t d_o = q + tile;
+  static constexpr uint32_t k = d_o + tile;
+  static constexpr uint32_t v = k + k_stages * tile;
+  static constexpr uint32_t delta = v + v_stages * tile;          // float [2][128]
+  static constexpr uint32_t bars = delta + 1024;
+  static constexpr uint32_t misc = bars + 32 * 8;
+  static constexpr uint32_t total = misc + 16;
+};
+static_assert(DqSmem<128>::total <= 232448, "shared memory of the cross attention dQ pass");
+enum DqBar { Q_QDO_FULL = 0, Q_QDO_EMPTY = 1, Q_K_FULL = 2, Q_K_EMPTY = 5, Q_V_FULL = 8, Q_V_EMPTY = 10, Q_S_FULL = 12, Q_S_EMPTY = 14,
+             Q_DP_FULL = 16, Q_DP_EMPTY = 17, Q_DS_FULL = 18, Q_ACC_FULL = 20 };
+
+struct DqItem {
+  int b, h, row0, len, n;                       // n key tiles
+  __device__ __forceinline__ DqItem(const VsaCross& a, int qtiles, int item) {
+    const int bh = item / qtiles;
+    row0 = (item - bh * qtiles) * kRows;
+    b = bh / (int)a.H;
+    h = bh - b * (int)a.H;
+    len = cross_length(a, b);
+    n = (len + kRows - 1) / kRows;
+  }
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kDqThreads, 1)
+cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ VsaCross a,
+                     int qtiles, int items, int* status) {
+  using Sm = DqSmem<HD>;
+  extern __shared__ __align__(1024) uint8_t cross_smem[];
+  if (*(volatile int*)status != 0) return;
+  uint8_t* sm = cross_smem;
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, 80);
+    return;
+  }
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sm + Sm::misc);
+  auto bar = [&](int i) -> uint32_t { return base + Sm::bars + 8u * i; };
+  if (tid == 0) {
+    mbar_init(bar(Q_QDO_FULL), 1);
+    mbar_init(bar(Q_QDO_EMPTY), 2 + 4 * kDqGroups);      // the last products that read them, and the warps that read dO
+    for (int i = 0; i < Sm::k_stages; ++i) {
+      mbar_init(bar(Q_K_FULL + i), 1);
+      mbar_init(bar(Q_K_EMPTY + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(Q_V_FULL + i), 1);
+      mbar_init(bar(Q_V_EMPTY + i), 1);
+      mbar_init(bar(Q_S_FULL + i), 1);
+      mbar_init(bar(Q_S_EMPTY + i), 1);
+      mbar_init(bar(Q_DS_FULL + i), 4 * kDqGroups);
+    }
+    mbar_init(bar(Q_DP_FULL), 1);
+    mbar_init(bar(Q_DP_EMPTY), 4 * kDqGroups);
+    mbar_init(bar(Q_ACC_FULL), 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_do);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(base + Sm::misc, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+  const uint32_t tmem_dp = tmem + 256, tmem_acc = tmem + 384;
+  const int group_heads = (int)(a.H / a.Hkv);
+  bool ok = true;
+  uint32_t n = 0, live_items = 0;                // key tiles and pieces (with a key tile) so far
+
+  if (warp == 0) {
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const DqItem it(a, qtiles, item);
+      if (it.n == 0) continue;
+      ok = CROSS_WAIT(bar(Q_QDO_EMPTY), (live_items & 1) ^ 1);
+      if (!ok) break;
+      ++live_items;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(bar(Q_QDO_FULL), 2 * Sm::tile);
+        load_rows<HD>(base + Sm::q, &map_q, it.row0, it.h, it.b, kHalf, bar(Q_QDO_FULL));
+        load_rows<HD>(base + Sm::d_o, &map_do, it.row0, it.h, it.b, kHalf, bar(Q_QDO_FULL));
+      }
+      __syncwarp();
+      const int hk = it.h / group_heads;
+      for (int j = 0; j < it.n; ++j, ++n) {
+        const uint32_t sk = n % Sm::k_stages, sv = n % Sm::v_stages;
+        ok = CROSS_WAIT(bar(Q_K_EMPTY + sk), ((n / Sm::k_stages) & 1) ^ 1);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(Q_K_FULL + sk), Sm::tile);
+          load_rows<HD>(base + Sm::k + sk * Sm::tile, &map_k, j * kRows, hk, it.b, kHalf, bar(Q_K_FULL + sk));
+        }
+        __syncwarp();
+        ok = CROSS_WAIT(bar(Q_V_EMPTY + sv), ((n / Sm::v_stages) & 1) ^ 1);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar(Q_V_FULL + sv), Sm::tile);
+          load_rows<HD>(base + Sm::v + sv * Sm::tile, &map_v, j * kRows, hk, it.b, kHalf, bar(Q_V_FULL + sv));
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 81);
+  } else if (warp == 2) {
+    // S = Q K^T
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const DqItem it(a, qtiles, item);
+      if (it.n == 0) continue;
+      ok = CROSS_WAIT(bar(Q_QDO_FULL), live_items & 1);
+      ++live_items;
+      for (int j = 0; j < it.n && ok; ++j, ++n) {
+        const uint32_t s = n % Sm::k_stages, b = n & 1;
+        ok = CROSS_WAIT(bar(Q_K_FULL + s), (n / Sm::k_stages) & 1) && CROSS_WAIT(bar(Q_S_EMPTY + b), ((n >> 1) & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_scores<T, HD, 128, kHalf>(tmem + b * 128, base + Sm::q, base + Sm::k + s * Sm::tile);
+          mma_commit(bar(Q_S_FULL + b));
+          if (j == it.n - 1) mma_commit(bar(Q_QDO_EMPTY));
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 82);
+  } else if (warp == 1) {
+    // dP = dO V^T
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const DqItem it(a, qtiles, item);
+      if (it.n == 0) continue;
+      ok = CROSS_WAIT(bar(Q_QDO_FULL), live_items & 1);
+      ++live_items;
+      for (int j = 0; j < it.n && ok; ++j, ++n) {
+        const uint32_t s = n % Sm::v_stages;
+        ok = CROSS_WAIT(bar(Q_V_FULL + s), (n / Sm::v_stages) & 1) && CROSS_WAIT(bar(Q_DP_EMPTY), (n & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_scores<T, HD, 128, kHalf>(tmem_dp, base + Sm::d_o, base + Sm::v + s * Sm::tile);
+          mma_commit(bar(Q_V_EMPTY + s));
+          mma_commit(bar(Q_DP_FULL));
+          if (j == it.n - 1) mma_commit(bar(Q_QDO_EMPTY));
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 83);
+  } else if (warp == 3) {
+    // dQ += dS K
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const DqItem it(a, qtiles, item);
+      for (int j = 0; j < it.n && ok; ++j, ++n) {
+        const uint32_t s = n % Sm::k_stages, b = n & 1;
+        ok = CROSS_WAIT(bar(Q_K_FULL + s), (n / Sm::k_stages) & 1) && CROSS_WAIT(bar(Q_DS_FULL + b), (n >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_product<T, HD, 128, kDqCols, 128>(tmem_acc, tmem + b * 128, base + Sm::k + s * Sm::tile, j > 0);
+          mma_commit(bar(Q_K_EMPTY + s));
+          mma_commit(bar(Q_S_EMPTY + b));
+          if (j == it.n - 1) mma_commit(bar(Q_ACC_FULL));
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 84);
+  } else {
+    const int quarter = warp & 3, cg = (warp - 4) >> 2, row = quarter * 32 + lane;
+    const int c0 = cg * kDqCols, st = tid - 128;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const float c = a.scale * kLog2e, log_scale = log2f(fabsf(a.scale));
+    const float2 c2 = make_float2(c, c);
+    const long long lp = cross_rows(a.Lq);
+    // delta: four neighbouring threads a row, HD/4 dims each
+    const int dr = st / kDqGroups, part = st % kDqGroups;
+    constexpr int kPieces = HD / kDqGroups / 8;                  // of 8 dims
+    uint4 out_r[kPieces];
+    float lse_r = 0.f;
+    auto fetch = [&](int item) {
+      const DqItem it(a, qtiles, item);
+      const T* o = (const T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1] + (long long)(it.row0 + dr) * a.out_stride[2];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int d = part * (HD / kDqGroups) + i * 8;
+        out_r[i] = it.row0 + dr < a.Lq && d < a.D ? *reinterpret_cast<const uint4*>(o + d) : make_uint4(0, 0, 0, 0);
+      }
+      lse_r = a.lse2[((long long)it.b * a.H + it.h) * lp + it.row0 + row];
+    };
+    if ((int)blockIdx.x < items) fetch(blockIdx.x);
+    uint32_t pieces = 0;                                         // all pieces so far, of which live_items have key tiles
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++pieces) {
+      const DqItem it(a, qtiles, item);
+      const long long bh = (long long)it.b * a.H + it.h;
+      T* dq = (T*)a.dq + it.b * a.dq_stride[0] + it.h * a.dq_stride[1] + (long long)(it.row0 + row) * a.dq_stride[2];
+      const bool there = it.row0 + row < a.Lq;
+      if (it.n == 0) {                                           // no key: zeros
+        if (part == 0) a.delta[bh * lp + it.row0 + dr] = 0.f;
+#pragma unroll
+        for (int d = c0; d < c0 + kDqCols; d += 8)
+          if (there && d < a.D) *reinterpret_cast<uint4*>(dq + d) = make_uint4(0, 0, 0, 0);
+        if (item + (int)gridDim.x < items) fetch(item + gridDim.x);
+        continue;
+      }
+      ok = CROSS_WAIT(bar(Q_QDO_FULL), live_items & 1);
+      if (!ok) break;
+      float* s_delta = reinterpret_cast<float*>(sm + Sm::delta) + (live_items & 1) * kRows;
+      {
+        float acc = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int ch = part * (HD / kDqGroups / 8) + i;        // 16-byte piece of the row
+          const uint4 x = *reinterpret_cast<const uint4*>(sm + Sm::d_o + (ch >> 3) * kHalf + dr * 128 + (((ch ^ dr) & 7) << 4));
+          const uint32_t *p = &out_r[i].x, *q = &x.x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 u = Elem<T>::unpack(p[e]), y = Elem<T>::unpack(q[e]);
+            acc = fmaf(u.x, y.x, fmaf(u.y, y.y, acc));
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < kDqGroups; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+        if (part == 0) {
+          s_delta[dr] = acc;
+          a.delta[bh * lp + it.row0 + dr] = acc;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Q_QDO_EMPTY));
+      named_barrier(1, kDqEwThreads);
+      const float dl = s_delta[row], neg_lse = log_scale - lse_r;        // 2^(s c - lse) * |scale| in one exponential
+      const float2 l2 = make_float2(neg_lse, neg_lse), d2 = make_float2(-dl, -dl);
+      for (int j = 0; j < it.n; ++j, ++n) {
+        const uint32_t b = n & 1;
+        const TileKeys keys = tile_keys(a, it.b, it.len, j);
+        ok = CROSS_WAIT(bar(Q_S_FULL + b), (n >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t s_addr = tmem + b * 128 + lane_addr + c0;
+        uint32_t sv[kDqCols];
+        tmem_ld(s_addr, sv);
+        tmem_ld_wait();
+        if (!keys.full() && cg == 0) {           // rows of K that no key takes part with meet dS = 0: they must be finite (S is done)
+          if (!keys.bit(row)) {
+            uint8_t* krow = sm + Sm::k + (n % Sm::k_stages) * Sm::tile + row * 128;
+#pragma unroll
+            for (int ch = 0; ch < HD / 8; ++ch)
+              *reinterpret_cast<uint4*>(krow + (ch >> 3) * kHalf + ((ch ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        float2 pf[kDqCols / 2];
+#pragma unroll
+        for (int i = 0; i < kDqCols / 2; ++i) {
+          const float2 x = fma2(word_pair(sv + 2 * i), c2, l2);
+          pf[i] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+        }
+        ok = CROSS_WAIT(bar(Q_DP_FULL), n & 1);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t dv[kDqCols];
+        tmem_ld(tmem_dp + lane_addr + c0, dv);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Q_DP_EMPTY));
+        uint32_t pk[kDqCols / 2];
+#pragma unroll
+        for (int i = 0; i < kDqCols / 2; ++i) {
+          const float2 y = mul2(pf[i], add2(word_pair(dv + 2 * i), d2));
+          pk[i] = Elem<T>::pack(y.x, y.y);
+        }
+        const uint32_t word = cg < 2 ? (cg == 0 ? keys.w[0] : keys.w[1]) : (cg == 2 ? keys.w[2] : keys.w[3]);
+        if (word != 0xffffffffu) {               // what stands in a key that takes no part may be anything
+#pragma unroll
+          for (int i = 0; i < kDqCols / 2; ++i)
+            pk[i] &= (word >> (2 * i) & 1u ? 0xffffu : 0u) | (word >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+        }
+        tmem_st(s_addr, pk);                     // over this thread's own scores
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Q_DS_FULL + b));
+      }
+      if (!ok) break;
+      if (item + (int)gridDim.x < items) fetch(item + gridDim.x);
+      ok = CROSS_WAIT(bar(Q_ACC_FULL), live_items & 1);
+      if (!ok) break;
+      ++live_items;
+      tc_fence_after();
+      if (c0 < HD) {
+        uint32_t av[32];
+        tmem_ld(tmem_acc + lane_addr + c0, av);
+        tmem_ld_wait();
+        if (a.scale < 0.f) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) av[i] ^= 0x80000000u;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+          if (there && c0 + i < a.D) *reinterpret_cast<uint4*>(dq + c0 + i) = pack8<T>(av + i);
+      }
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 85);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ------------------------------------------------------------------------------------------------------
+// dK / dV: lanes = 128 key rows, columns = 64 query rows of a streamed tile
+// ------------------------------------------------------------------------------------------------------
+// A CTA owns 128 keys of one key head and walks a range of the query tiles of all heads that share it; K and V stay in shared memory,
+// dK and dV in tensor memory.  S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q: 2560 tensor cycles per 128 x 128 scores.  The
+// range is cut so that the CTAs fill whole waves of SMs; parts are added by a kernel of their own, in the order of the cuts.
+constexpr int kQTile = 64;
+constexpr int kSlab = kQTile * 128;
+constexpr int kDkCols = 32;
+constexpr int kDkGroups = kQTile / kDkCols;
+constexpr int kDkEwThreads = 128 * kDkGroups;
+constexpr int kDkThreads = 128 + kDkEwThreads;
+template <int HD>
+struct DkSmem {
+  static constexpr uint32_t tile = HD * 256;          // 128 resident rows
+  static constexpr uint32_t part = HD * 128;          // 64 streamed rows
+  static constexpr int q_stages = 5, do_stages = 5;
+  static constexpr uint32_t k = 0;
+  static constexpr uint32_t v = k + tile;
+  static constexpr uint32_t q = v + tile;
+  static constexpr uint32_t d_o = q + q_stages * part;
+  static constexpr uint32_t stats = d_o + do_stages * part;       // per Q stage: lse [64], delta [64]
+  static constexpr uint32_t bars = stats + q_stages * 512;
+  static constexpr uint32_t misc = bars + 40 * 8;
+  static constexpr uint32_t total = misc + 16;
+};
+static_assert(DkSmem<128>::total <= 232448, "shared memory of the cross attention dK/dV pass");
+enum DkBar { K_KV_FULL = 0, K_Q_FULL = 1, K_Q_EMPTY = 6, K_DO_FULL = 11, K_DO_EMPTY = 16, K_S_FULL = 21, K_S_EMPTY = 23,
+             K_DP_FULL = 25, K_DP_EMPTY = 27, K_P_FULL = 29, K_DS_FULL = 31, K_ACC_FULL = 33 };
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kDkThreads, 1)
+cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ VsaCross a,
+                       int ktiles, int splits, float* part, int* status) {
+  using Sm = DkSmem<HD>;
+  extern __shared__ __align__(1024) uint8_t cross_smem[];
+  if (*(volatile int*)status != 0) return;
+  uint8_t* sm = cross_smem;
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, 90);
+    return;
+  }
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  // the parts of a key head's tiles lie next to each other in launch order: they stream the same query tiles
+  const int unit = blockIdx.x;
+  const int ktile = unit % ktiles, rest = unit / ktiles, split = rest % splits, bhk = rest / splits;
+  const int b = bhk / (int)a.Hkv, hk = bhk - b * (int)a.Hkv, group_heads = (int)(a.H / a.Hkv);
+  const int krow0 = ktile * kRows;
+  const TileKeys keys = tile_keys(a, b, cross_length(a, b), ktile);
+  const int qtiles = (int)((a.Lq + kQTile - 1) / kQTile);
+  const long long total = (long long)qtiles * group_heads, per = (total + splits - 1) / splits;
+  const long long first = split * per, last = first + per < total ? first + per : total;
+  const bool any = (keys.w[0] | keys.w[1] | keys.w[2] | keys.w[3]) != 0u;
+  const int n_tiles = any && last > first ? (int)(last - first) : 0;
+  const float c = a.scale * kLog2e;
+  const long long lp = cross_rows(a.Lq);
+  const long long one = (long long)a.B * a.Hkv * a.Lkv * a.D;      // values of a partial dK
+  const long long part_row = ((long long)bhk * a.Lkv + krow0) * a.D;
+
+  if (n_tiles == 0) {                             // no query, or no key that takes part: zeros
+    for (int i = tid; i < kRows * HD / 8; i += kDkThreads) {
+      const int r = i / (HD / 8), d = i % (HD / 8) * 8;
+      if (krow0 + r >= a.Lkv || d >= a.D) continue;
+      if (splits == 1) {
+        *reinterpret_cast<uint4*>((T*)a.dk + b * a.dk_stride[0] + hk * a.dk_stride[1] + (krow0 + r) * a.dk_stride[2] + d) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>((T*)a.dv + b * a.dv_stride[0] + hk * a.dv_stride[1] + (krow0 + r) * a.dv_stride[2] + d) = make_uint4(0, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float* p = part + (2 * split + x) * one + part_row + (long long)r * a.D + d;
+          reinterpret_cast<float4*>(p)[0] = reinterpret_cast<float4*>(p)[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+    }
+    return;
+  }
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(sm + Sm::misc);
+  auto bar = [&](int i) -> uint32_t { return base + Sm::bars + 8u * i; };
+  if (tid == 0) {
+    mbar_init(bar(K_KV_FULL), 1);
+    for (int i = 0; i < Sm::q_stages; ++i) {
+      mbar_init(bar(K_Q_FULL + i), 33);       // the TMA boxes' lane and 32 lanes' copies of the statistics
+      mbar_init(bar(K_Q_EMPTY + i), 1);
+    }
+    for (int i = 0; i < Sm::do_stages; ++i) {
+      mbar_init(bar(K_DO_FULL + i), 1);
+      mbar_init(bar(K_DO_EMPTY + i), 2);      // read by the dP products of one issuer and the dV products of the other
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(K_S_FULL + i), 1);
+      mbar_init(bar(K_S_EMPTY + i), 1);
+      mbar_init(bar(K_DP_FULL + i), 1);
+      mbar_init(bar(K_DP_EMPTY + i), 1);
+      mbar_init(bar(K_P_FULL + i), 4 * kDkGroups);
+      mbar_init(bar(K_DS_FULL + i), 4 * kDkGroups);
+    }
+    mbar_init(bar(K_ACC_FULL), 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_do);
+    mbar_arrive_expect_tx(bar(K_KV_FULL), 2 * Sm::tile);
+    load_rows<HD>(base + Sm::k, &map_k, krow0, hk, b, kHalf, bar(K_KV_FULL));
+    load_rows<HD>(base + Sm::v, &map_v, krow0, hk, b, kHalf, bar(K_KV_FULL));
+  }
+  if (warp == 1) {
+    tmem_alloc(base + Sm::misc, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+  // two buffers of (S^T 64 columns, dP^T 64 columns), P^T and dS^T packed over them; then dK and dV
+  const uint32_t tmem_dk = tmem + 256, tmem_dv = tmem + 384;
+  bool ok = true;
+
+  if (warp == 0) {       // dO tiles; Q tiles and the statistics of their rows
+    int g = (int)(first / qtiles), qt = (int)(first - (long long)g * qtiles);
+    for (int p = 0; p < n_tiles; ++p) {
+      const int sq = p % Sm::q_stages, sd = p % Sm::do_stages;
+      const int h = hk * group_heads + g, row0 = qt * kQTile;
+      ok = CROSS_WAIT(bar(K_Q_EMPTY + sq), ((p / Sm::q_stages) & 1) ^ 1) && CROSS_WAIT(bar(K_DO_EMPTY + sd), ((p / Sm::do_stages) & 1) ^ 1);
+      if (!ok) break;
+      const uint32_t st = base + Sm::stats + sq * 512 + lane * 4;
+      const long long stat = ((long long)b * a.H + h) * lp + row0 + lane;
+      cp_async4(st, a.lse2 + stat);
+      cp_async4(st + 128, a.lse2 + stat + 32);
+      cp_async4(st + 256, a.delta + stat);
+      cp_async4(st + 384, a.delta + stat + 32);
+      cp_async_arrive_noinc(bar(K_Q_FULL + sq));
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar(K_Q_FULL + sq), Sm::part);
+        load_rows<HD>(base + Sm::q + sq * Sm::part, &map_q, row0, h, b, kSlab, bar(K_Q_FULL + sq));
+        mbar_arrive_expect_tx(bar(K_DO_FULL + sd), Sm::part);
+        load_rows<HD>(base + Sm::d_o + sd * Sm::part, &map_do, row0, h, b, kSlab, bar(K_DO_FULL + sd));
+      }
+      if (++qt == qtiles) qt = 0, ++g;
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 91);
+  } else if (warp == 2) {
+    // S^T = K Q^T
+    ok = CROSS_WAIT(bar(K_KV_FULL), 0);
+    for (int p = 0; p < n_tiles && ok; ++p) {
+      const int s = p % Sm::q_stages, bf = p & 1;
+      ok = CROSS_WAIT(bar(K_Q_FULL + s), (p / Sm::q_stages) & 1) && CROSS_WAIT(bar(K_S_EMPTY + bf), ((p >> 1) & 1) ^ 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        issue_scores<T, HD, 64, kSlab>(tmem + bf * 128, base + Sm::k, base + Sm::q + s * Sm::part);
+        mma_commit(bar(K_S_FULL + bf));
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 92);
+  } else if (warp == 1) {
+    // dP^T = V dO^T
+    ok = CROSS_WAIT(bar(K_KV_FULL), 0);
+    for (int p = 0; p < n_tiles && ok; ++p) {
+      const int s = p % Sm::do_stages, bf = p & 1;
+      ok = CROSS_WAIT(bar(K_DO_FULL + s), (p / Sm::do_stages) & 1) && CROSS_WAIT(bar(K_DP_EMPTY + bf), ((p >> 1) & 1) ^ 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        issue_scores<T, HD, 64, kSlab>(tmem + bf * 128 + 64, base + Sm::v, base + Sm::d_o + s * Sm::part);
+        mma_commit(bar(K_DO_EMPTY + s));
+        mma_commit(bar(K_DP_FULL + bf));
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 93);
+  } else if (warp == 3) {
+    // dV += P^T dO, dK += dS^T Q
+    for (int p = 0; p < n_tiles && ok; ++p) {
+      const int sq = p % Sm::q_stages, sd = p % Sm::do_stages, bf = p & 1;
+      const uint32_t ph = (p >> 1) & 1;
+      ok = CROSS_WAIT(bar(K_DO_FULL + sd), (p / Sm::do_stages) & 1) && CROSS_WAIT(bar(K_P_FULL + bf), ph);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        issue_product<T, HD, 64, kDkCols, 64>(tmem_dv, tmem + bf * 128, base + Sm::d_o + sd * Sm::part, p > 0);
+        mma_commit(bar(K_DO_EMPTY + sd));
+        mma_commit(bar(K_S_EMPTY + bf));
+      }
+      __syncwarp();
+      ok = CROSS_WAIT(bar(K_DS_FULL + bf), ph);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        issue_product<T, HD, 64, kDkCols, 64>(tmem_dk, tmem + bf * 128 + 64, base + Sm::q + sq * Sm::part, p > 0);
+        mma_commit(bar(K_Q_EMPTY + sq));
+        mma_commit(bar(K_DP_EMPTY + bf));
+      }
+      __syncwarp();
+    }
+    if (ok && elect_one()) mma_commit(bar(K_ACC_FULL));
+    __syncwarp();
+    if (!ok && lane == 0) atomicCAS(status, 0, 94);
+  } else {
+    const int quarter = warp & 3, cg = (warp - 4) >> 2;
+    const int row = quarter * 32 + lane, c0 = cg * kDkCols, st = tid - 128;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const bool live = keys.bit(row);
+    const float2 c2 = make_float2(-c, -c), m1 = make_float2(-1.f, -1.f);
+    for (int p = 0; p < n_tiles && ok; ++p) {
+      const int bf = p & 1, sq = p % Sm::q_stages;
+      const uint32_t ph = (p >> 1) & 1;
+      ok = CROSS_WAIT(bar(K_S_FULL + bf), ph) && CROSS_WAIT(bar(K_Q_FULL + sq), (p / Sm::q_stages) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const float4* s_lse = reinterpret_cast<const float4*>(sm + Sm::stats + sq * 512 + c0 * 4);
+      const uint32_t s_addr = tmem + bf * 128 + lane_addr + c0;
+      uint32_t sv[kDkCols];
+      tmem_ld(s_addr, sv);
+      tmem_ld_wait();
+      float2 pf[kDkCols / 2];
+      uint32_t pk[kDkCols / 2];
+#pragma unroll
+      for (int i = 0; i < kDkCols / 4; ++i) {
+        const float4 l4 = s_lse[i];
+        // lse - S c, negated in the exponential: the packed operations have no sign of their own to spend on the statistics
+        const float2 x = fma2(word_pair(sv + 4 * i), c2, make_float2(l4.x, l4.y));
+        const float2 y = fma2(word_pair(sv + 4 * i + 2), c2, make_float2(l4.z, l4.w));
+        pf[2 * i] = make_float2(fast_exp2(-x.x), fast_exp2(-x.y));
+        pf[2 * i + 1] = make_float2(fast_exp2(-y.x), fast_exp2(-y.y));
+        // a key that takes no part: its scores come from whatever sits in K there
+        pk[2 * i] = live ? Elem<T>::pack(pf[2 * i].x, pf[2 * i].y) : 0u;
+        pk[2 * i + 1] = live ? Elem<T>::pack(pf[2 * i + 1].x, pf[2 * i + 1].y) : 0u;
+      }
+      tmem_st(s_addr, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(K_P_FULL + bf));
+      ok = CROSS_WAIT(bar(K_DP_FULL + bf), ph);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t dvv[kDkCols];
+      tmem_ld(s_addr + 64, dvv);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < kDkCols / 4; ++i) {
+        const float4 d4 = s_lse[16 + i];       // delta: 64 floats behind the statistics
+        const float2 x = mul2(pf[2 * i], fma2(word_pair(dvv + 4 * i), m1, make_float2(d4.x, d4.y)));      // -dS
+        const float2 y = mul2(pf[2 * i + 1], fma2(word_pair(dvv + 4 * i + 2), m1, make_float2(d4.z, d4.w)));
+        pk[2 * i] = live ? Elem<T>::pack(x.x, x.y) : 0u;
+        pk[2 * i + 1] = live ? Elem<T>::pack(y.x, y.y) : 0u;
+      }
+      tmem_st(s_addr + 64, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(K_DS_FULL + bf));
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 95);
+    if (ok) ok = CROSS_WAIT(bar(K_ACC_FULL), 0);
+    if (ok) {
+      tc_fence_after();
+      uint8_t* stage_k = sm + Sm::k;          // every MMA is done: dK over K, dV over V
+      uint8_t* stage_v = sm + Sm::v;
+      for (int j = cg; j < 2 * (HD / 32); j += kDkGroups) {
+        const bool is_k = j < HD / 32;
+        const int jj = is_k ? j : j - HD / 32;
+        uint32_t av[32];
+        tmem_ld((is_k ? tmem_dk : tmem_dv) + lane_addr + 32 * jj, av);
+        tmem_ld_wait();
+        const float mul = is_k ? -a.scale : 1.f;       // the products summed -dS
+#pragma unroll
+        for (int i = 0; i < 32; ++i) av[i] = live ? __float_as_uint(__uint_as_float(av[i]) * mul) : 0u;
+        if (splits == 1) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<uint4*>((is_k ? stage_k : stage_v) + row * (HD * 2) + (((4 * jj + q4) ^ (row & 7)) << 4)) = pack8<T>(av + 8 * q4);
+        } else if (krow0 + row < a.Lkv) {
+          float* dst = part + (2 * split + !is_k) * one + part_row + (long long)row * a.D + 32 * jj;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            if (32 * jj + i < a.D) *reinterpret_cast<uint4*>(dst + i) = make_uint4(av[i], av[i + 1], av[i + 2], av[i + 3]);
+        }
+      }
+      if (splits == 1) {
+        named_barrier(1, kDkEwThreads);
+        for (int i = st; i < kRows * HD / 8; i += kDkEwThreads) {
+          const int r = i / (HD / 8), ch = i % (HD / 8);
+          if (krow0 + r >= a.Lkv || ch * 8 >= a.D) continue;
+          const uint32_t off = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>((T*)a.dk + b * a.dk_stride[0] + hk * a.dk_stride[1] + (krow0 + r) * a.dk_stride[2] + ch * 8) =
+              *reinterpret_cast<const uint4*>(stage_k + off);
+          *reinterpret_cast<uint4*>((T*)a.dv + b * a.dv_stride[0] + hk * a.dv_stride[1] + (krow0 + r) * a.dv_stride[2] + ch * 8) =
+              *reinterpret_cast<const uint4*>(stage_v + off);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------
 template <typename Kern>
 int reserve(Kern kern, int bytes, const char* what) {
@@ -474,10 +1105,10 @@ template <typename T, int HD>
 int launch_fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   int rc, *status;
+  if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to a thread that has none yet
   if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention forward (q)"))) return rc;
   if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (k)"))) return rc;
   if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (v)"))) return rc;
-  if ((rc = device_status_word(&status))) return rc;
   if ((rc = reserve(cross_fwd_umma_kernel<T, HD>, FwdSmem<HD>::total, "cross attention forward"))) return rc;
   const int64_t pairs = (a.Lq + 2 * kRows - 1) / (2 * kRows), items = a.B * a.H * pairs * splits;
   if (items > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention forward: too many query rows");
@@ -485,6 +1116,30 @@ int launch_fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, 
   const int64_t sms = device_sms();
   cross_fwd_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kFwdThreads, FwdSmem<HD>::total, st>>>(mq, mk, mv, a, w, status);
   return check_launch("cross_fwd_umma_kernel");
+}
+
+template <typename T, int HD>
+int launch_bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  CUtensorMap mq, mdo, mk, mv, mq64, mdo64;
+  int rc, *status;
+  if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to a thread that has none yet
+  if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention backward (q)"))) return rc;
+  if ((rc = map_of(&mdo, a, a.dout, a.dout_stride, a.H, a.Lq, kRows, "cross attention backward (dout)"))) return rc;
+  if ((rc = map_of(&mq64, a, a.q, a.q_stride, a.H, a.Lq, kQTile, "cross attention backward (q)"))) return rc;
+  if ((rc = map_of(&mdo64, a, a.dout, a.dout_stride, a.H, a.Lq, kQTile, "cross attention backward (dout)"))) return rc;
+  if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention backward (k)"))) return rc;
+  if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention backward (v)"))) return rc;
+  if ((rc = reserve(cross_dq_umma_kernel<T, HD>, DqSmem<HD>::total, "cross attention dQ"))) return rc;
+  if ((rc = reserve(cross_dkdv_umma_kernel<T, HD>, DkSmem<HD>::total, "cross attention dK/dV"))) return rc;
+  const int64_t qtiles = (a.Lq + kRows - 1) / kRows, items = a.B * a.H * qtiles, ktiles = (a.Lkv + kRows - 1) / kRows;
+  const int64_t units = a.B * a.Hkv * ktiles * splits;
+  if (items > 0x3fffffff || units > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention backward: too many rows");
+  const int64_t sms = device_sms();
+  cross_dq_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kDqThreads, DqSmem<HD>::total, st>>>(mq, mdo, mk, mv, a, (int)qtiles, (int)items,
+                                                                                                       status);
+  if ((rc = check_launch("cross_dq_umma_kernel"))) return rc;
+  cross_dkdv_umma_kernel<T, HD><<<(unsigned)units, kDkThreads, DkSmem<HD>::total, st>>>(mq64, mdo64, mk, mv, a, (int)ktiles, splits, part, status);
+  return check_launch("cross_dkdv_umma_kernel");
 }
 
 bool aligned(const void* p, const int64_t (&s)[3], int64_t heads, int64_t rows, int64_t batch) {
@@ -513,6 +1168,11 @@ int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_l
     return a.D <= 64 ? launch_fwd<__half, 64>(a, splits, part_out, part_lse, st) : launch_fwd<__half, 128>(a, splits, part_out, part_lse, st);
   return a.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(a, splits, part_out, part_lse, st)
                    : launch_fwd<__nv_bfloat16, 128>(a, splits, part_out, part_lse, st);
+}
+
+int cross_bwd_umma(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  if (a.dtype == VSA_F16) return a.D <= 64 ? launch_bwd<__half, 64>(a, splits, part, st) : launch_bwd<__half, 128>(a, splits, part, st);
+  return a.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(a, splits, part, st) : launch_bwd<__nv_bfloat16, 128>(a, splits, part, st);
 }
 
 }  // namespace vsa

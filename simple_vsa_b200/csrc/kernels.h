@@ -79,6 +79,7 @@ int cross_generic_tile(int D);
 bool cross_umma_shape(int D, int dtype);
 bool cross_umma_eligible(const VsaCross& a, bool backward);
 int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
+int cross_bwd_umma(const VsaCross& a, int splits, float* part, cudaStream_t st);
 // splits > 1: partial outputs [splits][B*H][Lq][D] and statistics [splits][B*H][Lq] (-inf: no live key), for cross_join
 int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 // splits > 1: partial dK and dV [splits][2][B*Hkv][Lkv][D], for cross_sum
