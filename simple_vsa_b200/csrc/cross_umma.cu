@@ -6,7 +6,7 @@
 // work to the next.
 #include <cuda.h>
 
-#include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -24,7 +24,35 @@ constexpr uint32_t kTmemCols = 512;
 template <typename T> constexpr uint32_t kFmt = 1u;
 template <> constexpr uint32_t kFmt<__half> = 0u;
 
-#define CROSS_WAIT(bar_, parity_) warp_wait((bar_), (parity_), status)
+// Whole-warp wait, bounded by the SM's clock.  Short on purpose: a role's loop with a dozen inlined waits that each look at a global
+// timer and the status word as well is more code than the instruction caches keep beside the softmax (a wait for a barrier that
+// had long flipped took 340 cycles).
+constexpr uint32_t kWaitCycles = 500u * 1000u * 1000u;      // a quarter of a second
+__device__ __forceinline__ uint32_t sm_clock() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  return t;
+}
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint32_t t0 = sm_clock();
+#pragma unroll 1
+  for (;;) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, sm_clock() - t0 > kWaitCycles)) return false;
+  }
+}
+#define CROSS_WAIT(bar_, parity_) wait_for((bar_), (parity_))
+
+// Division of n < 2^31 by a number known on the host: (n + umulhi(n, mul)) >> shift.
+struct Divisor {
+  uint32_t by, mul, shift;
+  explicit Divisor(uint32_t d) : by(d), shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)(((uint32_t)n + __umulhi((uint32_t)n, mul)) >> shift); }
+};
 
 // D[128 x N] = A[128 x HD] B[N x HD]^T, both K-major; halves of 64 head dims kHalf / B_HALF bytes apart.
 template <typename T, int HD, int N, int B_HALF>
@@ -62,6 +90,42 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
   for (int h = 0; h < HD / 64; ++h) tma_load_4d(dst + h * half_bytes, map, h * 64, row, head, batch, bar);
 }
 
+__device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+__device__ __forceinline__ float max3(float x, uint32_t y, uint32_t z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(__uint_as_float(y)), "f"(__uint_as_float(z)));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe, for a share of the exponentials (the MUFU makes 16 a clock and SM, one for every 64 multiply-adds
+// of the tensor cores at head dim 128): x = n + f with n the nearest integer, a polynomial in f on [-1/2, 1/2] (minimax of the relative
+// error: degree 3, 7.5e-5, a twentieth of bf16's half step; degree 4, 2.6e-6, for fp16), times 2^n.  Below 2^-126: 2^-126.  NaN stays NaN.
+template <typename T>
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));       // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+  const float2 magic = make_float2(12582912.f, 12582912.f);           // 1.5 * 2^23: the integer lands in the low bits
+  const float2 t = add2(x, magic), n = add2(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p;
+  if (sizeof(T) == 2 && kFmt<T> == 1u) {
+    p = fma2(make_float2(0.0551716685f, 0.0551716685f), f, make_float2(0.242611125f, 0.242611125f));
+    p = fma2(p, f, make_float2(0.693260968f, 0.693260968f));
+    p = fma2(p, f, make_float2(0.999928057f, 0.999928057f));
+  } else {
+    p = fma2(make_float2(0.00957010221f, 0.00957010221f), f, make_float2(0.0559178591f, 0.0559178591f));
+    p = fma2(p, f, make_float2(0.240247443f, 0.240247443f));
+    p = fma2(p, f, make_float2(0.693121791f, 0.693121791f));
+    p = fma2(p, f, make_float2(0.999999285f, 0.999999285f));
+  }
+  return mul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
+}
+template <typename T>
+__device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
+  return poly ? poly_exp2<T>(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+}
+
 // Live keys of tile j of a sample: a bit each.
 struct TileKeys {
   uint32_t w[4];
@@ -79,10 +143,7 @@ __device__ __forceinline__ TileKeys tile_keys(const VsaCross& a, int b, int len,
   } else {
     const int left = len - j * kRows;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = left - 32 * i;
-      t.w[i] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-    }
+    for (int i = 0; i < 4; ++i) t.w[i] = first_bits(left - 32 * i);
   }
   return t;
 }
@@ -91,14 +152,17 @@ __device__ __forceinline__ TileKeys tile_keys(const VsaCross& a, int b, int len,
 // forward
 // ------------------------------------------------------------------------------------------------------
 // A piece of work is 256 query rows of one head (two tiles of 128, which are the M dimension) against the key tiles of one split.  Both
-// tiles take every K and V tile from the same buffers; a softmax group of four warps owns a tile, a thread owns a row, and while one
-// group exponentiates the tensor cores form the other tile's products.  P goes over the scores it came from in tensor memory.
-// Per 128 x 128 scores at D = 128: 1024 tensor cycles, 1024 cycles of exponentials, 128 KB of shared-memory traffic at 128 B/clk.
-// The tensor cores run the MMAs of a CTA in the order of their issue: S(j+1) of a tile is issued behind its O += P(j) V(j) and
-// overwrites that P after it has been read.
+// tiles take every K and V tile from the same buffers; four softmax warps own a tile, a thread a row.  The keys are walked 64 at a
+// time and a tile has two score accumulators, so that the next scores are there when a softmax group has finished: with one
+// accumulator of 128 keys the groups idled 42 % of the time behind S, and eight warps a tile that shared its rows gained nothing
+// (5200 cycles per 256 x 128 scores either way; this form ...).  P goes over the scores it came from in tensor memory.
+// Per 128 x 128 scores at D = 128: 1280 tensor cycles (an M128 x N64 x K16 product takes 48 of the 32 that its size asks for), 1024
+// of exponentials.
 // The softmax keeps a running maximum, but moves the accumulated row only when the maximum has grown by more than 2^8: P stays below
 // 2^8 (fp16 holds 2^16, the sums are fp32), and moving O through registers is rare.
-constexpr int kFwdThreads = 384;
+constexpr int kFwdThreads = 256 + 256;     // loads and four issuers of MMAs (eight warps), two softmax groups
+constexpr int kKeys = 64;                  // keys of a step
+constexpr int kFwdPoly = 3;                // of eight pairs of exponentials, on the FMA pipe
 template <int HD>
 struct FwdSmem {
   static constexpr uint32_t tile = HD * 256;                      // 128 rows
@@ -107,36 +171,41 @@ struct FwdSmem {
   static constexpr uint32_t kv = q + 2 * tile;
   static constexpr uint32_t stage = kv + stages * tile;           // 32 rows x 128 bytes a softmax warp
   static constexpr uint32_t bars = stage + 8 * 4096;
-  static constexpr uint32_t misc = bars + 40 * 8;
+  static constexpr uint32_t misc = bars + 34 * 8;
   static constexpr uint32_t total = misc + 16;
 };
 static_assert(FwdSmem<128>::total <= 232448 && FwdSmem<64>::total <= 232448, "shared memory of the cross attention forward");
-enum FwdBar { F_Q_FULL = 0, F_Q_EMPTY = 2, F_S_FULL = 4, F_P_FULL = 6, F_P2_FULL = 8, F_O_FULL = 10, F_KV_FULL = 12, F_KV_EMPTY = 20 };
+// the score accumulators of a tile: index 2 * tile + (step & 1)
+enum FwdBar { F_Q_FULL = 0, F_Q_EMPTY = 2, F_O_FULL = 4, F_S_FULL = 6, F_S_EMPTY = 10, F_P_FULL = 14, F_KV_FULL = 18, F_KV_EMPTY = 26 };
 
 struct FwdWork {
-  int pairs, splits, items;       // pairs of query tiles per head, splits of the keys, all pieces
+  Divisor splits, pairs, heads, group;          // splits of the keys; pairs of query tiles per head; query heads, and per key head
+  int items;                                    // all pieces
   float *part_out, *part_lse;
 };
 struct FwdItem {
   int b, h, row0, tiles, len, j0, j1, split;    // tiles: 1 or 2 live query tiles; key tiles j0 .. j1
   __device__ __forceinline__ FwdItem(const VsaCross& a, const FwdWork& w, int item) {
-    const int rest = item / w.splits, bh = rest / w.pairs;
-    split = item - rest * w.splits;
-    b = bh / (int)a.H;
-    h = bh - b * (int)a.H;
-    row0 = (rest - bh * w.pairs) * 2 * kRows;
-    tiles = row0 + kRows < a.Lq ? 2 : 1;
+    const int rest = w.splits(item), bh = w.pairs(rest);
+    split = item - rest * (int)w.splits.by;
+    b = w.heads(bh);
+    h = bh - b * (int)w.heads.by;
+    row0 = (rest - bh * (int)w.pairs.by) * 2 * kRows;
+    tiles = row0 + kRows < (int)a.Lq ? 2 : 1;
     len = cross_length(a, b);
-    const int n = (len + kRows - 1) / kRows, per = (n + w.splits - 1) / w.splits;
+    const int n = (len + kRows - 1) / kRows, per = w.splits(n + (int)w.splits.by - 1);
     j0 = split * per;
     j1 = min(n, j0 + per);
   }
+  // steps of 64 keys: the last tile may need only one
+  __device__ __forceinline__ int halves() const { return j1 <= j0 ? 0 : min(2 * (j1 - j0), (len + kKeys - 1) / kKeys - 2 * j0); }
 };
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ VsaCross a, const FwdWork w, int* status) {
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+                      const __grid_constant__ VsaCross a, const FwdWork w, int* status) {
   using Sm = FwdSmem<HD>;
   extern __shared__ __align__(1024) uint8_t cross_smem[];
   if (*(volatile int*)status != 0) return;
@@ -153,21 +222,23 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar(F_Q_FULL + t), 1);
       mbar_init(bar(F_Q_EMPTY + t), 1);
-      mbar_init(bar(F_S_FULL + t), 1);
-      mbar_init(bar(F_P_FULL + t), 4);
-      mbar_init(bar(F_P2_FULL + t), 4);
       mbar_init(bar(F_O_FULL + t), 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(F_S_FULL + i), 1);
+      mbar_init(bar(F_S_EMPTY + i), 1);
+      mbar_init(bar(F_P_FULL + i), 4);
     }
     for (int i = 0; i < Sm::stages; ++i) {
       mbar_init(bar(F_KV_FULL + i), 1);
-      mbar_init(bar(F_KV_EMPTY + i), 1);
+      mbar_init(bar(F_KV_EMPTY + i), 2);           // one issuer for each query tile
     }
     fence_barrier_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
-  if (warp == 2) {
+  if (warp == 5) {
     tmem_alloc(base + Sm::misc, kTmemCols);
     tmem_relinquish();
   }
@@ -175,61 +246,65 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = misc[0];
-  const uint32_t tmem_o = tmem + 256;              // S of the two tiles, then O of the two tiles
-  const int group_heads = (int)(a.H / a.Hkv);
+  const uint32_t tmem_o = tmem + 256;              // two score accumulators of each tile, then O of the two tiles
   bool ok = true;
 
-  if (warp >= 4) {                                 // 2 x 208 + 80 registers are within the three groups' 168 at launch
-    registers_inc<208>();
-    const int quarter = warp & 3, t = (warp - 4) >> 2, row = quarter * 32 + lane;
+  if (warp >= 8) {                                 // 256 x 184 + 256 x 72 registers are the block's 512 x 128 at launch
+    registers_inc<184>();
+    const int quarter = warp & 3, t = (warp - 8) >> 2, row = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + 128 * t + lane_addr, o_addr = tmem_o + HD * t + lane_addr;
-    const float c = a.scale * kLog2e, c_abs = fabsf(c);
-    uint32_t s_uses = 0, o_uses = 0, steps = 0;    // phases of this tile's barriers; K/V pairs so far
+    const uint32_t o_addr = tmem_o + HD * t + lane_addr;
+    const float c = a.scale * kLog2e;          // > 0
+    uint32_t u = 0, pieces = 0, tiles = 0;         // steps and pieces of this tile so far; K/V tiles
     for (int item = blockIdx.x; item < w.items && ok; item += gridDim.x) {
       const FwdItem it(a, w, item);
+      const int halves = it.halves();
       if (t >= it.tiles) {
-        if (it.j1 > it.j0) steps += it.j1 - it.j0;
+        tiles += (halves + 1) >> 1;
         continue;
       }
       float m = -INFINITY;
       float2 lsum = make_float2(0.f, 0.f);
-      for (int j = it.j0; j < it.j1; ++j, ++steps) {
-        const TileKeys keys = tile_keys(a, it.b, it.len, j);
-        const bool full = keys.full();
-        ok = CROSS_WAIT(bar(F_S_FULL + t), s_uses & 1);
-        if (!ok) break;
-        ++s_uses;
-        tc_fence_after();
-        uint32_t sv[4][32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld(s_addr + 32 * i, sv[i]);
-        tmem_ld_wait();
-        float top;
-        {
-          float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (full && c >= 0.f) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) x[q] = fmaxf(x[q], __uint_as_float(sv[q][i]));
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float s = c >= 0.f ? __uint_as_float(sv[q][i]) : -__uint_as_float(sv[q][i]);
-                x[q] = fmaxf(x[q], keys.w[q] >> i & 1u ? s : -INFINITY);
-              }
-          }
-          top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          top = top == -INFINITY ? top : top * c_abs;
+      for (int i = 0; i < halves; ++i, ++u) {
+        const int key0 = it.j0 * kRows + i * kKeys;
+        uint32_t w0 = 0xffffffffu, w1 = 0xffffffffu;               // the live keys of this step
+        if (a.key_bits != nullptr) {
+          const uint2 x = *reinterpret_cast<const uint2*>(a.key_bits + (long long)it.b * cross_words(a.Lkv) + (key0 >> 5));
+          w0 = x.x, w1 = x.y;
+        } else if (it.len - key0 < kKeys) {
+          w0 = first_bits(it.len - key0), w1 = first_bits(it.len - key0 - 32);
         }
-        if (j == it.j0) {
+        const bool full = (w0 & w1) == 0xffffffffu;
+        const int acc = 2 * t + (u & 1);
+        const uint32_t s_addr = tmem + 64 * acc + lane_addr;
+        ok = CROSS_WAIT(bar(F_S_FULL + acc), (u >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sv[2][32];
+        tmem_ld(s_addr, sv[0]);
+        tmem_ld(s_addr + 32, sv[1]);
+        tmem_ld_wait();
+        if (!full) {                               // what stands in a key that takes no part may be anything: P = 2^-inf
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (!(w0 >> e & 1u)) sv[0][e] = 0xff800000u;
+            if (!(w1 >> e & 1u)) sv[1][e] = 0xff800000u;
+          }
+        }
+        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[q] = max3(x[q], sv[q & 1][e + (q & 2)], sv[q & 1][e + (q & 2) + 1]);
+        const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * c;
+        if (i == 0) {
           m = top;
         } else {
           const bool up = top > m + 8.f;
-          if (__any_sync(0xffffffffu, up)) {       // O holds P V of every tile before this one: S came behind it in the pipe
+          if (__any_sync(0xffffffffu, up)) {       // all products before this step's must be in O; only this group lets the next start
+            ok = CROSS_WAIT(bar(F_S_EMPTY + (acc ^ 1)), ((u - 1) >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
             const float keep = up ? fast_exp2(m - top) : 1.f;
             if (up) m = top;
             lsum = mul2(lsum, make_float2(keep, keep));
@@ -239,112 +314,107 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
               tmem_ld(o_addr + d, ov);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * keep);
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * keep);
               tmem_st(o_addr + d, ov);
             }
           }
         }
-        if (!full && t == 0) {                     // rows of V that no key takes part with meet P = 0: they must be finite
-          const uint32_t r = 2 * steps + 1, s = r % Sm::stages;
+        if (!full) {                               // rows of V that no key takes part with meet P = 0: they must be finite.  Both tiles'
+                                                   // groups clear them, each before the product that it starts.
+          const uint32_t r = 2 * (tiles + (i >> 1)) + 1, s = r % Sm::stages;
           ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1);
           if (!ok) break;
-          if (!keys.bit(row)) {
-            uint8_t* vrow = sm + Sm::kv + s * Sm::tile + row * 128;
+          const int vr = (i & 1) * kKeys + (row & 63);             // two threads a row
+          if (!((row & 32 ? w1 : w0) >> (row & 31) & 1u)) {
+            uint8_t* vrow = sm + Sm::kv + s * Sm::tile + vr * 128;
 #pragma unroll
-            for (int ch = 0; ch < HD / 8; ++ch)
-              *reinterpret_cast<uint4*>(vrow + (ch >> 3) * kHalf + ((ch ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < HD / 16; ++e) {
+              const int ch = (row >> 6) * (HD / 16) + e;
+              *reinterpret_cast<uint4*>(vrow + (ch >> 3) * kHalf + ((ch ^ vr) & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
           }
           fence_proxy_async_smem();
         }
         const float shift = m == -INFINITY ? 0.f : m;
         const float2 c2 = make_float2(c, c), m2 = make_float2(-shift, -shift);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
           uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 x = fma2(word_pair(sv[q] + 2 * i), c2, m2);
-            float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-            if (!full) {                           // what stands in a key that takes no part may be anything: select
-              if (!(keys.w[q] >> (2 * i) & 1u)) e.x = 0.f;
-              if (!(keys.w[q] >> (2 * i + 1) & 1u)) e.y = 0.f;
-            }
-            lsum = add2(lsum, e);
-            pk[i] = Elem<T>::pack(e.x, e.y);
+          for (int e = 0; e < 16; ++e) {
+            const float2 p = exp2_pair<T>(fma2(word_pair(sv[q] + 2 * e), c2, m2), kFwdPoly > 0 && e % 8 < kFwdPoly);
+            lsum = add2(lsum, p);
+            pk[e] = Elem<T>::pack(p.x, p.y);
           }
           tmem_st(s_addr + 16 * q, pk);
-          if (q & 1) {                             // the product of the first 64 keys starts under the others
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar((q == 1 ? F_P_FULL : F_P2_FULL) + t));
-          }
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(F_P_FULL + acc));
       }
       if (!ok) break;
-      const float l = lsum.x + lsum.y, inv = l == 0.f ? 0.f : 1.f / l;
-      const bool any = it.j1 > it.j0;
+      tiles += (halves + 1) >> 1;
+      const float sum = lsum.x + lsum.y, l = sum < 1e-6f ? 0.f : sum, inv = l == 0.f ? 0.f : 1.f / l;      // a live key is worth 2^-8 at least
+      const bool any = halves > 0;
       if (any) {
-        ok = CROSS_WAIT(bar(F_O_FULL + t), o_uses & 1);
+        ok = CROSS_WAIT(bar(F_O_FULL + t), pieces & 1);
         if (!ok) break;
-        ++o_uses;
+        ++pieces;
         tc_fence_after();
       }
       const int row_w = it.row0 + t * kRows + quarter * 32;         // first row of this warp
       const long long bh = (long long)it.b * a.H + it.h;
-      if (w.splits == 1) {
+      if (w.splits.by == 1) {
         a.lse2[bh * cross_rows(a.Lq) + row_w + lane] = l == 0.f || row_w + lane >= a.Lq ? INFINITY : m + log2f(l);
-        T* out = (T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1];
-        uint8_t* stage = sm + Sm::stage + (warp - 4) * 4096;
-#pragma unroll
-        for (int hh = 0; hh < HD / 64; ++hh) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t ov[32];
-            if (any) {
-              tmem_ld(o_addr + hh * 64 + half * 32, ov);
-              tmem_ld_wait();
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] = any ? __float_as_uint(__uint_as_float(ov[i]) * inv) : 0u;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * half + q) ^ (lane & 7)) << 4)) = pack8<T>(ov + 8 * q);
-          }
+        // 64 dims at a time through 32 rows x 128 bytes of shared memory and out by TMA, which leaves what lies outside the tensor
+        uint8_t* stage = sm + Sm::stage + (warp - 8) * 4096;
+#pragma unroll 1
+        for (int d0 = 0; d0 < HD; d0 += 64) {
+          uint32_t ov[2][32];
+          tmem_ld(o_addr + d0, ov[0]);
+          tmem_ld(o_addr + d0 + 32, ov[1]);
+          if (lane == 0) bulk_wait_read();         // the boxes before have left the buffer
           __syncwarp();
+          tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3), ch = lane & 7, d = hh * 64 + ch * 8;
-            if (row_w + r < a.Lq && d < a.D)
-              *reinterpret_cast<uint4*>(out + (row_w + r) * a.out_stride[2] + d) =
-                  *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+          for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[q][e] = any ? __float_as_uint(__uint_as_float(ov[q][e]) * inv) : 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * q + e) ^ (lane & 7)) << 4)) = pack8<T>(ov[q] + 8 * e);
           }
+          fence_proxy_async_smem();
           __syncwarp();
+          if (lane == 0) {
+            if (row_w < a.Lq) tma_store_4d(&map_out, smem_u32(stage), d0, row_w, it.h, it.b);
+            bulk_commit();
+          }
         }
       } else {
         const long long at = (it.split * (long long)a.B * a.H + bh) * a.Lq + row_w + lane;
         const bool there = row_w + lane < a.Lq;
         if (there) w.part_lse[at] = l == 0.f ? -INFINITY : m + log2f(l);
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 16) {
+          uint32_t ov[16];
+          tmem_ld(o_addr + d, ov);
+          tmem_ld_wait();
 #pragma unroll
-        for (int d = 0; d < HD; d += 32) {
-          uint32_t ov[32];
-          if (any) {
-            tmem_ld(o_addr + d, ov);
-            tmem_ld_wait();
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            if (there && d + i < a.D)
-              *reinterpret_cast<float4*>(w.part_out + at * a.D + d + i) =
-                  any ? make_float4(__uint_as_float(ov[i]) * inv, __uint_as_float(ov[i + 1]) * inv, __uint_as_float(ov[i + 2]) * inv,
-                                    __uint_as_float(ov[i + 3]) * inv)
+          for (int e = 0; e < 16; e += 4)
+            if (there && d + e < a.D)
+              *reinterpret_cast<float4*>(w.part_out + at * a.D + d + e) =
+                  any ? make_float4(__uint_as_float(ov[e]) * inv, __uint_as_float(ov[e + 1]) * inv, __uint_as_float(ov[e + 2]) * inv,
+                                    __uint_as_float(ov[e + 3]) * inv)
                       : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
     }
+    if (lane == 0) bulk_wait();
     if (!ok && lane == 0) atomicCAS(status, 0, 71);
   } else {
-    registers_dec<80>();
+    registers_dec<72>();
     if (warp == 0) {
       uint32_t q_phase = 3, r = 0;                 // a bit per tile
       auto load_q = [&](const FwdItem& it, int t) {
@@ -357,105 +427,101 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
         __syncwarp();
       };
-      auto load_kv = [&](const FwdItem& it, const CUtensorMap* map, int j) {
+      auto load_kv = [&](const FwdItem& it, const CUtensorMap* map, int j, int hk) {
         const uint32_t s = r % Sm::stages;
         ok = CROSS_WAIT(bar(F_KV_EMPTY + s), ((r / Sm::stages) & 1) ^ 1);
         if (!ok) return;
         ++r;
         if (elect_one()) {
           mbar_arrive_expect_tx(bar(F_KV_FULL + s), Sm::tile);
-          load_rows<HD>(base + Sm::kv + s * Sm::tile, map, j * kRows, it.h / group_heads, it.b, kHalf, bar(F_KV_FULL + s));
+          load_rows<HD>(base + Sm::kv + s * Sm::tile, map, j * kRows, hk, it.b, kHalf, bar(F_KV_FULL + s));
         }
         __syncwarp();
       };
       for (int item = blockIdx.x; item < w.items && ok; item += gridDim.x) {
         const FwdItem it(a, w, item);
-        if (it.j1 <= it.j0) continue;
+        if (it.halves() == 0) continue;
+        const int hk = w.group(it.h);
         load_q(it, 0);
         for (int j = it.j0; j < it.j1 && ok; ++j) {
-          load_kv(it, &map_k, j);
+          load_kv(it, &map_k, j, hk);
           if (j == it.j0 && it.tiles == 2 && ok) load_q(it, 1);
-          if (ok) load_kv(it, &map_v, j);
+          if (ok) load_kv(it, &map_v, j, hk);
         }
       }
       if (!ok && lane == 0) atomicCAS(status, 0, 72);
-    } else if (warp == 1) {
-      // step n: key tile j of a piece, K in buffer 2n and V in buffer 2n+1 of the ring
-      struct Cursor {
-        int item, tiles, j, j0, j1;
-      };
-      auto settle = [&](Cursor& x) {               // the first piece from x.item on that has a key tile
-        for (; x.item < w.items; x.item += gridDim.x) {
-          const FwdItem it(a, w, x.item);
-          if (it.j1 > it.j0) {
-            x.tiles = it.tiles;
-            x.j = x.j0 = it.j0;
-            x.j1 = it.j1;
-            return;
-          }
-        }
-      };
-      uint32_t q_phase = 0, p_phase = 0;           // a bit per tile
-      auto issue_s = [&](const Cursor& x, uint32_t n, int t) {
-        const uint32_t r = 2 * n, s = r % Sm::stages;
-        if (x.j == x.j0) {
-          ok = CROSS_WAIT(bar(F_Q_FULL + t), q_phase >> t & 1);
-          if (!ok) return;
-          q_phase ^= 1u << t;
-        }
-        ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        if (elect_one()) {
-          issue_scores<T, HD, 128, kHalf>(tmem + 128 * t, base + Sm::q + t * Sm::tile, base + Sm::kv + s * Sm::tile);
-          mma_commit(bar(F_S_FULL + t));
-          if (x.j == x.j1 - 1) mma_commit(bar(F_Q_EMPTY + t));
-          if (t == x.tiles - 1) mma_commit(bar(F_KV_EMPTY + s));
-        }
-        __syncwarp();
-      };
-      Cursor next{(int)blockIdx.x, 0, 0, 0, 0};
-      settle(next);
-      if (next.item < w.items)
-        for (int t = 0; t < next.tiles && ok; ++t) issue_s(next, 0, t);
-      for (uint32_t n = 0; ok && next.item < w.items; ++n) {
-        const Cursor cur = next;
-        if (++next.j == next.j1) {
-          next.item += gridDim.x;
-          settle(next);
-        }
-        const bool more = next.item < w.items;
-        const uint32_t r = 2 * n + 1, s = r % Sm::stages;
-        const uint32_t v_tile = base + Sm::kv + s * Sm::tile;
-#pragma unroll 1
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (t < cur.tiles) {
-            ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1) && CROSS_WAIT(bar(F_P_FULL + t), p_phase >> t & 1);
+    } else if (warp <= 2) {
+      // S = Q K^T of query tile t: K tile n is in buffer 2n of the ring.  A warp issues an MMA in 40 cycles and a commit in 70 to 100; one
+      // warp for both products of both tiles took 3500 cycles per step and was what bounded the kernel.
+      const int t = warp - 1;
+      uint32_t u = 0, pieces = 0, r = 0;
+      for (int item = blockIdx.x; item < w.items && ok; item += gridDim.x) {
+        const FwdItem it(a, w, item);
+        const int halves = it.halves();
+        if (t < it.tiles && halves > 0) {
+          ok = CROSS_WAIT(bar(F_Q_FULL + t), pieces & 1);
+          ++pieces;
+          for (int i = 0; i < halves && ok; ++i, ++u) {
+            const uint32_t rk = r + (i & ~1), s = rk % Sm::stages;
+            const int acc = 2 * t + (u & 1);
+            ok = CROSS_WAIT(bar(F_KV_FULL + s), (rk / Sm::stages) & 1) && CROSS_WAIT(bar(F_S_EMPTY + acc), ((u >> 1) & 1) ^ 1);
             if (!ok) break;
-            tc_fence_after();
-            if (elect_one())
-              issue_product<T, HD, 64, 128, 128>(tmem_o + HD * t, tmem + 128 * t, v_tile, cur.j > cur.j0);
-            __syncwarp();
-            ok = CROSS_WAIT(bar(F_P2_FULL + t), p_phase >> t & 1);
-            if (!ok) break;
-            p_phase ^= 1u << t;
             tc_fence_after();
             if (elect_one()) {
-              issue_product<T, HD, 64, 128, 128>(tmem_o + HD * t, tmem + 128 * t + 32, v_tile + 64 * 128, true);
-              if (cur.j == cur.j1 - 1) mma_commit(bar(F_O_FULL + t));
-              if (t == cur.tiles - 1) mma_commit(bar(F_KV_EMPTY + s));
+              issue_scores<T, HD, kKeys, kHalf>(tmem + 64 * acc, base + Sm::q + t * Sm::tile, base + Sm::kv + s * Sm::tile + (i & 1) * kKeys * 128);
+              mma_commit(bar(F_S_FULL + acc));
+              if (i == halves - 1) mma_commit(bar(F_Q_EMPTY + t));
+              if ((i & 1) || i == halves - 1) mma_commit(bar(F_KV_EMPTY + s));
             }
             __syncwarp();
           }
-          if (more && t < next.tiles) issue_s(next, n + 1, t);
+        } else if (t == 1) {                       // a piece of one query tile: its K tiles are free when the other has read them
+          for (int i = 0; i < halves; i += 2) {
+            const uint32_t s = (r + i) % Sm::stages;
+            ok = ok && CROSS_WAIT(bar(F_KV_FULL + s), ((r + i) / Sm::stages) & 1);
+            if (ok && lane == 0) mbar_arrive(bar(F_KV_EMPTY + s));
+          }
         }
+        r += (halves + 1) & ~1;
       }
       if (!ok && lane == 0) atomicCAS(status, 0, 73);
+    } else if (warp <= 4) {
+      // O += P V of query tile t: V tile n is in buffer 2n + 1
+      const int t = warp - 3;
+      uint32_t u = 0, r = 0;
+      for (int item = blockIdx.x; item < w.items && ok; item += gridDim.x) {
+        const FwdItem it(a, w, item);
+        const int halves = it.halves();
+        if (t < it.tiles) {
+          for (int i = 0; i < halves && ok; ++i, ++u) {
+            const uint32_t rv = r + (i & ~1) + 1, s = rv % Sm::stages;
+            const int acc = 2 * t + (u & 1);
+            ok = CROSS_WAIT(bar(F_KV_FULL + s), (rv / Sm::stages) & 1) && CROSS_WAIT(bar(F_P_FULL + acc), (u >> 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              issue_product<T, HD, kKeys, kKeys, kRows>(tmem_o + HD * t, tmem + 64 * acc, base + Sm::kv + s * Sm::tile + (i & 1) * kKeys * 128, i > 0);
+              mma_commit(bar(F_S_EMPTY + acc));
+              if (i == halves - 1) mma_commit(bar(F_O_FULL + t));
+              if ((i & 1) || i == halves - 1) mma_commit(bar(F_KV_EMPTY + s));
+            }
+            __syncwarp();
+          }
+        } else {
+          for (int i = 0; i < halves; i += 2) {
+            const uint32_t rv = r + i + 1, s = rv % Sm::stages;
+            ok = ok && CROSS_WAIT(bar(F_KV_FULL + s), (rv / Sm::stages) & 1);
+            if (ok && lane == 0) mbar_arrive(bar(F_KV_EMPTY + s));
+          }
+        }
+        r += (halves + 1) & ~1;
+      }
+      if (!ok && lane == 0) atomicCAS(status, 0, 74);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 2) tmem_dealloc(tmem, kTmemCols);
+  if (warp == 5) tmem_dealloc(tmem, kTmemCols);
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -467,17 +533,19 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // shared memory and out from registers that were filled while the piece before was finished.
 constexpr int kDqCols = 32;
 constexpr int kDqGroups = kRows / kDqCols;
+constexpr int kDqPoly = 3;                 // of eight pairs of exponentials, on the FMA pipe
 constexpr int kDqEwThreads = 128 * kDqGroups;
 constexpr int kDqThreads = 128 + kDqEwThreads;
 template <int HD>
 struct DqSmem {
   static constexpr uint32_t tile = HD * 256;
-  static constexpr int k_stages = 3, v_stages = 2;
+  static constexpr int k_stages = 3, v_stages = HD == 128 ? 1 : 2;
   static constexpr uint32_t q = 0;
   static constexpr uint32_t d_o = q + tile;
   static constexpr uint32_t k = d_o + tile;
   static constexpr uint32_t v = k + k_stages * tile;
-  static constexpr uint32_t delta = v + v_stages * tile;          // float [2][128]
+  static constexpr uint32_t stage = v + v_stages * tile;          // 32 rows x 64 bytes an elementwise warp
+  static constexpr uint32_t delta = stage + 16 * 2048;            // float [2][128]
   static constexpr uint32_t bars = delta + 1024;
   static constexpr uint32_t misc = bars + 32 * 8;
   static constexpr uint32_t total = misc + 16;
@@ -488,11 +556,11 @@ enum DqBar { Q_QDO_FULL = 0, Q_QDO_EMPTY = 1, Q_K_FULL = 2, Q_K_EMPTY = 5, Q_V_F
 
 struct DqItem {
   int b, h, row0, len, n;                       // n key tiles
-  __device__ __forceinline__ DqItem(const VsaCross& a, int qtiles, int item) {
-    const int bh = item / qtiles;
-    row0 = (item - bh * qtiles) * kRows;
-    b = bh / (int)a.H;
-    h = bh - b * (int)a.H;
+  __device__ __forceinline__ DqItem(const VsaCross& a, const Divisor& qtiles, const Divisor& heads, int item) {
+    const int bh = qtiles(item);
+    row0 = (item - bh * (int)qtiles.by) * kRows;
+    b = heads(bh);
+    h = bh - b * (int)heads.by;
     len = cross_length(a, b);
     n = (len + kRows - 1) / kRows;
   }
@@ -501,8 +569,9 @@ struct DqItem {
 template <typename T, int HD>
 __global__ void __launch_bounds__(kDqThreads, 1)
 cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ VsaCross a,
-                     int qtiles, int items, int* status) {
+                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ CUtensorMap map_dq, const __grid_constant__ VsaCross a, const Divisor qtiles, const Divisor heads,
+                     const Divisor group_heads, int items, int* status) {
   using Sm = DqSmem<HD>;
   extern __shared__ __align__(1024) uint8_t cross_smem[];
   if (*(volatile int*)status != 0) return;
@@ -547,13 +616,12 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   tc_fence_after();
   const uint32_t tmem = misc[0];
   const uint32_t tmem_dp = tmem + 256, tmem_acc = tmem + 384;
-  const int group_heads = (int)(a.H / a.Hkv);
   bool ok = true;
   uint32_t n = 0, live_items = 0;                // key tiles and pieces (with a key tile) so far
 
   if (warp == 0) {
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const DqItem it(a, qtiles, item);
+      const DqItem it(a, qtiles, heads, item);
       if (it.n == 0) continue;
       ok = CROSS_WAIT(bar(Q_QDO_EMPTY), (live_items & 1) ^ 1);
       if (!ok) break;
@@ -564,7 +632,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         load_rows<HD>(base + Sm::d_o, &map_do, it.row0, it.h, it.b, kHalf, bar(Q_QDO_FULL));
       }
       __syncwarp();
-      const int hk = it.h / group_heads;
+      const int hk = group_heads(it.h);
       for (int j = 0; j < it.n; ++j, ++n) {
         const uint32_t sk = n % Sm::k_stages, sv = n % Sm::v_stages;
         ok = CROSS_WAIT(bar(Q_K_EMPTY + sk), ((n / Sm::k_stages) & 1) ^ 1);
@@ -587,7 +655,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   } else if (warp == 2) {
     // S = Q K^T
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const DqItem it(a, qtiles, item);
+      const DqItem it(a, qtiles, heads, item);
       if (it.n == 0) continue;
       ok = CROSS_WAIT(bar(Q_QDO_FULL), live_items & 1);
       ++live_items;
@@ -608,7 +676,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   } else if (warp == 1) {
     // dP = dO V^T
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const DqItem it(a, qtiles, item);
+      const DqItem it(a, qtiles, heads, item);
       if (it.n == 0) continue;
       ok = CROSS_WAIT(bar(Q_QDO_FULL), live_items & 1);
       ++live_items;
@@ -630,7 +698,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   } else if (warp == 3) {
     // dQ += dS K
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const DqItem it(a, qtiles, item);
+      const DqItem it(a, qtiles, heads, item);
       for (int j = 0; j < it.n && ok; ++j, ++n) {
         const uint32_t s = n % Sm::k_stages, b = n & 1;
         ok = CROSS_WAIT(bar(Q_K_FULL + s), (n / Sm::k_stages) & 1) && CROSS_WAIT(bar(Q_DS_FULL + b), (n >> 1) & 1);
@@ -659,11 +727,11 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     uint4 out_r[kPieces];
     float lse_r = 0.f;
     auto fetch = [&](int item) {
-      const DqItem it(a, qtiles, item);
+      const DqItem it(a, qtiles, heads, item);
       const T* o = (const T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1] + (long long)(it.row0 + dr) * a.out_stride[2];
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        const int d = part * (HD / kDqGroups) + i * 8;
+        const int d = (i * kDqGroups + part) * 8;
         out_r[i] = it.row0 + dr < a.Lq && d < a.D ? *reinterpret_cast<const uint4*>(o + d) : make_uint4(0, 0, 0, 0);
       }
       lse_r = a.lse2[((long long)it.b * a.H + it.h) * lp + it.row0 + row];
@@ -671,7 +739,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     if ((int)blockIdx.x < items) fetch(blockIdx.x);
     uint32_t pieces = 0;                                         // all pieces so far, of which live_items have key tiles
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++pieces) {
-      const DqItem it(a, qtiles, item);
+      const DqItem it(a, qtiles, heads, item);
       const long long bh = (long long)it.b * a.H + it.h;
       T* dq = (T*)a.dq + it.b * a.dq_stride[0] + it.h * a.dq_stride[1] + (long long)(it.row0 + row) * a.dq_stride[2];
       const bool there = it.row0 + row < a.Lq;
@@ -690,7 +758,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         float acc = 0.f;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-          const int ch = part * (HD / kDqGroups / 8) + i;        // 16-byte piece of the row
+          const int ch = i * kDqGroups + part;                   // 16-byte piece of the row
           const uint4 x = *reinterpret_cast<const uint4*>(sm + Sm::d_o + (ch >> 3) * kHalf + dr * 128 + (((ch ^ dr) & 7) << 4));
           const uint32_t *p = &out_r[i].x, *q = &x.x;
 #pragma unroll
@@ -733,8 +801,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         float2 pf[kDqCols / 2];
 #pragma unroll
         for (int i = 0; i < kDqCols / 2; ++i) {
-          const float2 x = fma2(word_pair(sv + 2 * i), c2, l2);
-          pf[i] = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+          pf[i] = exp2_pair<T>(fma2(word_pair(sv + 2 * i), c2, l2), kDqPoly > 0 && i % 8 < kDqPoly);
         }
         ok = CROSS_WAIT(bar(Q_DP_FULL), n & 1);
         if (!ok) break;
@@ -777,11 +844,22 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 #pragma unroll
           for (int i = 0; i < 32; ++i) av[i] ^= 0x80000000u;
         }
+        // TMA's 64-byte swizzle (pieces xor row / 2); what lies outside the tensor is not written.  Stored by the threads, 16 bytes a
+        // row and instruction, it took 3400 cycles of a piece's 17600.
+        uint8_t* stage = sm + Sm::stage + (warp - 4) * 2048;
+        if (lane == 0) bulk_wait_read();         // the box before has left the buffer
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 32; i += 8)
-          if (there && c0 + i < a.D) *reinterpret_cast<uint4*>(dq + c0 + i) = pack8<T>(av + i);
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = pack8<T>(av + 8 * q);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (it.row0 + quarter * 32 < a.Lq && c0 < a.D) tma_store_4d(&map_dq, smem_u32(stage), c0, it.row0 + quarter * 32, it.h, it.b);
+          bulk_commit();
+        }
       }
     }
+    if (lane == 0) bulk_wait();
     if (!ok && lane == 0) atomicCAS(status, 0, 85);
   }
   tc_fence_before();
@@ -1096,31 +1174,33 @@ int reserve(Kern kern, int bytes, const char* what) {
   return e == cudaSuccess ? VSA_OK : fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
 }
 
-int map_of(CUtensorMap* map, const VsaCross& a, const void* p, const int64_t (&stride)[3], int64_t heads, int64_t rows, int box, const char* what) {
+int map_of(CUtensorMap* map, const VsaCross& a, const void* p, const int64_t (&stride)[3], int64_t heads, int64_t rows, int box, const char* what,
+           int box_dims = 64) {
   return make_map_rows(map, a.dtype == VSA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p, a.D, rows, heads, a.B,
-                       stride[2], stride[1], stride[0], box, what);
+                       stride[2], stride[1], stride[0], box, what, box_dims);
 }
 
 template <typename T, int HD>
 int launch_fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   int rc, *status;
   if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to a thread that has none yet
   if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention forward (q)"))) return rc;
   if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (k)"))) return rc;
   if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (v)"))) return rc;
+  if ((rc = map_of(&mo, a, a.out, a.out_stride, a.H, a.Lq, 32, "cross attention forward (out)"))) return rc;
   if ((rc = reserve(cross_fwd_umma_kernel<T, HD>, FwdSmem<HD>::total, "cross attention forward"))) return rc;
   const int64_t pairs = (a.Lq + 2 * kRows - 1) / (2 * kRows), items = a.B * a.H * pairs * splits;
   if (items > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention forward: too many query rows");
-  const FwdWork w{(int)pairs, splits, (int)items, part_out, part_lse};
+  const FwdWork w{Divisor((uint32_t)splits), Divisor((uint32_t)pairs), Divisor((uint32_t)a.H), Divisor((uint32_t)(a.H / a.Hkv)), (int)items, part_out, part_lse};
   const int64_t sms = device_sms();
-  cross_fwd_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kFwdThreads, FwdSmem<HD>::total, st>>>(mq, mk, mv, a, w, status);
+  cross_fwd_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kFwdThreads, FwdSmem<HD>::total, st>>>(mq, mk, mv, mo, a, w, status);
   return check_launch("cross_fwd_umma_kernel");
 }
 
 template <typename T, int HD>
 int launch_bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
-  CUtensorMap mq, mdo, mk, mv, mq64, mdo64;
+  CUtensorMap mq, mdo, mk, mv, mq64, mdo64, mdq;
   int rc, *status;
   if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to a thread that has none yet
   if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention backward (q)"))) return rc;
@@ -1129,14 +1209,15 @@ int launch_bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   if ((rc = map_of(&mdo64, a, a.dout, a.dout_stride, a.H, a.Lq, kQTile, "cross attention backward (dout)"))) return rc;
   if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention backward (k)"))) return rc;
   if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention backward (v)"))) return rc;
+  if ((rc = map_of(&mdq, a, a.dq, a.dq_stride, a.H, a.Lq, 32, "cross attention backward (dq)", 32))) return rc;
   if ((rc = reserve(cross_dq_umma_kernel<T, HD>, DqSmem<HD>::total, "cross attention dQ"))) return rc;
   if ((rc = reserve(cross_dkdv_umma_kernel<T, HD>, DkSmem<HD>::total, "cross attention dK/dV"))) return rc;
   const int64_t qtiles = (a.Lq + kRows - 1) / kRows, items = a.B * a.H * qtiles, ktiles = (a.Lkv + kRows - 1) / kRows;
   const int64_t units = a.B * a.Hkv * ktiles * splits;
   if (items > 0x3fffffff || units > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention backward: too many rows");
   const int64_t sms = device_sms();
-  cross_dq_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kDqThreads, DqSmem<HD>::total, st>>>(mq, mdo, mk, mv, a, (int)qtiles, (int)items,
-                                                                                                       status);
+  cross_dq_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kDqThreads, DqSmem<HD>::total, st>>>(
+      mq, mdo, mk, mv, mdq, a, Divisor((uint32_t)qtiles), Divisor((uint32_t)a.H), Divisor((uint32_t)(a.H / a.Hkv)), (int)items, status);
   if ((rc = check_launch("cross_dq_umma_kernel"))) return rc;
   cross_dkdv_umma_kernel<T, HD><<<(unsigned)units, kDkThreads, DkSmem<HD>::total, st>>>(mq64, mdo64, mk, mv, a, (int)ktiles, splits, part, status);
   return check_launch("cross_dkdv_umma_kernel");
@@ -1155,7 +1236,7 @@ bool aligned(const void* p, const int64_t (&s)[3], int64_t heads, int64_t rows, 
 bool cross_umma_shape(int D, int dtype) { return (dtype == VSA_BF16 || dtype == VSA_F16) && D % 8 == 0 && D >= 8 && D <= 128; }
 
 bool cross_umma_eligible(const VsaCross& a, bool backward) {
-  if (!cross_umma_shape(a.D, a.dtype) || a.Lkv < 1 || a.Lq < 1) return false;
+  if (!cross_umma_shape(a.D, a.dtype) || a.Lkv < 1 || a.Lq < 1 || !(a.scale > 0.f)) return false;
   if (!aligned(a.q, a.q_stride, a.H, a.Lq, a.B) || !aligned(a.k, a.k_stride, a.Hkv, a.Lkv, a.B) || !aligned(a.v, a.v_stride, a.Hkv, a.Lkv, a.B) ||
       !aligned(a.out, a.out_stride, a.H, a.Lq, a.B))
     return false;

@@ -425,7 +425,7 @@ int wait_timeout_selftest(unsigned long long limit_ns, int* gave_up, cudaStream_
 }
 
 int make_map_rows(CUtensorMap* map, CUtensorMapDataType elem, const void* ptr, int64_t dim, int64_t rows, int64_t heads, int64_t batch,
-                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows, const char* what) {
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows, const char* what, int box_dims) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(VSA_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled is not available from the driver", what);
   if (reinterpret_cast<uintptr_t>(ptr) % 16) return fail(VSA_ERR_BAD_ARGUMENT, "%s: pointer is not 16-byte aligned", what);
@@ -438,9 +438,9 @@ int make_map_rows(CUtensorMap* map, CUtensorMapDataType elem, const void* ptr, i
     gstride[i] = (cuuint64_t)s * 2;
   }
   const cuuint64_t gdim[4] = {(cuuint64_t)dim, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
-  const CUresult r = fn(map, elem, 4, const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t box[4] = {(cuuint32_t)box_dims, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, elem, 4, const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        box_dims == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(VSA_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed with code %d", what, (int)r);
   return VSA_OK;
 }

@@ -9,9 +9,9 @@
 namespace vsa {
 
 // Host side, sparse_umma.cu: a [batch, heads, rows, dim] operand of a 16-bit type with any strides (in elements, multiples of 8), boxes of
-// box_rows rows x 64 dims of one slice, 128-byte swizzle; the address of the status word on the current device.
+// box_rows rows x 64 dims of one slice, 128-byte swizzle (32 dims: 64-byte swizzle); the address of the status word on the current device.
 int make_map_rows(CUtensorMap* map, CUtensorMapDataType elem, const void* ptr, int64_t dim, int64_t rows, int64_t heads, int64_t batch,
-                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows, const char* what);
+                  int64_t row_stride, int64_t head_stride, int64_t batch_stride, int box_rows, const char* what, int box_dims = 64);
 int device_status_word(int** word);
 int device_sms();
 
@@ -128,6 +128,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
+// One 4-D box shared -> global (what lies outside the tensor is not written); reads and writes counted in bulk groups of the thread.
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
