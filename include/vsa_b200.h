@@ -479,7 +479,8 @@ int vsa_rotary(const VsaRotary* a, void* stream);
  *   lse2      [B * H, Lq rounded up to 128] fp32: base-2 log-sum-exp of the scaled scores, +inf for rows without a live key and
  *             for the padding; written by the forward, read by the backward
  *   delta     the same shape, scratch of the backward
- *   workspace vsa_cross_workspace_bytes(backward, ...) bytes (0: may be NULL), 16-byte aligned, free again after the call
+ *   workspace vsa_cross_workspace_bytes(backward, ..., key_bits != NULL) bytes (0: may be NULL), 16-byte aligned, free again after the
+ *             call
  * bf16 and fp16 with head dims that are multiples of 8 up to 128, 16-byte aligned pointers and strides of multiples of 8 run on
  * tcgen05 kernels (vsa_cross_on_tensor_cores), everything else up to head dim 256 on CUDA cores in fp32.  Results do not
  * depend on the order in which blocks run.  No reference counterpart (its operator is self-attention over one token grid). */
@@ -499,7 +500,8 @@ typedef struct VsaCross {
 int vsa_cross_fwd(const VsaCross* a, void* stream);
 int vsa_cross_bwd(const VsaCross* a, void* stream);
 int vsa_cross_on_tensor_cores(const VsaCross* a, int backward);
-int64_t vsa_cross_workspace_bytes(int backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype);
+int64_t vsa_cross_workspace_bytes(int backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype,
+                                  int with_mask);
 int64_t vsa_cross_words(int64_t Lkv);
 /* mask [B, Lkv] bytes, rows mask_stride apart: non-zero = live. */
 int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* kv_lengths, uint32_t* key_bits, int64_t B, int64_t Lkv,

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -38,7 +39,9 @@ class OperatorBwd(ctypes.Structure):
 
 
 class Rotary(ctypes.Structure):
-    """``VsaRotary`` of the header."""
+    """``VsaRotary`` of the header.  ``PACK`` is the same layout for one ``struct.pack`` of all fields in order, which is
+    some ten times faster than assigning them (None is 0 there)."""
+    PACK = struct.Struct("@8P5q12q2i5i0q")
     _fields_ = [("x", P * 2), ("y", P * 2)] + [(n, P) for n in ("cos_table", "sin_table", "positions", "src_map")] + \
                [(n, L) for n in ("B", "rows", "src_rows", "table_rows", "positions_stride")] + \
                [("x_stride", (L * 3) * 2), ("y_stride", (L * 3) * 2), ("heads", I * 2)] + \
@@ -46,7 +49,8 @@ class Rotary(ctypes.Structure):
 
 
 class Cross(ctypes.Structure):
-    """``VsaCross`` of the header."""
+    """``VsaCross`` of the header; ``PACK`` as in ``Rotary``."""
+    PACK = struct.Struct("@13P5q24qf2i0q")
     _fields_ = [(n, P) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "lse2", "delta", "kv_lengths", "key_bits",
                                  "workspace")] + \
                [(n, L) for n in ("B", "H", "Hkv", "Lq", "Lkv")] + \
@@ -108,7 +112,7 @@ PLAIN = {"vsa_last_error_string": ([], c_char_p), "vsa_version": ([], c_int),
          "vsa_sparse_pass_kernels": ([I, L, L, I, I, I, I], c_int),
          "vsa_sparse_bwd_ds_workspace_bytes": ([L, L, I, I], c_int64),
          "vsa_cross_on_tensor_cores": ([ctypes.POINTER(Cross), I], c_int),
-         "vsa_cross_workspace_bytes": ([I, L, L, L, L, L, I, I], c_int64),
+         "vsa_cross_workspace_bytes": ([I, L, L, L, L, L, I, I, I], c_int64),
          "vsa_cross_words": ([L], c_int64)}
 
 

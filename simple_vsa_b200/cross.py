@@ -21,38 +21,40 @@ from ._lib import call
 def _usable(x: Tensor) -> Tensor:
     """The tensor itself where its rows can be read in place, else a dense copy: head dim contiguous, and in 16-bit types with
     head dims of whole 16-byte pieces everything on 16-byte boundaries (other rows run on CUDA cores, element by element)."""
-    if x.shape[3] > 1 and x.stride(3) != 1:
+    shape, stride = x.shape, x.stride()
+    if shape[3] > 1 and stride[3] != 1:
         return x.contiguous()
-    if x.element_size() == 2 and x.shape[3] % 8 == 0:
-        steps = [s for s, n in zip(x.stride()[:3], x.shape[:3]) if n > 1]
-        if x.data_ptr() % 16 or any(s % 8 or s <= 0 for s in steps):
-            return ops._dense(x)
+    if shape[3] % 8 == 0 and x.dtype != torch.float32:
+        if x.data_ptr() % 16 or (stride[0] | stride[1] | stride[2]) % 8 or not (stride[0] and stride[1] and stride[2]):
+            if x.data_ptr() % 16 or any(n > 1 and (s % 8 or s == 0) for s, n in zip(stride[:3], shape[:3])):
+                return ops._dense(x)
     return x
 
 
-def _arguments(q, k, v, kv_lengths, key_bits, scale: float, dt: int) -> _lib.Cross:
-    a = _lib.Cross()
-    a.B, a.H, a.Lq, a.D = q.shape
-    a.Hkv, a.Lkv = k.shape[1], k.shape[2]
-    a.scale, a.dtype = scale, dt
-    a.kv_lengths, a.key_bits = ops._ptr(kv_lengths), ops._ptr(key_bits)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _operand(a, name, t)
-    return a
+_NO_STRIDES = (0, 0, 0)
 
 
-def _operand(a: _lib.Cross, name: str, t: Tensor) -> None:
-    setattr(a, name, t.data_ptr())
-    getattr(a, name + "_stride")[:] = t.stride()[:3]
+def _launch(name: str, backward: int, scale: float, dt: int, q, k, v, out, lse, kv_lengths, key_bits, dout=None, dq=None, dk=None,
+            dv=None, delta=None) -> None:
+    B, H, Lq, D = q.shape
+    Hkv, Lkv = k.shape[1], k.shape[2]
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    n = _lib.lib.vsa_cross_workspace_bytes(backward, B, H, Hkv, Lq, Lkv, D, dt, key_bits is not None)
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n > 0 else None
+    grads = (*dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]) if backward else _NO_STRIDES * 4
+    a = _lib.Cross.from_buffer_copy(_lib.Cross.PACK.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(dout), out.data_ptr(), ptr(dq), ptr(dk), ptr(dv), lse.data_ptr(), ptr(delta),
+        ptr(kv_lengths), ptr(key_bits), ptr(ws), B, H, Hkv, Lq, Lkv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        *out.stride()[:3], *grads, scale, D, dt))
+    call(name, a, ops._stream(q.device))
 
 
-def _workspace(a: _lib.Cross, backward: int, device) -> Optional[Tensor]:
-    n = _lib.lib.vsa_cross_workspace_bytes(backward, a.B, a.H, a.Hkv, a.Lq, a.Lkv, a.D, a.dtype)
-    if n <= 0:
-        return None
-    ws = torch.empty(n, device=device, dtype=torch.uint8)
-    a.workspace = ws.data_ptr()
-    return ws
+def _forward(q, k, v, kv_lengths, key_bits, scale: float):
+    B, H, L, D = q.shape
+    out = torch.empty_like(q)
+    lse = torch.empty((B * H, -(-L // 128) * 128), device=q.device, dtype=torch.float32)
+    _launch("vsa_cross_fwd", 0, scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits)
+    return out, lse
 
 
 def _key_bits(kv_mask: Tensor, kv_lengths: Optional[Tensor]) -> Tensor:
@@ -66,36 +68,20 @@ def _key_bits(kv_mask: Tensor, kv_lengths: Optional[Tensor]) -> Tensor:
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, kv_lengths, key_bits, scale, need_grad):
-        B, H, L, D = q.shape
-        dt = ops._check_device_dtype(q, k, v)
-        out = torch.empty_like(q)
-        lse = torch.empty((B * H, -(-L // 128) * 128), device=q.device, dtype=torch.float32)
-        a = _arguments(q, k, v, kv_lengths, key_bits, scale, dt)
-        _operand(a, "out", out)
-        a.lse2 = lse.data_ptr()
-        ws = _workspace(a, 0, q.device)  # noqa: F841  alive until the launch
-        call("vsa_cross_fwd", a, ops._stream(q.device))
-        if need_grad:
-            ctx.save_for_backward(q, k, v, out, lse, kv_lengths, key_bits)
-            ctx.scale = scale
+    def forward(ctx, q, k, v, kv_lengths, key_bits, scale):
+        out, lse = _forward(q, k, v, kv_lengths, key_bits, scale)
+        ctx.save_for_backward(q, k, v, out, lse, kv_lengths, key_bits)
+        ctx.scale = scale
         return out
 
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, key_bits = ctx.saved_tensors
         with torch.cuda.device(q.device):
-            dt = ops._check_device_dtype(q, k, v)
-            dout = _usable(dout)
-            a = _arguments(q, k, v, kv_lengths, key_bits, ctx.scale, dt)
-            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-            delta = torch.empty_like(lse)
-            for name, t in (("out", out), ("dout", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
-                _operand(a, name, t)
-            a.lse2, a.delta = lse.data_ptr(), delta.data_ptr()
-            ws = _workspace(a, 1, q.device)  # noqa: F841
-            call("vsa_cross_bwd", a, ops._stream(q.device))
-        return dq, dk, dv, None, None, None, None
+            dq, dk, dv, delta = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), torch.empty_like(lse)
+            _launch("vsa_cross_bwd", 1, ctx.scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits,
+                    _usable(dout), dq, dk, dv, delta)
+        return dq, dk, dv, None, None, None
 
 
 def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
@@ -135,7 +121,8 @@ def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
             key_bits = _key_bits(kv_mask if T <= 1 or kv_mask.stride(1) == 1 else kv_mask.contiguous(), kv_lengths)
         q, k, v = _usable(q), _usable(k), _usable(v)
         need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-        out = _CrossAttention.apply(q, k, v, kv_lengths, key_bits, scale, need_grad)
+        out = _CrossAttention.apply(q, k, v, kv_lengths, key_bits, scale) if need_grad else \
+            _forward(q, k, v, kv_lengths, key_bits, scale)[0]
     return out.transpose(1, 2) if raster else out
 
 

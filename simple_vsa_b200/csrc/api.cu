@@ -665,15 +665,30 @@ static bool cross_extents_fine(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, in
 
 int64_t vsa_cross_words(int64_t Lkv) { return Lkv < 0 ? -1 : cross_words(Lkv); }
 
-int64_t vsa_cross_workspace_bytes(int backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
+// The workspace: partial results, then what a compaction of the keys needs (16-bit types with a mask).
+struct CrossSpace {
+  int splits;
+  int64_t parts, prefix, counts, k, v, bytes;      // byte offsets behind the partial results, which begin at 0
+};
+static CrossSpace cross_space(bool backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype, bool mask) {
+  CrossSpace s{1, 0, 0, 0, 0, 0, 0};
+  if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return s;
+  const bool compact = mask && cross_umma_shape(D, dtype);
+  s.splits = backward ? cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype) : cross_fwd_splits(B, H, Lq, Lkv, D, dtype);
+  if (!backward) s.parts = s.splits == 1 ? 0 : s.splits * B * H * Lq * (int64_t)(D + 1) * 4;
+  else s.parts = s.splits == 1 && !compact ? 0 : s.splits * 2 * B * Hkv * Lkv * (int64_t)D * 4;
+  s.parts = (s.parts + 15) / 16 * 16;
+  s.prefix = s.parts;
+  s.counts = s.prefix + (compact ? B * cross_words(Lkv) * 4 : 0);
+  s.k = (s.counts + (compact ? B * 4 : 0) + 15) / 16 * 16;
+  s.v = s.k + (compact ? B * Hkv * Lkv * (int64_t)D * 2 : 0);
+  s.bytes = s.v + (compact ? B * Hkv * Lkv * (int64_t)D * 2 : 0);
+  return s;
+}
+
+int64_t vsa_cross_workspace_bytes(int backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype, int with_mask) {
   if (!cross_extents_fine(B, H, Hkv, Lq, Lkv, D) || (dtype != VSA_BF16 && dtype != VSA_F32 && dtype != VSA_F16)) return -1;
-  if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return 0;
-  if (!backward) {
-    const int64_t s = cross_fwd_splits(B, H, Lq, Lkv, D, dtype);
-    return s == 1 ? 0 : s * B * H * Lq * (D + 1) * 4;
-  }
-  const int64_t s = cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype);
-  return s == 1 ? 0 : s * 2 * B * Hkv * Lkv * D * 4;
+  return cross_space(backward != 0, B, H, Hkv, Lq, Lkv, D, dtype, with_mask != 0).bytes;
 }
 
 static int check_cross(const VsaCross* a, bool backward, const char* what) {
@@ -690,7 +705,7 @@ static int check_cross(const VsaCross* a, bool backward, const char* what) {
   VSA_REQUIRE(!rows || !keys || (a->k && a->v), "%s: null pointer", what);
   VSA_REQUIRE(!backward || !rows || (a->dout && a->dq && a->delta), "%s: null pointer", what);
   VSA_REQUIRE(!backward || !keys || (a->dk && a->dv), "%s: null pointer", what);
-  VSA_REQUIRE(a->workspace || vsa_cross_workspace_bytes(backward, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype) == 0,
+  VSA_REQUIRE(a->workspace || cross_space(backward, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr).bytes == 0,
               "%s: a workspace is needed", what);
   VSA_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "%s: the workspace is not 16-byte aligned", what);
   return VSA_OK;
@@ -708,16 +723,37 @@ static bool cross_on_umma(const VsaCross& a, bool backward) { return !scalar_for
 
 int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) { return a != nullptr && cross_on_umma(*a, backward != 0) ? 1 : 0; }
 
+// The call on compacted keys: dense K and V of which the first counts[b] rows of a sample take part.
+static int compacted(const VsaCross& a, const CrossSpace& s, VsaCross* out, cudaStream_t st) {
+  uint8_t* ws = (uint8_t*)a.workspace;
+  *out = a;
+  out->key_bits = nullptr;
+  out->kv_lengths = (const int32_t*)(ws + s.counts);
+  out->k = ws + s.k;
+  out->v = ws + s.v;
+  const int64_t dense[3] = {a.Hkv * a.Lkv * a.D, a.Lkv * a.D, a.D};
+  for (int i = 0; i < 3; ++i) out->k_stride[i] = out->v_stride[i] = dense[i];
+  return cross_compact(a, (int32_t*)(ws + s.prefix), (int32_t*)(ws + s.counts), ws + s.k, ws + s.v, st);
+}
+
 int vsa_cross_fwd(const VsaCross* a, void* stream) {
   int rc = check_cross(a, false, "cross attention forward");
   if (rc || a->B == 0 || a->H == 0 || a->Lq == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  const int splits = a->Lkv == 0 ? 1 : cross_fwd_splits(a->B, a->H, a->Lq, a->Lkv, a->D, a->dtype);
+  const CrossSpace s = cross_space(false, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr);
   float* part_out = (float*)a->workspace;
-  float* part_lse = part_out + (splits == 1 ? 0 : splits * a->B * a->H * a->Lq * a->D);
-  rc = cross_on_umma(*a, false) ? cross_fwd_umma(*a, splits, part_out, part_lse, st) : cross_fwd_generic(*a, splits, part_out, part_lse, st);
+  float* part_lse = part_out + (s.splits == 1 ? 0 : s.splits * a->B * a->H * a->Lq * a->D);
+  if (!cross_on_umma(*a, false)) {
+    rc = cross_fwd_generic(*a, s.splits, part_out, part_lse, st);
+  } else if (a->key_bits == nullptr) {
+    rc = cross_fwd_umma(*a, s.splits, part_out, part_lse, st);
+  } else {
+    VsaCross c;
+    if ((rc = compacted(*a, s, &c, st))) return rc;
+    rc = cross_fwd_umma(c, s.splits, part_out, part_lse, st);
+  }
   if (rc) return rc;
-  return splits == 1 ? VSA_OK : cross_join(*a, splits, part_out, part_lse, st);
+  return s.splits == 1 ? VSA_OK : cross_join(*a, s.splits, part_out, part_lse, st);
 }
 
 int vsa_cross_bwd(const VsaCross* a, void* stream) {
@@ -725,10 +761,16 @@ int vsa_cross_bwd(const VsaCross* a, void* stream) {
   if (rc || a->B == 0 || a->Hkv == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (a->Lq == 0 || a->H == 0) return a->Lkv == 0 ? VSA_OK : cross_sum(*a, 0, nullptr, st);       // no query: zeros
-  const int splits = a->Lkv == 0 ? 1 : cross_bwd_splits(a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype);
-  rc = cross_on_umma(*a, true) ? cross_bwd_umma(*a, splits, (float*)a->workspace, st) : cross_bwd_generic(*a, splits, (float*)a->workspace, st);
-  if (rc) return rc;
-  return splits == 1 ? VSA_OK : cross_sum(*a, splits, (const float*)a->workspace, st);
+  const CrossSpace s = cross_space(true, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr);
+  float* part = (float*)a->workspace;
+  if (!cross_on_umma(*a, true) || a->key_bits == nullptr) {
+    const bool parts = s.splits > 1;
+    rc = cross_on_umma(*a, true) ? cross_bwd_umma(*a, s.splits, parts, part, st) : cross_bwd_generic(*a, s.splits, part, st);
+    return rc || !parts ? rc : cross_sum(*a, s.splits, part, st);
+  }
+  VsaCross c;
+  if ((rc = compacted(*a, s, &c, st)) || (rc = cross_bwd_umma(c, s.splits, true, part, st))) return rc;
+  return cross_sum(*a, s.splits, part, st, (const int32_t*)((uint8_t*)a->workspace + s.prefix));
 }
 
 int vsa_rotary(const VsaRotary* a, void* stream) {

@@ -18,9 +18,9 @@ template <typename T> __device__ __forceinline__ T from_f(float x) { return Elem
 template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
 
 // DP: head dim rounded up; KT: tile edge; P: patch edge
-template <int DP_>
+template <int DP_, int KT_ = (DP_ > 128 ? 32 : 64)>
 struct Tile {
-  static constexpr int DP = DP_, KT = DP_ > 128 ? 32 : 64, P = KT / 16, PITCH = DP_ + 4, SPITCH = KT + 4;
+  static constexpr int DP = DP_, KT = KT_, P = KT / 16, PITCH = DP_ + 4, SPITCH = KT + 4;
   static constexpr int floats = KT * PITCH, score_floats = KT * SPITCH;
 };
 
@@ -384,20 +384,6 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const __grid_constant__
   for (long long i = at; i < pads; i += step) a.lse2[(i / pad) * lp + a.Lq + i % pad] = INFINITY;
 }
 
-// dK and dV: the parts are added in the order of the splits, whatever ran first.
-template <typename T>
-__global__ void __launch_bounds__(256) cross_sum_kernel(const __grid_constant__ VsaCross a, int splits, const float* __restrict__ part) {
-  const long long one = (long long)a.B * a.Hkv * a.Lkv * a.D;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < 2 * one; i += (long long)gridDim.x * 256) {
-    const bool is_v = i >= one;
-    const long long e = is_v ? i - one : i, row = e / a.D, bh = row / a.Lkv, l = row - bh * a.Lkv;
-    float x = 0.f;
-    for (int s = 0; s < splits; ++s) x += part[(2 * s + is_v) * one + e];
-    const int64_t(&st)[3] = is_v ? a.dv_stride : a.dk_stride;
-    ((T*)(is_v ? a.dv : a.dk))[(bh / a.Hkv) * st[0] + (bh % a.Hkv) * st[1] + l * st[2] + (e - row * a.D)] = from_f<T>(x);
-  }
-}
-
 __global__ void __launch_bounds__(256) cross_bits_kernel(const uint8_t* __restrict__ mask, long long stride, const int32_t* __restrict__ lengths,
                                                          uint32_t* __restrict__ bits, long long Lkv, long long words) {
   const int b = blockIdx.y;
@@ -407,6 +393,109 @@ __global__ void __launch_bounds__(256) cross_bits_kernel(const uint8_t* __restri
   if (lengths != nullptr) len = min(len, (long long)max(0, lengths[b]));
   const unsigned word = __ballot_sync(0xffffffffu, key < len && mask[b * stride + key] != 0);
   if ((threadIdx.x & 31) == 0) bits[b * words + w] = word;
+}
+
+// ---- compacted keys ---------------------------------------------------------------------------------------------------------
+// The tensor path knows lengths only: with a mask, the rows of K and V that take part are gathered into dense tensors first (a few MB,
+// once per call, against a select per score and the clearing of rows of V in every tile: forward 135 us at [2, 12 + 4, 8190, 64] x
+// 1001 keys, 78 with them compacted), in their order; their gradients go back the same way when the parts are added.
+// prefix [B][words]: live keys of the sample before each word; counts [B].
+__global__ void __launch_bounds__(1024) cross_rank_kernel(const uint32_t* __restrict__ bits, int words, int32_t* __restrict__ prefix,
+                                                          int32_t* __restrict__ counts) {
+  __shared__ int warp_sums[32];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int before = 0;
+  for (int w0 = 0; w0 < words; w0 += 1024) {
+    const int n = w0 + tid < words ? __popc(bits[(long long)b * words + w0 + tid]) : 0;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+      int s = warp_sums[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      warp_sums[lane] = s;
+    }
+    __syncthreads();
+    if (w0 + tid < words) prefix[(long long)b * words + w0 + tid] = before + x - n + (warp ? warp_sums[warp - 1] : 0);
+    before += warp_sums[31];
+    __syncthreads();
+  }
+  if (tid == 0) counts[b] = before;
+}
+
+// The place of key l among the live ones of its sample, or -1.
+__device__ __forceinline__ int rank_of(const uint32_t* bits, const int32_t* prefix, long long b, int words, int l) {
+  const long long w = b * words + (l >> 5);
+  const uint32_t word = bits[w], bit = 1u << (l & 31);
+  return word & bit ? prefix[w] + __popc(word & (bit - 1u)) : -1;
+}
+
+// One 16-byte piece of a row a thread: K and V rows to their places, zeros behind the last one.
+__global__ void __launch_bounds__(256) cross_compact_kernel(const __grid_constant__ VsaCross a, const int32_t* __restrict__ prefix,
+                                                            const int32_t* __restrict__ counts, uint4* __restrict__ k_out, uint4* __restrict__ v_out) {
+  const unsigned per_row = (unsigned)(a.D / 8), rows = (unsigned)(a.B * a.Hkv * a.Lkv);
+  const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= rows) return;
+  const unsigned bh = row / (unsigned)a.Lkv, b = bh / (unsigned)a.Hkv, h = bh - b * (unsigned)a.Hkv;
+  const int l = (int)(row - bh * (unsigned)a.Lkv), words = (int)cross_words(a.Lkv);
+  const int to = rank_of(a.key_bits, prefix, b, words, l);
+  const bool behind = l >= counts[b];
+  const __half* k = (const __half*)a.k + b * a.k_stride[0] + h * a.k_stride[1] + l * a.k_stride[2];      // any 16-bit type
+  const __half* v = (const __half*)a.v + b * a.v_stride[0] + h * a.v_stride[1] + l * a.v_stride[2];
+  for (unsigned c = threadIdx.x; c < per_row; c += blockDim.x) {
+    const size_t at = (size_t)bh * a.Lkv;
+    if (to >= 0) {
+      k_out[(at + to) * per_row + c] = reinterpret_cast<const uint4*>(k)[c];
+      v_out[(at + to) * per_row + c] = reinterpret_cast<const uint4*>(v)[c];
+    }
+    if (behind) k_out[(at + l) * per_row + c] = v_out[(at + l) * per_row + c] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// dK and dV: the parts are added in the order of the splits, whatever ran first.  A thread owns W neighbouring dims of a key row; the
+// loads of eight parts fly together (bound by their latency: a few MB).  With `prefix` the parts' rows are those of the compacted keys.
+template <typename T, int W>
+__global__ void __launch_bounds__(256) cross_sum_kernel(const __grid_constant__ VsaCross a, int splits, const float* __restrict__ part,
+                                                        const int32_t* __restrict__ prefix) {
+  struct alignas(4 * W) Floats { float v[W]; };
+  struct alignas(W * sizeof(T)) Values { T v[W]; };
+  const long long one = (long long)a.B * a.Hkv * a.Lkv * a.D;
+  const unsigned per_row = (unsigned)(a.D / W), rows = (unsigned)(a.B * a.Hkv * a.Lkv);
+  const unsigned row = blockIdx.x * blockDim.y + threadIdx.y, is_v = blockIdx.y;
+  if (row >= rows) return;
+  const unsigned bh = row / (unsigned)a.Lkv, l = row - bh * (unsigned)a.Lkv, b = bh / (unsigned)a.Hkv;
+  const int64_t(&st)[3] = is_v ? a.dv_stride : a.dk_stride;
+  const int from = prefix == nullptr ? (int)l : rank_of(a.key_bits, prefix, b, (int)cross_words(a.Lkv), (int)l);
+  if (from < 0) splits = 0;            // a key that takes no part
+  T* out = (T*)(is_v ? a.dv : a.dk) + b * st[0] + (bh - b * (unsigned)a.Hkv) * st[1] + l * st[2];
+  for (unsigned c = threadIdx.x; c < per_row; c += blockDim.x) {
+    const float* p = part + is_v * one + ((long long)bh * a.Lkv + from) * a.D + c * W;
+    float sum[W] = {};
+    for (int s = 0; s < splits; s += 8) {
+      Floats x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s + i < splits) x[i] = *reinterpret_cast<const Floats*>(p + 2 * (s + i) * one);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          if (s + i < splits) sum[j] += x[i].v[j];
+    }
+    Values y;
+#pragma unroll
+    for (int j = 0; j < W; ++j) y.v[j] = from_f<T>(sum[j]);
+    *reinterpret_cast<Values*>(out + c * W) = y;
+  }
 }
 
 bool vec4(const VsaCross& a, bool backward) {      // 16-byte reads of fp32 rows
@@ -435,15 +524,21 @@ int fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStr
   return check_launch("cross_fwd_generic_kernel");
 }
 template <typename T, typename TL>
-int bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
-  int bytes = (4 * TL::floats + TL::score_floats) * 4;
-  int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
+int dq_pass(const VsaCross& a, cudaStream_t st) {
+  const int bytes = (4 * TL::floats + TL::score_floats) * 4;
+  const int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
   if (rc) return rc;
   cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::KT - 1) / TL::KT), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
       a, vec4(a, true));
-  if ((rc = check_launch("cross_dq_generic_kernel"))) return rc;
-  if (a.Lkv == 0) return VSA_OK;
-  bytes = (4 * TL::floats + 2 * TL::score_floats) * 4;
+  return check_launch("cross_dq_generic_kernel");
+}
+template <typename T, typename TL>
+int bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  // dQ on tiles of 32 x 32 where tiles of 64 leave SMs without work ([1, 2, 1025, 64] x 333: 34 CTAs, 67 us; 66 CTAs, 58)
+  using Small = Tile<TL::DP, 32>;
+  int rc = TL::KT == 64 && a.B * a.H * ((a.Lq + 63) / 64) < 148 ? dq_pass<T, Small>(a, st) : dq_pass<T, TL>(a, st);
+  if (rc || a.Lkv == 0) return rc;
+  const int bytes = (4 * TL::floats + 2 * TL::score_floats) * 4;
   if ((rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV"))) return rc;
   cross_dkdv_generic_kernel<T, TL><<<dim3((unsigned)((a.Lkv + TL::KT - 1) / TL::KT * splits), (unsigned)a.Hkv, (unsigned)a.B), kThreads, bytes,
                                      st>>>(a, splits, part, vec4(a, true));
@@ -470,13 +565,32 @@ int cross_join(const VsaCross& a, int splits, const float* part_out, const float
   else cross_join_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, splits, part_out, part_lse);
   return check_launch("cross_join_kernel");
 }
-int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st) {
-  const int64_t n = 2 * a.B * a.Hkv * a.Lkv * a.D;
-  const unsigned blocks = (unsigned)(n / 256 + 1 < 148 * 8 ? n / 256 + 1 : 148 * 8);
-  if (a.dtype == VSA_F32) cross_sum_kernel<float><<<blocks, 256, 0, st>>>(a, splits, part);
-  else if (a.dtype == VSA_F16) cross_sum_kernel<__half><<<blocks, 256, 0, st>>>(a, splits, part);
-  else cross_sum_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a, splits, part);
+template <typename T>
+static int sum_of(const VsaCross& a, int splits, const float* part, const int32_t* prefix, cudaStream_t st) {
+  // four dims a thread where rows and their places allow it
+  bool wide = a.D % 4 == 0;
+  for (int i = 0; i < 3; ++i) wide = wide && a.dk_stride[i] % 4 == 0 && a.dv_stride[i] % 4 == 0;
+  wide = wide && reinterpret_cast<uintptr_t>(a.dk) % 16 == 0 && reinterpret_cast<uintptr_t>(a.dv) % 16 == 0;
+  const int64_t rows = a.B * a.Hkv * a.Lkv;
+  if (rows > 0x7fffffffLL) return fail(VSA_ERR_UNSUPPORTED, "cross attention backward: too many key rows");
+  const int cols = a.D / (wide ? 4 : 1), x = cols <= 16 ? 16 : cols <= 32 ? 32 : 64, y = 256 / x;
+  const dim3 grid((unsigned)((rows + y - 1) / y), 2), block((unsigned)x, (unsigned)y);
+  if (wide) cross_sum_kernel<T, 4><<<grid, block, 0, st>>>(a, splits, part, prefix);
+  else cross_sum_kernel<T, 1><<<grid, block, 0, st>>>(a, splits, part, prefix);
   return check_launch("cross_sum_kernel");
+}
+int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st, const int32_t* prefix) {
+  if (a.dtype == VSA_F32) return sum_of<float>(a, splits, part, prefix, st);
+  return a.dtype == VSA_F16 ? sum_of<__half>(a, splits, part, prefix, st) : sum_of<__nv_bfloat16>(a, splits, part, prefix, st);
+}
+int cross_compact(const VsaCross& a, int32_t* prefix, int32_t* counts, void* k, void* v, cudaStream_t st) {
+  cross_rank_kernel<<<(unsigned)a.B, 1024, 0, st>>>(a.key_bits, (int)cross_words(a.Lkv), prefix, counts);
+  const int rc = check_launch("cross_rank_kernel");
+  if (rc) return rc;
+  const int x = a.D <= 64 ? 8 : 16, y = 256 / x;
+  const int64_t rows = a.B * a.Hkv * a.Lkv;
+  cross_compact_kernel<<<(unsigned)((rows + y - 1) / y), dim3((unsigned)x, (unsigned)y), 0, st>>>(a, prefix, counts, (uint4*)k, (uint4*)v);
+  return check_launch("cross_compact_kernel");
 }
 int cross_key_bits(const uint8_t* mask, int64_t stride, const int32_t* lengths, uint32_t* bits, int64_t B, int64_t Lkv, cudaStream_t st) {
   const int64_t words = cross_words(Lkv);

@@ -6,7 +6,7 @@
 // work to the next.
 #include <cuda.h>
 
-#include <type_traits>
+#include <atomic>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -90,8 +90,6 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
   for (int h = 0; h < HD / 64; ++h) tma_load_4d(dst + h * half_bytes, map, h * 64, row, head, batch, bar);
 }
 
-__device__ __forceinline__ uint32_t first_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
-
 __device__ __forceinline__ float max3(float x, uint32_t y, uint32_t z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(__uint_as_float(y)), "f"(__uint_as_float(z)));
@@ -124,28 +122,6 @@ __device__ __forceinline__ float2 poly_exp2(float2 x) {
 template <typename T>
 __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
   return poly ? poly_exp2<T>(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
-}
-
-// Live keys of tile j of a sample: a bit each.
-struct TileKeys {
-  uint32_t w[4];
-  __device__ __forceinline__ bool full() const { return (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu; }
-  __device__ __forceinline__ bool bit(int key) const {
-    const uint32_t x = key < 64 ? (key < 32 ? w[0] : w[1]) : (key < 96 ? w[2] : w[3]);
-    return x >> (key & 31) & 1u;
-  }
-};
-__device__ __forceinline__ TileKeys tile_keys(const VsaCross& a, int b, int len, int j) {
-  TileKeys t;
-  if (a.key_bits != nullptr) {
-    const uint4 x = *reinterpret_cast<const uint4*>(a.key_bits + (long long)b * cross_words(a.Lkv) + j * 4);
-    t.w[0] = x.x, t.w[1] = x.y, t.w[2] = x.z, t.w[3] = x.w;
-  } else {
-    const int left = len - j * kRows;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.w[i] = first_bits(left - 32 * i);
-  }
-  return t;
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -267,14 +243,8 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       float2 lsum = make_float2(0.f, 0.f);
       for (int i = 0; i < halves; ++i, ++u) {
         const int key0 = it.j0 * kRows + i * kKeys;
-        uint32_t w0 = 0xffffffffu, w1 = 0xffffffffu;               // the live keys of this step
-        if (a.key_bits != nullptr) {
-          const uint2 x = *reinterpret_cast<const uint2*>(a.key_bits + (long long)it.b * cross_words(a.Lkv) + (key0 >> 5));
-          w0 = x.x, w1 = x.y;
-        } else if (it.len - key0 < kKeys) {
-          w0 = first_bits(it.len - key0), w1 = first_bits(it.len - key0 - 32);
-        }
-        const bool full = (w0 & w1) == 0xffffffffu;
+        const int live = it.len - key0;                            // keys of this step that take part, or more
+        const bool full = live >= kKeys;
         const int acc = 2 * t + (u & 1);
         const uint32_t s_addr = tmem + 64 * acc + lane_addr;
         ok = CROSS_WAIT(bar(F_S_FULL + acc), (u >> 1) & 1);
@@ -287,8 +257,8 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (!full) {                               // what stands in a key that takes no part may be anything: P = 2^-inf
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            if (!(w0 >> e & 1u)) sv[0][e] = 0xff800000u;
-            if (!(w1 >> e & 1u)) sv[1][e] = 0xff800000u;
+            if (e >= live) sv[0][e] = 0xff800000u;
+            if (32 + e >= live) sv[1][e] = 0xff800000u;
           }
         }
         float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -325,7 +295,7 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           ok = CROSS_WAIT(bar(F_KV_FULL + s), (r / Sm::stages) & 1);
           if (!ok) break;
           const int vr = (i & 1) * kKeys + (row & 63);             // two threads a row
-          if (!((row & 32 ? w1 : w0) >> (row & 31) & 1u)) {
+          if ((row & 63) >= live) {
             uint8_t* vrow = sm + Sm::kv + s * Sm::tile + vr * 128;
 #pragma unroll
             for (int e = 0; e < HD / 16; ++e) {
@@ -781,7 +751,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const float2 l2 = make_float2(neg_lse, neg_lse), d2 = make_float2(-dl, -dl);
       for (int j = 0; j < it.n; ++j, ++n) {
         const uint32_t b = n & 1;
-        const TileKeys keys = tile_keys(a, it.b, it.len, j);
+        const int live = it.len - j * kRows;     // keys of this tile that take part, or more
         ok = CROSS_WAIT(bar(Q_S_FULL + b), (n >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
@@ -789,8 +759,8 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         uint32_t sv[kDqCols];
         tmem_ld(s_addr, sv);
         tmem_ld_wait();
-        if (!keys.full() && cg == 0) {           // rows of K that no key takes part with meet dS = 0: they must be finite (S is done)
-          if (!keys.bit(row)) {
+        if (live < kRows && cg == 0) {           // rows of K that no key takes part with meet dS = 0: they must be finite (S is done)
+          if (row >= live) {
             uint8_t* krow = sm + Sm::k + (n % Sm::k_stages) * Sm::tile + row * 128;
 #pragma unroll
             for (int ch = 0; ch < HD / 8; ++ch)
@@ -818,11 +788,12 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           const float2 y = mul2(pf[i], add2(word_pair(dv + 2 * i), d2));
           pk[i] = Elem<T>::pack(y.x, y.y);
         }
-        const uint32_t word = cg < 2 ? (cg == 0 ? keys.w[0] : keys.w[1]) : (cg == 2 ? keys.w[2] : keys.w[3]);
-        if (word != 0xffffffffu) {               // what stands in a key that takes no part may be anything
+        if (c0 + kDqCols > live) {               // what stands in a key that takes no part may be anything
 #pragma unroll
-          for (int i = 0; i < kDqCols / 2; ++i)
-            pk[i] &= (word >> (2 * i) & 1u ? 0xffffu : 0u) | (word >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+          for (int i = 0; i < kDqCols / 2; ++i) {
+            if (c0 + 2 * i >= live) pk[i] = 0u;
+            else if (c0 + 2 * i + 1 >= live) pk[i] &= 0xffffu;
+          }
         }
         tmem_st(s_addr, pk);                     // over this thread's own scores
         tmem_st_wait();
@@ -917,12 +888,11 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const int ktile = unit % ktiles, rest = unit / ktiles, split = rest % splits, bhk = rest / splits;
   const int b = bhk / (int)a.Hkv, hk = bhk - b * (int)a.Hkv, group_heads = (int)(a.H / a.Hkv);
   const int krow0 = ktile * kRows;
-  const TileKeys keys = tile_keys(a, b, cross_length(a, b), ktile);
+  const int live_keys = cross_length(a, b) - krow0;      // keys of this tile that take part, or more
   const int qtiles = (int)((a.Lq + kQTile - 1) / kQTile);
   const long long total = (long long)qtiles * group_heads, per = (total + splits - 1) / splits;
   const long long first = split * per, last = first + per < total ? first + per : total;
-  const bool any = (keys.w[0] | keys.w[1] | keys.w[2] | keys.w[3]) != 0u;
-  const int n_tiles = any && last > first ? (int)(last - first) : 0;
+  const int n_tiles = live_keys > 0 && last > first ? (int)(last - first) : 0;
   const float c = a.scale * kLog2e;
   const long long lp = cross_rows(a.Lq);
   const long long one = (long long)a.B * a.Hkv * a.Lkv * a.D;      // values of a partial dK
@@ -932,7 +902,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     for (int i = tid; i < kRows * HD / 8; i += kDkThreads) {
       const int r = i / (HD / 8), d = i % (HD / 8) * 8;
       if (krow0 + r >= a.Lkv || d >= a.D) continue;
-      if (splits == 1) {
+      if (part == nullptr) {
         *reinterpret_cast<uint4*>((T*)a.dk + b * a.dk_stride[0] + hk * a.dk_stride[1] + (krow0 + r) * a.dk_stride[2] + d) = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>((T*)a.dv + b * a.dv_stride[0] + hk * a.dv_stride[1] + (krow0 + r) * a.dv_stride[2] + d) = make_uint4(0, 0, 0, 0);
       } else {
@@ -1070,7 +1040,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int quarter = warp & 3, cg = (warp - 4) >> 2;
     const int row = quarter * 32 + lane, c0 = cg * kDkCols, st = tid - 128;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const bool live = keys.bit(row);
+    const bool live = row < live_keys;
     const float2 c2 = make_float2(-c, -c), m1 = make_float2(-1.f, -1.f);
     for (int p = 0; p < n_tiles && ok; ++p) {
       const int bf = p & 1, sq = p % Sm::q_stages;
@@ -1137,7 +1107,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const float mul = is_k ? -a.scale : 1.f;       // the products summed -dS
 #pragma unroll
         for (int i = 0; i < 32; ++i) av[i] = live ? __float_as_uint(__uint_as_float(av[i]) * mul) : 0u;
-        if (splits == 1) {
+        if (part == nullptr) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4)
             *reinterpret_cast<uint4*>((is_k ? stage_k : stage_v) + row * (HD * 2) + (((4 * jj + q4) ^ (row & 7)) << 4)) = pack8<T>(av + 8 * q4);
@@ -1148,7 +1118,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (32 * jj + i < a.D) *reinterpret_cast<uint4*>(dst + i) = make_uint4(av[i], av[i + 1], av[i + 2], av[i + 3]);
         }
       }
-      if (splits == 1) {
+      if (part == nullptr) {
         named_barrier(1, kDkEwThreads);
         for (int i = st; i < kRows * HD / 8; i += kDkEwThreads) {
           const int r = i / (HD / 8), ch = i % (HD / 8);
@@ -1168,10 +1138,17 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
+// The kernels' shared memory, once per device: `ready` has a bit for each.
 template <typename Kern>
-int reserve(Kern kern, int bytes, const char* what) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == cudaSuccess ? VSA_OK : fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
+int reserve(Kern kern, int bytes, const char* what, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && dev < 64 && (ready.load(std::memory_order_relaxed) & bit)) return VSA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
+  if (dev < 64) ready.fetch_or(bit, std::memory_order_relaxed);
+  return VSA_OK;
 }
 
 int map_of(CUtensorMap* map, const VsaCross& a, const void* p, const int64_t (&stride)[3], int64_t heads, int64_t rows, int box, const char* what,
@@ -1184,12 +1161,13 @@ template <typename T, int HD>
 int launch_fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
   CUtensorMap mq, mk, mv, mo;
   int rc, *status;
-  if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to a thread that has none yet
+  if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to the thread
   if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention forward (q)"))) return rc;
   if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (k)"))) return rc;
   if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention forward (v)"))) return rc;
   if ((rc = map_of(&mo, a, a.out, a.out_stride, a.H, a.Lq, 32, "cross attention forward (out)"))) return rc;
-  if ((rc = reserve(cross_fwd_umma_kernel<T, HD>, FwdSmem<HD>::total, "cross attention forward"))) return rc;
+  static std::atomic<uint64_t> ready{0};
+  if ((rc = reserve(cross_fwd_umma_kernel<T, HD>, FwdSmem<HD>::total, "cross attention forward", ready))) return rc;
   const int64_t pairs = (a.Lq + 2 * kRows - 1) / (2 * kRows), items = a.B * a.H * pairs * splits;
   if (items > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention forward: too many query rows");
   const FwdWork w{Divisor((uint32_t)splits), Divisor((uint32_t)pairs), Divisor((uint32_t)a.H), Divisor((uint32_t)(a.H / a.Hkv)), (int)items, part_out, part_lse};
@@ -1199,10 +1177,10 @@ int launch_fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, 
 }
 
 template <typename T, int HD>
-int launch_bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+int launch_bwd(const VsaCross& a, int splits, bool parts, float* part, cudaStream_t st) {
   CUtensorMap mq, mdo, mk, mv, mq64, mdo64, mdq;
   int rc, *status;
-  if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to a thread that has none yet
+  if ((rc = device_status_word(&status))) return rc;      // first: it binds the device's context to the thread
   if ((rc = map_of(&mq, a, a.q, a.q_stride, a.H, a.Lq, kRows, "cross attention backward (q)"))) return rc;
   if ((rc = map_of(&mdo, a, a.dout, a.dout_stride, a.H, a.Lq, kRows, "cross attention backward (dout)"))) return rc;
   if ((rc = map_of(&mq64, a, a.q, a.q_stride, a.H, a.Lq, kQTile, "cross attention backward (q)"))) return rc;
@@ -1210,8 +1188,9 @@ int launch_bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   if ((rc = map_of(&mk, a, a.k, a.k_stride, a.Hkv, a.Lkv, kRows, "cross attention backward (k)"))) return rc;
   if ((rc = map_of(&mv, a, a.v, a.v_stride, a.Hkv, a.Lkv, kRows, "cross attention backward (v)"))) return rc;
   if ((rc = map_of(&mdq, a, a.dq, a.dq_stride, a.H, a.Lq, 32, "cross attention backward (dq)", 32))) return rc;
-  if ((rc = reserve(cross_dq_umma_kernel<T, HD>, DqSmem<HD>::total, "cross attention dQ"))) return rc;
-  if ((rc = reserve(cross_dkdv_umma_kernel<T, HD>, DkSmem<HD>::total, "cross attention dK/dV"))) return rc;
+  static std::atomic<uint64_t> dq_ready{0}, dkdv_ready{0};
+  if ((rc = reserve(cross_dq_umma_kernel<T, HD>, DqSmem<HD>::total, "cross attention dQ", dq_ready))) return rc;
+  if ((rc = reserve(cross_dkdv_umma_kernel<T, HD>, DkSmem<HD>::total, "cross attention dK/dV", dkdv_ready))) return rc;
   const int64_t qtiles = (a.Lq + kRows - 1) / kRows, items = a.B * a.H * qtiles, ktiles = (a.Lkv + kRows - 1) / kRows;
   const int64_t units = a.B * a.Hkv * ktiles * splits;
   if (items > 0x3fffffff || units > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention backward: too many rows");
@@ -1219,7 +1198,7 @@ int launch_bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   cross_dq_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kDqThreads, DqSmem<HD>::total, st>>>(
       mq, mdo, mk, mv, mdq, a, Divisor((uint32_t)qtiles), Divisor((uint32_t)a.H), Divisor((uint32_t)(a.H / a.Hkv)), (int)items, status);
   if ((rc = check_launch("cross_dq_umma_kernel"))) return rc;
-  cross_dkdv_umma_kernel<T, HD><<<(unsigned)units, kDkThreads, DkSmem<HD>::total, st>>>(mq64, mdo64, mk, mv, a, (int)ktiles, splits, part, status);
+  cross_dkdv_umma_kernel<T, HD><<<(unsigned)units, kDkThreads, DkSmem<HD>::total, st>>>(mq64, mdo64, mk, mv, a, (int)ktiles, splits, parts ? part : nullptr, status);
   return check_launch("cross_dkdv_umma_kernel");
 }
 
@@ -1251,9 +1230,9 @@ int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_l
                    : launch_fwd<__nv_bfloat16, 128>(a, splits, part_out, part_lse, st);
 }
 
-int cross_bwd_umma(const VsaCross& a, int splits, float* part, cudaStream_t st) {
-  if (a.dtype == VSA_F16) return a.D <= 64 ? launch_bwd<__half, 64>(a, splits, part, st) : launch_bwd<__half, 128>(a, splits, part, st);
-  return a.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(a, splits, part, st) : launch_bwd<__nv_bfloat16, 128>(a, splits, part, st);
+int cross_bwd_umma(const VsaCross& a, int splits, bool parts, float* part, cudaStream_t st) {
+  if (a.dtype == VSA_F16) return a.D <= 64 ? launch_bwd<__half, 64>(a, splits, parts, part, st) : launch_bwd<__half, 128>(a, splits, parts, part, st);
+  return a.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(a, splits, parts, part, st) : launch_bwd<__nv_bfloat16, 128>(a, splits, parts, part, st);
 }
 
 }  // namespace vsa

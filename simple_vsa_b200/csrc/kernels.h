@@ -75,17 +75,20 @@ __device__ __forceinline__ int cross_length(const VsaCross& a, int b) {
 }
 #endif
 int cross_generic_tile(int D);
-// tensor path (cross_umma.cu): by head dim and type; with pointers and strides
+// tensor path (cross_umma.cu), lengths only (key_bits is not looked at): by head dim and type; with pointers and strides
 bool cross_umma_shape(int D, int dtype);
 bool cross_umma_eligible(const VsaCross& a, bool backward);
 int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
-int cross_bwd_umma(const VsaCross& a, int splits, float* part, cudaStream_t st);
+// parts: dK and dV go to `part` in fp32 (always with more than one split)
+int cross_bwd_umma(const VsaCross& a, int splits, bool parts, float* part, cudaStream_t st);
 // splits > 1: partial outputs [splits][B*H][Lq][D] and statistics [splits][B*H][Lq] (-inf: no live key), for cross_join
 int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 // splits > 1: partial dK and dV [splits][2][B*Hkv][Lkv][D], for cross_sum
 int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st);
 int cross_join(const VsaCross& a, int splits, const float* part_out, const float* part_lse, cudaStream_t st);
-int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st);
+int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st, const int32_t* prefix = nullptr);
+// live rows of K and V (16-bit types) to the front, zeros behind: k, v dense [B][Hkv][Lkv][D]; prefix [B][cross_words(Lkv)], counts [B]
+int cross_compact(const VsaCross& a, int32_t* prefix, int32_t* counts, void* k, void* v, cudaStream_t st);
 int cross_key_bits(const uint8_t* mask, int64_t stride, const int32_t* lengths, uint32_t* bits, int64_t B, int64_t Lkv, cudaStream_t st);
 
 // ---- fp32 on 64 x 64 tiles, head dim 64 or 128, block volume 64, 128 or 256 (sparse_f32.cu) --------------------

@@ -12,13 +12,14 @@ namespace vsa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;               // heads whose loads are in flight together
 
 struct RotaryArgs {
   VsaRotary a;
   int chunks;                            // 16-byte pieces (or elements) of a head
   int rows_per_block;
   int heads_per_block;
+  uint32_t total_rows;
+  bool wide_table;                       // rows of the table in 16-byte pieces
 };
 
 // N consecutive elements of T, moved as one word
@@ -27,21 +28,28 @@ template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T e[N]; };
 // How the partners of a thread's elements are read (halves): whole pieces, two elements at a time, one at a time.
 enum Partner { kNeighbour, kPieces, kTwos, kOnes };
 
+// U heads a batch; the next batch's loads are in flight while one is turned and stored.  Neighbours, us for U = 2 (five blocks an SM)
+// and U = 4 (three): [1, 12 + 12, 16384, 128] 48 / 53; tiling [1, 81000, 8, 128] 83 / 100; raster [2, 92160, 40 + 40, 128] 1337 / 1264: the
+// short form unless a block walks many heads.  (U = 4 with four blocks: 74 / 125 / 1976, U = 2 with four: 72 / 85 / 1311.)
+constexpr int kManyHeads = 48;
+template <Partner PARTNER, int U> constexpr int kBlocks = PARTNER == kNeighbour && U == 2 ? 5 : 3;
+
 template <typename T> __device__ __forceinline__ float to_f(T x) { return Elem<T>::to(x); }
 template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
 template <typename T> __device__ __forceinline__ T from_f(float x) { return Elem<T>::from(x); }
 template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
 
-template <typename T, int VEC, Partner PARTNER>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs args) {
+template <typename T, int VEC, Partner PARTNER, int U>
+__global__ void __launch_bounds__(kThreads, kBlocks<PARTNER, U>) rotary_kernel(const __grid_constant__ RotaryArgs args) {
   const VsaRotary& a = args.a;
   const int r_in = threadIdx.x / args.chunks, chunk = threadIdx.x - r_in * args.chunks;
-  const long long row = (long long)blockIdx.x * args.rows_per_block + r_in;
-  if (r_in >= args.rows_per_block || row >= a.B * a.rows) return;
-  const long long b = row / a.rows, l = row - b * a.rows;
+  const uint32_t row = blockIdx.x * (uint32_t)args.rows_per_block + r_in;
+  if (r_in >= args.rows_per_block || row >= args.total_rows) return;
+  const uint32_t b32 = row / (uint32_t)a.rows, l32 = row - b32 * (uint32_t)a.rows;
+  const long long b = b32, l = l32;
   long long s = l;
   if (a.src_map != nullptr) {
-    s = a.src_map[l];
+    s = a.src_map[l32];
     if (s >= a.src_rows) s = -1;
   }
   const bool absent = s < 0;             // a padding row: zeros
@@ -57,18 +65,47 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   unsigned live = 0;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const int e = e0 + i;
     c[i] = 1.f;
     n[i] = 0.f;
-    if (turned && e < a.rotary_dim) {
-      const bool second = PARTNER == kNeighbour ? (e & 1) : e >= half;
-      const int p = PARTNER == kNeighbour ? e >> 1 : (second ? e - half : e);
-      if (PARTNER != kNeighbour || VEC == 1 || (i & 1) == 0) {
-        c[i] = a.cos_table[pos * half + p];
-        const float sine = a.sin_table[pos * half + p];
-        n[i] = second != (a.inverse != 0) ? sine : -sine;
+  }
+  if (turned && e0 < a.rotary_dim) {
+    const float *cos_row = a.cos_table + pos * half, *sin_row = a.sin_table + pos * half;
+    constexpr int N = PARTNER == kNeighbour ? VEC / 2 : VEC;      // angles of a thread
+    // With one head a block this prologue was most of the kernel (scalar loads and 64-bit divisions: 130 us instead of 51 at
+    // [1, 12 + 12, 16384, 128]).
+    if (args.wide_table && N >= 4 && e0 + VEC <= a.rotary_dim && (PARTNER == kNeighbour || PARTNER == kPieces)) {
+      const bool second = PARTNER == kPieces && e0 >= half;
+      const int p = PARTNER == kNeighbour ? e0 >> 1 : (second ? e0 - half : e0);
+      const bool plus = second != (a.inverse != 0);
+      constexpr int W = N / 4 > 0 ? N / 4 : 1;
+      float4 cv[W], sv[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        cv[i] = reinterpret_cast<const float4*>(cos_row + p)[i];
+        sv[i] = reinterpret_cast<const float4*>(sin_row + p)[i];
       }
-      live |= 1u << i;
+      const float *cf = &cv[0].x, *sf = &sv[0].x;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = PARTNER == kNeighbour ? 2 * i : i;
+        c[e % VEC] = cf[i % (4 * W)];
+        n[e % VEC] = plus ? sf[i % (4 * W)] : -sf[i % (4 * W)];
+      }
+      live = (1u << VEC) - 1u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int e = e0 + i;
+        if (e >= a.rotary_dim) continue;
+        const bool second = PARTNER == kNeighbour ? (e & 1) : e >= half;
+        const int p = PARTNER == kNeighbour ? e >> 1 : (second ? e - half : e);
+        if (PARTNER != kNeighbour || VEC == 1 || (i & 1) == 0) {
+          c[i] = cos_row[p];
+          const float sine = sin_row[p];
+          n[i] = second != (a.inverse != 0) ? sine : -sine;
+        }
+        live |= 1u << i;
+      }
     }
   }
 
@@ -76,14 +113,17 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   const int total = a.heads[0] + a.heads[1];
   const int h_begin = blockIdx.y * args.heads_per_block;
   const int h_end = min(total, h_begin + args.heads_per_block);
-  for (int h0 = h_begin; h0 < h_end; h0 += kUnroll) {
-    P own[kUnroll], other[kUnroll];
+  // where the token's heads begin in q and in k; head h of the two together
+  const T* src0 = (const T*)a.x[0] + b * a.x_stride[0][0] + s * a.x_stride[0][2];
+  const T* src1 = (const T*)a.x[1] + b * a.x_stride[1][0] + s * a.x_stride[1][2] - a.heads[0] * a.x_stride[1][1];
+  T* dst0 = (T*)a.y[0] + b * a.y_stride[0][0] + l * a.y_stride[0][2] + e0;
+  T* dst1 = (T*)a.y[1] + b * a.y_stride[1][0] + l * a.y_stride[1][2] - a.heads[0] * a.y_stride[1][1] + e0;
+  auto load = [&](int h0, P(&own)[U], P(&other)[U]) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int h = h0 + u;
       if (h >= h_end || absent) continue;
-      const int t = h >= a.heads[0] ? 1 : 0, hh = t ? h - a.heads[0] : h;
-      const T* src = (const T*)a.x[t] + b * a.x_stride[t][0] + hh * a.x_stride[t][1] + s * a.x_stride[t][2];
+      const T* src = h < a.heads[0] ? src0 + h * a.x_stride[0][1] : src1 + h * a.x_stride[1][1];
       own[u] = *reinterpret_cast<const P*>(src + e0);
       if (PARTNER == kNeighbour) {
         if (VEC == 1 && live) other[u].e[0] = src[e0 ^ 1];
@@ -101,12 +141,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
           }
       }
     }
+  };
+  P own[U], other[U];
+  load(h_begin, own, other);
+  for (int h0 = h_begin; h0 < h_end; h0 += U) {
+    P own_next[U], other_next[U];
+    if (h0 + U < h_end) load(h0 + U, own_next, other_next);      // in flight under this batch's arithmetic and stores
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int h = h0 + u;
       if (h >= h_end) continue;
-      const int t = h >= a.heads[0] ? 1 : 0, hh = t ? h - a.heads[0] : h;
-      T* dst = (T*)a.y[t] + b * a.y_stride[t][0] + hh * a.y_stride[t][1] + l * a.y_stride[t][2];
       P res;
       if (absent) {
 #pragma unroll
@@ -125,29 +169,38 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         for (int i = 0; i < VEC; ++i)
           res.e[i] = live >> i & 1u ? from_f<T>(fmaf(to_f<T>(other[u].e[i]), n[i], to_f<T>(own[u].e[i]) * c[i])) : own[u].e[i];
       }
-      *reinterpret_cast<P*>(dst + e0) = res;
+      *reinterpret_cast<P*>(h < a.heads[0] ? dst0 + h * a.y_stride[0][1] : dst1 + h * a.y_stride[1][1]) = res;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) own[u] = own_next[u], other[u] = other_next[u];
   }
 }
 
-template <typename T, int VEC, Partner PARTNER>
-int launch(const VsaRotary& a, cudaStream_t st) {
-  RotaryArgs args{a, a.D / VEC, 0, 0};
+template <typename T, int VEC, Partner PARTNER, int U>
+int launch_of(const VsaRotary& a, cudaStream_t st) {
+  const bool wide = a.rotary_dim % 8 == 0 && reinterpret_cast<uintptr_t>(a.cos_table) % 16 == 0 && reinterpret_cast<uintptr_t>(a.sin_table) % 16 == 0;
+  RotaryArgs args{a, a.D / VEC, 0, 0, (uint32_t)(a.B * a.rows), wide};
   if (args.chunks > kThreads) return fail(VSA_ERR_UNSUPPORTED, "rotary: head dim %d is above 256", a.D);
   args.rows_per_block = kThreads / args.chunks;
   const long long rows = a.B * a.rows, blocks = (rows + args.rows_per_block - 1) / args.rows_per_block;
-  if (blocks > 0x7fffffffLL) return fail(VSA_ERR_UNSUPPORTED, "rotary: too many tokens");
+  if (rows > 0x7fffffffLL) return fail(VSA_ERR_UNSUPPORTED, "rotary: 2^31 tokens at most");
   // All heads of a token in one block where that fills the GPU sixteen times over (the table is then read once); fewer heads a
   // block, down to one, where there are few tokens.
   const int total = a.heads[0] + a.heads[1];
   const long long want = 148LL * 16;
   long long hpb = blocks >= want ? total : (total * blocks + want - 1) / want;
-  if (hpb > kUnroll) hpb = (hpb + kUnroll - 1) / kUnroll * kUnroll;
+  if (hpb > U) hpb = (hpb + U - 1) / U * U;
   if ((total + hpb - 1) / hpb > 65535) hpb = (total + 65534) / 65535;
   args.heads_per_block = (int)(hpb < 1 ? 1 : hpb);
   const dim3 grid((unsigned)blocks, (unsigned)((total + args.heads_per_block - 1) / args.heads_per_block));
-  rotary_kernel<T, VEC, PARTNER><<<grid, kThreads, 0, st>>>(args);
+  rotary_kernel<T, VEC, PARTNER, U><<<grid, kThreads, 0, st>>>(args);
   return check_launch("rotary_kernel");
+}
+
+template <typename T, int VEC, Partner PARTNER>
+int launch(const VsaRotary& a, cudaStream_t st) {
+  if (PARTNER == kNeighbour && VEC > 1 && a.heads[0] + a.heads[1] >= kManyHeads) return launch_of<T, VEC, PARTNER, 4>(a, st);
+  return launch_of<T, VEC, PARTNER, 2>(a, st);
 }
 
 template <typename T>

@@ -445,11 +445,20 @@ int make_map_rows(CUtensorMap* map, CUtensorMapDataType elem, const void* ptr, i
   return VSA_OK;
 }
 
+// Also what binds the device's context to a host thread that has had none yet (autograd's own threads), without which tensor maps
+// cannot be encoded; once per thread and device.
 int device_status_word(int** word) {
-  void* p = nullptr;
-  const cudaError_t e = cudaGetSymbolAddress(&p, g_device_status);
+  static thread_local int known_device = -1;
+  static thread_local int* known_word = nullptr;
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev != known_device) {
+    void* p = nullptr;
+    e = cudaGetSymbolAddress(&p, g_device_status);
+    if (e == cudaSuccess) known_device = dev, known_word = static_cast<int*>(p);
+  }
   if (e != cudaSuccess) return fail(VSA_ERR_LAUNCH, "device status: %s", cudaGetErrorString(e));
-  *word = static_cast<int*>(p);
+  *word = known_word;
   return VSA_OK;
 }
 

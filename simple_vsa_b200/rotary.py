@@ -94,7 +94,9 @@ def _table(rotary: Dict[str, object], head_dim: int, device) -> Tuple[Tensor, Te
         raise ValueError(f"the rotary table turns {2 * cos.shape[1]} dims of a head, the tensors have {head_dim}")
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("the rotary table is a constant: it receives no gradient")
-    cos, sin = (x.to(device=device, dtype=torch.float32).contiguous() for x in (cos, sin))
+    if cos.device != device or cos.dtype != torch.float32 or sin.device != device or sin.dtype != torch.float32:
+        cos, sin = cos.to(device=device, dtype=torch.float32), sin.to(device=device, dtype=torch.float32)
+    cos, sin = cos.contiguous(), sin.contiguous()
     return cos, sin, bool(rotary.get("interleaved", True))
 
 
@@ -112,22 +114,26 @@ def rotate(xs, ys, cos, sin, interleaved: bool, inverse: bool, *, x_raster: bool
            src_map=None) -> None:
     """``ys[i]`` = ``xs[i]`` with its heads turned (one or two tensors, one launch); the layouts may differ where
     ``src_map`` moves the rows."""
-    a = _lib.Rotary()
-    y0 = ys[0]
-    a.B, a.rows = y0.shape[0], y0.shape[1 if y_raster else 2]
-    a.src_rows = xs[0].shape[1 if x_raster else 2]
-    for i, (x, y) in enumerate(zip(xs, ys)):
-        a.x[i], a.y[i] = x.data_ptr(), y.data_ptr()
-        a.x_stride[i][:] = _strides(x, x_raster)
-        a.y_stride[i][:] = _strides(y, y_raster)
-        a.heads[i] = y.shape[2 if y_raster else 1]
-    a.cos_table, a.sin_table, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    a.positions, a.src_map = ops._ptr(positions), ops._ptr(src_map)
-    a.positions_stride = a.rows if positions is not None and positions.ndim == 2 else 0
-    a.D, a.rotary_dim = y0.shape[3], 2 * cos.shape[1]
-    a.interleaved, a.inverse = int(interleaved), int(inverse)
-    a.dtype = {torch.bfloat16: _lib.VSA_BF16, torch.float16: _lib.VSA_F16, torch.float32: _lib.VSA_F32}[y0.dtype]
+    x0, y0 = xs[0], ys[0]
+    two = len(xs) > 1
+    x1, y1 = (xs[1], ys[1]) if two else (x0, y0)
+    seq, head = (1, 2) if y_raster else (2, 1)
+    rows = y0.shape[seq]
+    dt = {torch.bfloat16: _lib.VSA_BF16, torch.float16: _lib.VSA_F16, torch.float32: _lib.VSA_F32}[y0.dtype]
+    a = _lib.Rotary.from_buffer_copy(_lib.Rotary.PACK.pack(
+        x0.data_ptr(), x1.data_ptr(), y0.data_ptr(), y1.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+        0 if positions is None else positions.data_ptr(), 0 if src_map is None else src_map.data_ptr(),
+        y0.shape[0], rows, x0.shape[1 if x_raster else 2], cos.shape[0], rows if positions is not None and positions.ndim == 2 else 0,
+        *_strides(x0, x_raster), *_strides(x1, x_raster), *_strides(y0, y_raster), *_strides(y1, y_raster),
+        y0.shape[head], y1.shape[head] if two else 0, y0.shape[3], 2 * cos.shape[1], interleaved, inverse, dt))
     call("vsa_rotary", a, ops._stream(y0.device))
+
+
+def _turned(q, k, cos, sin, positions, interleaved, raster):
+    xs = [_rows(x) for x in ((q,) if k is None else (q, k))]
+    ys = [torch.empty_like(x) for x in xs]
+    rotate(xs, ys, cos, sin, interleaved, False, x_raster=raster, y_raster=raster, positions=positions)
+    return ys[0], ys[1] if k is not None else None
 
 
 class _Rotary(torch.autograd.Function):
@@ -135,13 +141,11 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, cos, sin, positions, interleaved, raster):
-        xs = [_rows(x) for x in ((q,) if k is None else (q, k))]
-        ys = [torch.empty_like(x) for x in xs]
-        rotate(xs, ys, cos, sin, interleaved, False, x_raster=raster, y_raster=raster, positions=positions)
+        ys = _turned(q, k, cos, sin, positions, interleaved, raster)
         ctx.save_for_backward(cos, sin, *(() if positions is None else (positions,)))
         ctx.has_positions, ctx.interleaved, ctx.raster = positions is not None, interleaved, raster
         ctx.set_materialize_grads(False)
-        return ys[0], ys[1] if k is not None else None
+        return ys
 
     @staticmethod
     def backward(ctx, *grads):
@@ -183,7 +187,8 @@ def _turn(q: Tensor, k: Optional[Tensor], rotary: Dict[str, object], positions: 
     with torch.cuda.device(q.device):
         if positions is not None:
             positions = positions.to(device=q.device, dtype=torch.int32).contiguous()
-        out_q, out_k = _Rotary.apply(q, k, cos, sin, positions, interleaved, raster)
+        need_grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+        out_q, out_k = (_Rotary.apply if need_grad else _turned)(q, k, cos, sin, positions, interleaved, raster)
     return out_q if k is None else (out_q, out_k)
 
 

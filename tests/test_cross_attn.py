@@ -41,14 +41,14 @@ def test_c_entry_refusals_and_sizes():
         setattr(a, name, old)
     assert _lib.lib.vsa_cross_fwd(None, None) == _lib.ERR_BAD_ARGUMENT
     assert [_lib.lib.vsa_cross_words(n) for n in (-1, 0, 1, 128, 129)] == [-1, 0, 4, 4, 8]
-    assert _lib.lib.vsa_cross_workspace_bytes(0, 2, 4, 3, 10, 7, 16, _lib.VSA_BF16) == -1
-    assert _lib.lib.vsa_cross_workspace_bytes(1, 2, 4, 2, 10, 7, 16, 9) == -1
-    assert _lib.lib.vsa_cross_workspace_bytes(0, 0, 4, 2, 10, 7, 16, _lib.VSA_F32) == 0
+    assert _lib.lib.vsa_cross_workspace_bytes(0, 2, 4, 3, 10, 7, 16, _lib.VSA_BF16, 0) == -1
+    assert _lib.lib.vsa_cross_workspace_bytes(1, 2, 4, 2, 10, 7, 16, 9, 0) == -1
+    assert _lib.lib.vsa_cross_workspace_bytes(0, 0, 4, 2, 10, 7, 16, _lib.VSA_F32, 0) == 0
     # many rows: nothing is split; a row each against long states: the keys are, and the parts fit what is asked for
-    assert _lib.lib.vsa_cross_workspace_bytes(0, 2, 40, 40, 92160, 512, 128, _lib.VSA_BF16) == 0
-    n = _lib.lib.vsa_cross_workspace_bytes(0, 1, 2, 2, 1, 8192, 128, _lib.VSA_BF16)
+    assert _lib.lib.vsa_cross_workspace_bytes(0, 2, 40, 40, 92160, 512, 128, _lib.VSA_BF16, 0) == 0
+    n = _lib.lib.vsa_cross_workspace_bytes(0, 1, 2, 2, 1, 8192, 128, _lib.VSA_BF16, 0)
     assert n > 0 and n % (2 * (128 + 1) * 4) == 0
-    n = _lib.lib.vsa_cross_workspace_bytes(1, 1, 2, 2, 40000, 77, 64, _lib.VSA_F16)
+    n = _lib.lib.vsa_cross_workspace_bytes(1, 1, 2, 2, 40000, 77, 64, _lib.VSA_F16, 0)
     assert n > 0 and n % (2 * 2 * 77 * 64 * 4) == 0
 
 
