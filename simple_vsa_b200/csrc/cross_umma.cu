@@ -138,7 +138,7 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
 // 2^8 (fp16 holds 2^16, the sums are fp32), and moving O through registers is rare.
 constexpr int kFwdThreads = 256 + 256;     // loads and four issuers of MMAs (eight warps), two softmax groups
 constexpr int kKeys = 64;                  // keys of a step
-constexpr int kFwdPoly = 3;                // of eight pairs of exponentials, on the FMA pipe
+constexpr int kFwdPoly = 2;                // of eight pairs of exponentials, on the FMA pipe
 template <int HD>
 struct FwdSmem {
   static constexpr uint32_t tile = HD * 256;                      // 128 rows
@@ -850,11 +850,14 @@ constexpr int kDkCols = 32;
 constexpr int kDkGroups = kQTile / kDkCols;
 constexpr int kDkEwThreads = 128 * kDkGroups;
 constexpr int kDkThreads = 128 + kDkEwThreads;
+template <int HD> constexpr int kDkPoly = HD == 64 ? 2 : 0;      // of eight pairs of exponentials, on the FMA pipe
 template <int HD>
 struct DkSmem {
   static constexpr uint32_t tile = HD * 256;          // 128 resident rows
   static constexpr uint32_t part = HD * 128;          // 64 streamed rows
   static constexpr int q_stages = 5, do_stages = 5;
+  // buffers of (S^T, dP^T): at head dim 64 the gradients leave room for a third, and a step's chain is longer than its products
+  static constexpr int bufs = HD == 64 ? 3 : 2;
   static constexpr uint32_t k = 0;
   static constexpr uint32_t v = k + tile;
   static constexpr uint32_t q = v + tile;
@@ -865,8 +868,8 @@ struct DkSmem {
   static constexpr uint32_t total = misc + 16;
 };
 static_assert(DkSmem<128>::total <= 232448, "shared memory of the cross attention dK/dV pass");
-enum DkBar { K_KV_FULL = 0, K_Q_FULL = 1, K_Q_EMPTY = 6, K_DO_FULL = 11, K_DO_EMPTY = 16, K_S_FULL = 21, K_S_EMPTY = 23,
-             K_DP_FULL = 25, K_DP_EMPTY = 27, K_P_FULL = 29, K_DS_FULL = 31, K_ACC_FULL = 33 };
+enum DkBar { K_KV_FULL = 0, K_Q_FULL = 1, K_Q_EMPTY = 6, K_DO_FULL = 11, K_DO_EMPTY = 16, K_S_FULL = 21, K_S_EMPTY = 24,
+             K_DP_FULL = 27, K_DP_EMPTY = 30, K_P_FULL = 33, K_DS_FULL = 36, K_ACC_FULL = 39 };
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kDkThreads, 1)
@@ -927,7 +930,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
       mbar_init(bar(K_DO_FULL + i), 1);
       mbar_init(bar(K_DO_EMPTY + i), 2);      // read by the dP products of one issuer and the dV products of the other
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < Sm::bufs; ++i) {
       mbar_init(bar(K_S_FULL + i), 1);
       mbar_init(bar(K_S_EMPTY + i), 1);
       mbar_init(bar(K_DP_FULL + i), 1);
@@ -951,8 +954,9 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = misc[0];
-  // two buffers of (S^T 64 columns, dP^T 64 columns), P^T and dS^T packed over them; then dK and dV
-  const uint32_t tmem_dk = tmem + 256, tmem_dv = tmem + 384;
+  // buffers of (S^T 64 columns, dP^T 64 columns), P^T and dS^T packed over them; then dK and dV
+  const uint32_t tmem_dk = tmem + 128 * Sm::bufs, tmem_dv = tmem_dk + HD;
+  static_assert(128 * Sm::bufs + 2 * HD <= (int)kTmemCols, "tensor memory of the dK/dV pass");
   bool ok = true;
 
   if (warp == 0) {       // dO tiles; Q tiles and the statistics of their rows
@@ -982,8 +986,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // S^T = K Q^T
     ok = CROSS_WAIT(bar(K_KV_FULL), 0);
     for (int p = 0; p < n_tiles && ok; ++p) {
-      const int s = p % Sm::q_stages, bf = p & 1;
-      ok = CROSS_WAIT(bar(K_Q_FULL + s), (p / Sm::q_stages) & 1) && CROSS_WAIT(bar(K_S_EMPTY + bf), ((p >> 1) & 1) ^ 1);
+      const int s = p % Sm::q_stages, bf = p % Sm::bufs;
+      ok = CROSS_WAIT(bar(K_Q_FULL + s), (p / Sm::q_stages) & 1) && CROSS_WAIT(bar(K_S_EMPTY + bf), ((p / Sm::bufs) & 1) ^ 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -997,8 +1001,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     // dP^T = V dO^T
     ok = CROSS_WAIT(bar(K_KV_FULL), 0);
     for (int p = 0; p < n_tiles && ok; ++p) {
-      const int s = p % Sm::do_stages, bf = p & 1;
-      ok = CROSS_WAIT(bar(K_DO_FULL + s), (p / Sm::do_stages) & 1) && CROSS_WAIT(bar(K_DP_EMPTY + bf), ((p >> 1) & 1) ^ 1);
+      const int s = p % Sm::do_stages, bf = p % Sm::bufs;
+      ok = CROSS_WAIT(bar(K_DO_FULL + s), (p / Sm::do_stages) & 1) && CROSS_WAIT(bar(K_DP_EMPTY + bf), ((p / Sm::bufs) & 1) ^ 1);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -1012,8 +1016,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   } else if (warp == 3) {
     // dV += P^T dO, dK += dS^T Q
     for (int p = 0; p < n_tiles && ok; ++p) {
-      const int sq = p % Sm::q_stages, sd = p % Sm::do_stages, bf = p & 1;
-      const uint32_t ph = (p >> 1) & 1;
+      const int sq = p % Sm::q_stages, sd = p % Sm::do_stages, bf = p % Sm::bufs;
+      const uint32_t ph = (p / Sm::bufs) & 1;
       ok = CROSS_WAIT(bar(K_DO_FULL + sd), (p / Sm::do_stages) & 1) && CROSS_WAIT(bar(K_P_FULL + bf), ph);
       if (!ok) break;
       tc_fence_after();
@@ -1043,8 +1047,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const bool live = row < live_keys;
     const float2 c2 = make_float2(-c, -c), m1 = make_float2(-1.f, -1.f);
     for (int p = 0; p < n_tiles && ok; ++p) {
-      const int bf = p & 1, sq = p % Sm::q_stages;
-      const uint32_t ph = (p >> 1) & 1;
+      const int bf = p % Sm::bufs, sq = p % Sm::q_stages;
+      const uint32_t ph = (p / Sm::bufs) & 1;
       ok = CROSS_WAIT(bar(K_S_FULL + bf), ph) && CROSS_WAIT(bar(K_Q_FULL + sq), (p / Sm::q_stages) & 1);
       if (!ok) break;
       tc_fence_after();
@@ -1061,8 +1065,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         // lse - S c, negated in the exponential: the packed operations have no sign of their own to spend on the statistics
         const float2 x = fma2(word_pair(sv + 4 * i), c2, make_float2(l4.x, l4.y));
         const float2 y = fma2(word_pair(sv + 4 * i + 2), c2, make_float2(l4.z, l4.w));
-        pf[2 * i] = make_float2(fast_exp2(-x.x), fast_exp2(-x.y));
-        pf[2 * i + 1] = make_float2(fast_exp2(-y.x), fast_exp2(-y.y));
+        pf[2 * i] = kDkPoly<HD> > 2 * i % 8 ? poly_exp2<T>(mul2(x, m1)) : make_float2(fast_exp2(-x.x), fast_exp2(-x.y));
+        pf[2 * i + 1] = kDkPoly<HD> > (2 * i + 1) % 8 ? poly_exp2<T>(mul2(y, m1)) : make_float2(fast_exp2(-y.x), fast_exp2(-y.y));
         // a key that takes no part: its scores come from whatever sits in K there
         pk[2 * i] = live ? Elem<T>::pack(pf[2 * i].x, pf[2 * i].y) : 0u;
         pk[2 * i + 1] = live ? Elem<T>::pack(pf[2 * i + 1].x, pf[2 * i + 1].y) : 0u;
