@@ -647,7 +647,14 @@ static int cross_parts(int64_t units, int64_t steps, int64_t setup, int64_t most
   }
   return best;
 }
-static int cross_fwd_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D, int dtype) {
+static bool cross_few_rows(int64_t H, int64_t Hkv, int64_t Lq, int D, int dtype) { return cross_umma_shape(D, dtype) && H / Hkv * Lq <= 8; }
+static int cross_fwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  // a CTA of few rows takes 256 keys or 128 at a time; three of them on an SM hide its latencies, a cut costs the join's launch
+  if (cross_few_rows(H, Hkv, Lq, D, dtype)) {
+    const int64_t units = B * Hkv, steps = (Lkv + 255) / 256, most = (148 * 3 + units - 1) / units;
+    const int64_t s = units >= 148 ? 1 : most < steps ? most : steps;
+    return (int)(s < 64 ? s : 64);
+  }
   if (cross_umma_shape(D, dtype)) return cross_parts(B * H * ((Lq + 255) / 256), (Lkv + 127) / 128, 4, 64);
   const int tile = cross_generic_tile(D);
   return cross_parts(B * H * ((Lq + tile - 1) / tile), (Lkv + tile - 1) / tile, 2, 64);
@@ -673,8 +680,8 @@ struct CrossSpace {
 static CrossSpace cross_space(bool backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype, bool mask) {
   CrossSpace s{1, 0, 0, 0, 0, 0, 0};
   if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return s;
-  const bool compact = mask && cross_umma_shape(D, dtype);
-  s.splits = backward ? cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype) : cross_fwd_splits(B, H, Lq, Lkv, D, dtype);
+  const bool compact = mask && cross_umma_shape(D, dtype) && (backward || !cross_few_rows(H, Hkv, Lq, D, dtype));
+  s.splits = backward ? cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype) : cross_fwd_splits(B, H, Hkv, Lq, Lkv, D, dtype);
   if (!backward) s.parts = s.splits == 1 ? 0 : s.splits * B * H * Lq * (int64_t)(D + 1) * 4;
   else s.parts = s.splits == 1 && !compact ? 0 : s.splits * 2 * B * Hkv * Lkv * (int64_t)D * 4;
   s.parts = (s.parts + 15) / 16 * 16;
@@ -743,7 +750,9 @@ int vsa_cross_fwd(const VsaCross* a, void* stream) {
   const CrossSpace s = cross_space(false, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr);
   float* part_out = (float*)a->workspace;
   float* part_lse = part_out + (s.splits == 1 ? 0 : s.splits * a->B * a->H * a->Lq * a->D);
-  if (!cross_on_umma(*a, false)) {
+  if (cross_few_rows(a->H, a->Hkv, a->Lq, a->D, a->dtype) && !scalar_forced() && cross_aligned(*a, false)) {
+    rc = cross_fwd_rows(*a, s.splits, part_out, part_lse, st);
+  } else if (!cross_on_umma(*a, false)) {
     rc = cross_fwd_generic(*a, s.splits, part_out, part_lse, st);
   } else if (a->key_bits == nullptr) {
     rc = cross_fwd_umma(*a, s.splits, part_out, part_lse, st);

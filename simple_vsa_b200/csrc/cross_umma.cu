@@ -1218,8 +1218,10 @@ bool aligned(const void* p, const int64_t (&s)[3], int64_t heads, int64_t rows, 
 
 bool cross_umma_shape(int D, int dtype) { return (dtype == VSA_BF16 || dtype == VSA_F16) && D % 8 == 0 && D >= 8 && D <= 128; }
 
-bool cross_umma_eligible(const VsaCross& a, bool backward) {
-  if (!cross_umma_shape(a.D, a.dtype) || a.Lkv < 1 || a.Lq < 1 || !(a.scale > 0.f)) return false;
+bool cross_umma_eligible(const VsaCross& a, bool backward) { return a.scale > 0.f && cross_aligned(a, backward); }
+
+bool cross_aligned(const VsaCross& a, bool backward) {
+  if (!cross_umma_shape(a.D, a.dtype) || a.Lkv < 1 || a.Lq < 1) return false;
   if (!aligned(a.q, a.q_stride, a.H, a.Lq, a.B) || !aligned(a.k, a.k_stride, a.Hkv, a.Lkv, a.B) || !aligned(a.v, a.v_stride, a.Hkv, a.Lkv, a.B) ||
       !aligned(a.out, a.out_stride, a.H, a.Lq, a.B))
     return false;

@@ -77,7 +77,10 @@ __device__ __forceinline__ int cross_length(const VsaCross& a, int b) {
 int cross_generic_tile(int D);
 // tensor path (cross_umma.cu), lengths only (key_bits is not looked at): by head dim and type; with pointers and strides
 bool cross_umma_shape(int D, int dtype);
-bool cross_umma_eligible(const VsaCross& a, bool backward);
+bool cross_aligned(const VsaCross& a, bool backward);
+bool cross_umma_eligible(const VsaCross& a, bool backward);      // and a positive scale
+// at most eight rows of queries a key head (cross_rows.cu), any positive or negative scale, key_bits looked at; shapes and alignment as above
+int cross_fwd_rows(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 // parts: dK and dV go to `part` in fp32 (always with more than one split)
 int cross_bwd_umma(const VsaCross& a, int splits, bool parts, float* part, cudaStream_t st);

@@ -143,6 +143,27 @@ def test_output_and_gradients_match_float64(dtype, B, H, Hk, L, T, D):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,H,Hk,L,T,D", [(3, 2, 2, 1, 1, 64), (3, 2, 1, 1, 255, 128), (3, 4, 1, 1, 257, 72), (3, 4, 2, 2, 5000, 128),
+                                          (3, 4, 1, 2, 700, 64), (3, 3, 1, 3, 130, 128), (3, 160, 160, 1, 500, 128), (3, 5, 5, 7, 40, 8)])
+def test_few_rows(dtype, B, H, Hk, L, T, D):
+    """Up to eight and just above eight rows a key head, keys cut into parts or not, with lengths and a mask, and a sample without
+    keys; the gradient of such a call."""
+    q, k, v, dout = _inputs(B, H, Hk, L, T, D, dtype, T + H)
+    g = torch.Generator().manual_seed(T)
+    mask = torch.rand(B, T, generator=g) < 0.7
+    mask[0] = True
+    mask[2] = False
+    for ln, mk in ((None, None), (torch.tensor([T, max(1, T // 3), 0]), None), (None, mask), (torch.tensor([T // 2, T, T]), mask)):
+        live = _live(B, T, ln, mk)
+        kk, vv = k.clone(), v.clone()
+        dead = ~live[:, None, :, None].to(DEV).expand_as(kk)
+        kk[dead], vv[dead] = math.nan, math.nan
+        got = _run(q, kk, vv, dout, ln, None if mk is None else mk.to(DEV))
+        _compare(got, _exact(q, k, v, live, 1 / math.sqrt(D), dout), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("T,D", [(300, 128), (512, 64), (129, 72), (1, 64), (70, 20)])
 def test_lengths_and_masks(dtype, T, D):
     """Prompts of zero, one, full and odd lengths; masks with holes, whole tiles and whole samples gone; both together.  What stands
