@@ -13,6 +13,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from ._lib import call
@@ -75,6 +76,7 @@ class _CrossAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, key_bits = ctx.saved_tensors
         with torch.cuda.device(q.device):
@@ -103,7 +105,8 @@ def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
     if not 1 <= D <= 256:
         raise ValueError(f"cross attention supports head dimensions from 1 to 256, got {D}")
     ops._check_device_dtype(q, k, v)
-    if kv_lengths is not None and (kv_lengths.is_floating_point() or kv_lengths.dtype == torch.bool or tuple(kv_lengths.shape) != (B,)):
+    if kv_lengths is not None and (kv_lengths.is_floating_point() or kv_lengths.is_complex() or kv_lengths.dtype == torch.bool
+                                   or tuple(kv_lengths.shape) != (B,)):
         raise ValueError(f"kv_lengths must hold {B} integers, one per sample")
     if kv_mask is not None and (kv_mask.dtype != torch.bool or tuple(kv_mask.shape) != (B, T)):
         raise ValueError(f"kv_mask must be a bool tensor of shape [{B}, {T}], True where a key takes part")

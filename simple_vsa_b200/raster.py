@@ -23,6 +23,7 @@ from typing import Dict, Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from . import rotary as rot
@@ -223,6 +224,7 @@ class _TileTurned(torch.autograd.Function):
         return _tile_turned(x, tile_map, (cos, sin, interleaved), False, tile_map.numel())
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         untile_map, cos, sin = ctx.saved_tensors
         with torch.cuda.device(grad.device):

@@ -13,6 +13,7 @@ from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from ._lib import call
@@ -148,6 +149,7 @@ class _Rotary(torch.autograd.Function):
         return ys
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         cos, sin = ctx.saved_tensors[:2]
         positions = ctx.saved_tensors[2] if ctx.has_positions else None
