@@ -106,27 +106,30 @@ def _rows(x: Tensor) -> Tensor:
     return x if x.stride(3) == 1 or x.shape[3] <= 1 else x.contiguous()
 
 
-def _strides(x: Tensor, raster: bool) -> Tuple[int, int, int]:
-    s = x.stride()
-    return (s[0], s[2], s[1]) if raster else (s[0], s[1], s[2])
+_DTYPES = {torch.bfloat16: _lib.VSA_BF16, torch.float16: _lib.VSA_F16, torch.float32: _lib.VSA_F32}
+_PACK = _lib.Rotary.PACK.pack
+_ARGUMENTS = _lib.Rotary.from_buffer_copy
 
 
 def rotate(xs, ys, cos, sin, interleaved: bool, inverse: bool, *, x_raster: bool, y_raster: bool, positions=None,
            src_map=None) -> None:
     """``ys[i]`` = ``xs[i]`` with its heads turned (one or two tensors, one launch); the layouts may differ where
     ``src_map`` moves the rows."""
-    x0, y0 = xs[0], ys[0]
-    two = len(xs) > 1
-    x1, y1 = (xs[1], ys[1]) if two else (x0, y0)
-    seq, head = (1, 2) if y_raster else (2, 1)
-    rows = y0.shape[seq]
-    dt = {torch.bfloat16: _lib.VSA_BF16, torch.float16: _lib.VSA_F16, torch.float32: _lib.VSA_F32}[y0.dtype]
-    a = _lib.Rotary.from_buffer_copy(_lib.Rotary.PACK.pack(
+    x0, y0, x1, y1 = xs[0], ys[0], xs[-1], ys[-1]
+    (xa, xb, xc, _), (xd, xe, xf, _), (ya, yb, yc, _), (yd, ye, yf, _) = x0.stride(), x1.stride(), y0.stride(), y1.stride()
+    if x_raster:
+        xb, xc, xe, xf = xc, xb, xf, xe
+    if y_raster:
+        yb, yc, ye, yf = yc, yb, yf, ye
+        B, rows, heads, D = y0.shape
+    else:
+        B, heads, rows, D = y0.shape
+    a = _ARGUMENTS(_PACK(
         x0.data_ptr(), x1.data_ptr(), y0.data_ptr(), y1.data_ptr(), cos.data_ptr(), sin.data_ptr(),
         0 if positions is None else positions.data_ptr(), 0 if src_map is None else src_map.data_ptr(),
-        y0.shape[0], rows, x0.shape[1 if x_raster else 2], cos.shape[0], rows if positions is not None and positions.ndim == 2 else 0,
-        *_strides(x0, x_raster), *_strides(x1, x_raster), *_strides(y0, y_raster), *_strides(y1, y_raster),
-        y0.shape[head], y1.shape[head] if two else 0, y0.shape[3], 2 * cos.shape[1], interleaved, inverse, dt))
+        B, rows, x0.shape[1 if x_raster else 2], cos.shape[0], rows if positions is not None and positions.ndim == 2 else 0,
+        xa, xb, xc, xd, xe, xf, ya, yb, yc, yd, ye, yf,
+        heads, y1.shape[2 if y_raster else 1] if len(ys) > 1 else 0, D, 2 * cos.shape[1], interleaved, inverse, _DTYPES[y0.dtype]))
     call("vsa_rotary", a, ops._stream(y0.device))
 
 
@@ -142,26 +145,21 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, cos, sin, positions, interleaved, raster):
-        ys = _turned(q, k, cos, sin, positions, interleaved, raster)
-        ctx.save_for_backward(cos, sin, *(() if positions is None else (positions,)))
-        ctx.has_positions, ctx.interleaved, ctx.raster = positions is not None, interleaved, raster
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.interleaved, ctx.raster = interleaved, raster
         ctx.set_materialize_grads(False)
-        return ys
+        return _turned(q, k, cos, sin, positions, interleaved, raster)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, *grads):
-        cos, sin = ctx.saved_tensors[:2]
-        positions = ctx.saved_tensors[2] if ctx.has_positions else None
+    def backward(ctx, dq, dk):
+        (cos, sin, positions), raster = ctx.saved_tensors, ctx.raster
         with torch.cuda.device(cos.device):
-            there = [_rows(g) for g in grads if g is not None]
+            there = [_rows(g) for g in (dq, dk) if g is not None]
             back = [torch.empty_like(g) for g in there]
             if there:
-                rotate(there, back, cos, sin, ctx.interleaved, True, x_raster=ctx.raster, y_raster=ctx.raster,
-                       positions=positions)
-        back = iter(back)
-        dq, dk = (None if g is None else next(back) for g in grads)
-        return dq, dk, None, None, None, None, None
+                rotate(there, back, cos, sin, ctx.interleaved, True, x_raster=raster, y_raster=raster, positions=positions)
+        return back[0] if dq is not None else None, back[-1] if dk is not None else None, None, None, None, None, None
 
 
 def _turn(q: Tensor, k: Optional[Tensor], rotary: Dict[str, object], positions: Optional[Tensor], raster: bool):

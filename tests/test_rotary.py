@@ -343,3 +343,16 @@ def test_side_stream_and_captured_step():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(res[0], V.video_rotary(k, None, rot)) and torch.equal(res[1], V.video_rotary(q, None, rot))
+
+
+@pytest.mark.gpu
+def test_a_table_or_positions_changed_before_the_backward_are_refused():
+    rot = V.build_rotary_metadata((6,), 8, device=DEV)
+    for change in ("cos", "positions"):
+        table = {**rot, "cos": rot["cos"].clone()}
+        pos = torch.arange(6, device=DEV, dtype=torch.int32)
+        q = torch.randn(1, 2, 6, 8, device=DEV, requires_grad=True)
+        out = V.video_rotary(q, None, table, positions=pos)
+        (table["cos"] if change == "cos" else pos).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
