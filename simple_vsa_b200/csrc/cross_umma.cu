@@ -129,13 +129,18 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
 // ------------------------------------------------------------------------------------------------------
 // A piece of work is 256 query rows of one head (two tiles of 128, which are the M dimension) against the key tiles of one split.  Both
 // tiles take every K and V tile from the same buffers; four softmax warps own a tile, a thread a row.  The keys are walked 64 at a
-// time and a tile has two score accumulators, so that the next scores are there when a softmax group has finished: with one
-// accumulator of 128 keys the groups idled 42 % of the time behind S, and eight warps a tile that shared its rows gained nothing
-// (5200 cycles per 256 x 128 scores either way; this form ...).  P goes over the scores it came from in tensor memory.
-// Per 128 x 128 scores at D = 128: 1280 tensor cycles (an M128 x N64 x K16 product takes 48 of the 32 that its size asks for), 1024
-// of exponentials.
+// time and a tile has two score accumulators, so that the next scores are there when a softmax group has finished (with one accumulator
+// of 128 keys the groups idled 42 % of the time behind S).  P goes over the scores it came from in tensor memory; the MMAs have an
+// issuer warp for each product of each tile.
 // The softmax keeps a running maximum, but moves the accumulated row only when the maximum has grown by more than 2^8: P stays below
 // 2^8 (fp16 holds 2^16, the sums are fp32), and moving O through registers is rare.
+//
+// [1, 40, 92160, 128] x 512 keys, bf16: 835 us, 1157 TFLOP/s (994 in a long loop, power limit); [2, 12 + 4, 8190, 64] x 801 of 1001: 75 us.
+// Per 256 x 64 scores at D = 128, of some 1650 cycles: 1280 of MMAs (an M128 x N64 x K16 product takes 48 cycles of the 32 that its size
+// asks for), 1250 of shared-memory traffic (160 KB at 128 B/clk), 1024 of exponentials before a quarter of them moved to the FMA pipe;
+// what bounds it is a softmax group's chain (scores from tensor memory, maximum, exponentials, P back), which two groups overlap.
+// More warps were slower: eight a tile sharing its rows, and four groups on alternating steps with the maximum handed on (982 for
+// 860 us).  A piece's end (O out, the next piece's set-up) is some 3000 of 16000 cycles at 512 keys.
 constexpr int kFwdThreads = 256 + 256;     // loads and four issuers of MMAs (eight warps), two softmax groups
 constexpr int kKeys = 64;                  // keys of a step
 constexpr int kFwdPoly = 2;                // of eight pairs of exponentials, on the FMA pipe
@@ -499,8 +504,13 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // ------------------------------------------------------------------------------------------------------
 // A piece of work is 128 query rows of one head: S = Q K^T, dP = dO V^T, dQ += dS K per key tile.  All sixteen elementwise warps
 // share a tile, 32 score columns a thread; S (later dS) in two accumulators, dP in one that is free again as soon as it has been read.
-// Per 128 x 128 scores at D = 128: 1536 tensor cycles, 1024 of exponentials.  delta = rowsum(out * dout) takes dout from its tile in
-// shared memory and out from registers that were filled while the piece before was finished.
+// delta = rowsum(out * dout) takes dout from its tile in shared memory and out from registers that were filled while the piece before
+// was finished.
+//
+// [1, 8, 92160, 128] x 512 keys: 268 us, 1080 TFLOP/s.  A piece of four key tiles takes 12,000 cycles: 1700 to 1800 a tile (1536 of MMAs,
+// 1024 of exponentials before three of eight moved to the FMA pipe) and 5000 around them (delta, the wait for the last product, dQ out,
+// the next piece's rows): sixteen warps that all do the same at the same time.  Reading dQ under the next piece's first tile instead
+// of behind the last one changed nothing.
 constexpr int kDqCols = 32;
 constexpr int kDqGroups = kRows / kDqCols;
 constexpr int kDqPoly = 3;                 // of eight pairs of exponentials, on the FMA pipe
@@ -842,8 +852,10 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 // dK / dV: lanes = 128 key rows, columns = 64 query rows of a streamed tile
 // ------------------------------------------------------------------------------------------------------
 // A CTA owns 128 keys of one key head and walks a range of the query tiles of all heads that share it; K and V stay in shared memory,
-// dK and dV in tensor memory.  S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q: 2560 tensor cycles per 128 x 128 scores.  The
-// range is cut so that the CTAs fill whole waves of SMs; parts are added by a kernel of their own, in the order of the cuts.
+// dK and dV in tensor memory.  S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q: 2560 tensor cycles per 128 x 128 scores, which is
+// what bounds it at D = 128: [1, 8, 92160, 128] x 512 keys 257 us, 1500 TFLOP/s.  At D = 64 a step's chain does (139 us at
+// [2, 12 + 4, 8190, 64] x 801 of 1001 keys; with two buffers and all exponentials on the MUFU 155).  The range is cut so that the CTAs
+// fill whole waves of SMs; parts are added by a kernel of their own, in the order of the cuts.
 constexpr int kQTile = 64;
 constexpr int kSlab = kQTile * 128;
 constexpr int kDkCols = 32;
