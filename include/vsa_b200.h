@@ -479,6 +479,7 @@ int vsa_rotary(const VsaRotary* a, void* stream);
  *   lse2      [B * H, Lq rounded up to 128] fp32: base-2 log-sum-exp of the scaled scores, +inf for rows without a live key and
  *             for the padding; written by the forward, read by the backward
  *   delta     the same shape, scratch of the backward
+ *   dk, dv    both NULL: the pass over the keys is left out
  *   workspace vsa_cross_workspace_bytes(backward, ..., key_bits != NULL) bytes (0: may be NULL), 16-byte aligned, free again after the
  *             call
  * bf16 and fp16 with head dims that are multiples of 8 up to 128, 16-byte aligned pointers and strides of multiples of 8 run on

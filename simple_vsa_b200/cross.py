@@ -32,36 +32,50 @@ def _usable(x: Tensor) -> Tensor:
     return x
 
 
+_PACK = _lib.Cross.PACK.pack
+_ARGUMENTS = _lib.Cross.from_buffer_copy
 _NO_STRIDES = (0, 0, 0)
 
 
-def _launch(name: str, backward: int, scale: float, dt: int, q, k, v, out, lse, kv_lengths, key_bits, dout=None, dq=None, dk=None,
-            dv=None, delta=None) -> None:
-    B, H, Lq, D = q.shape
-    Hkv, Lkv = k.shape[1], k.shape[2]
+def _steps(x: Optional[Tensor], raster: bool):
+    """Batch, head and token stride."""
+    if x is None:
+        return _NO_STRIDES
+    a, b, c, _ = x.stride()
+    return (a, c, b) if raster else (a, b, c)
+
+
+def _launch(name: str, backward: int, raster: bool, scale: float, dt: int, q, k, v, out, lse, kv_lengths, key_bits, dout=None,
+            dq=None, dk=None, dv=None, delta=None) -> None:
+    if raster:
+        (B, Lq, H, D), (_, Lkv, Hkv, _) = q.shape, k.shape
+    else:
+        (B, H, Lq, D), (_, Hkv, Lkv, _) = q.shape, k.shape
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     n = _lib.lib.vsa_cross_workspace_bytes(backward, B, H, Hkv, Lq, Lkv, D, dt, key_bits is not None)
     ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n > 0 else None
-    grads = (*dout.stride()[:3], *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3]) if backward else _NO_STRIDES * 4
-    a = _lib.Cross.from_buffer_copy(_lib.Cross.PACK.pack(
+    grads = (*_steps(dout, raster), *_steps(dq, raster), *_steps(dk, raster), *_steps(dv, raster)) if backward else _NO_STRIDES * 4
+    a = _ARGUMENTS(_PACK(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(dout), out.data_ptr(), ptr(dq), ptr(dk), ptr(dv), lse.data_ptr(), ptr(delta),
-        ptr(kv_lengths), ptr(key_bits), ptr(ws), B, H, Hkv, Lq, Lkv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-        *out.stride()[:3], *grads, scale, D, dt))
+        ptr(kv_lengths), ptr(key_bits), ptr(ws), B, H, Hkv, Lq, Lkv, *_steps(q, raster), *_steps(k, raster), *_steps(v, raster),
+        *_steps(out, raster), *grads, scale, D, dt))
     call(name, a, ops._stream(q.device))
 
 
-def _forward(q, k, v, kv_lengths, key_bits, scale: float):
+def _forward(q, k, v, kv_lengths, key_bits, scale: float, raster: bool):
     B, H, L, D = q.shape
+    if raster:
+        H, L = L, H
     out = torch.empty_like(q)
     lse = torch.empty((B * H, -(-L // 128) * 128), device=q.device, dtype=torch.float32)
-    _launch("vsa_cross_fwd", 0, scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits)
+    _launch("vsa_cross_fwd", 0, raster, scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits)
     return out, lse
 
 
 def _key_bits(kv_mask: Tensor, kv_lengths: Optional[Tensor]) -> Tensor:
     """The mask packed to a bit per key, whole tiles of 128 keys, the lengths folded in."""
     B, T = kv_mask.shape
-    bits = torch.empty((B, _lib.lib.vsa_cross_words(T)), device=kv_mask.device, dtype=torch.int32)
+    bits = torch.empty((B, -(-T // 128) * 4), device=kv_mask.device, dtype=torch.int32)
     call("vsa_cross_key_bits", kv_mask.data_ptr(), kv_mask.stride(0), ops._ptr(kv_lengths), bits.data_ptr(), B, T,
          ops._stream(kv_mask.device))
     return bits
@@ -69,10 +83,10 @@ def _key_bits(kv_mask: Tensor, kv_lengths: Optional[Tensor]) -> Tensor:
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, kv_lengths, key_bits, scale):
-        out, lse = _forward(q, k, v, kv_lengths, key_bits, scale)
+    def forward(ctx, q, k, v, kv_lengths, key_bits, scale, raster):
+        out, lse = _forward(q, k, v, kv_lengths, key_bits, scale, raster)
         ctx.save_for_backward(q, k, v, out, lse, kv_lengths, key_bits)
-        ctx.scale = scale
+        ctx.scale, ctx.raster = scale, raster
         return out
 
     @staticmethod
@@ -80,26 +94,27 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, key_bits = ctx.saved_tensors
         with torch.cuda.device(q.device):
-            dq, dk, dv, delta = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), torch.empty_like(lse)
-            _launch("vsa_cross_bwd", 1, ctx.scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits,
+            dq, delta = torch.empty_like(q), torch.empty_like(lse)
+            # the pass over the keys is left out where neither needs its gradient
+            dk, dv = (torch.empty_like(k), torch.empty_like(v)) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
+            _launch("vsa_cross_bwd", 1, ctx.raster, ctx.scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits,
                     _usable(dout), dq, dk, dv, delta)
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None, None, None, None
 
 
 def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
     layout = "[batch, seq_len, heads, head_dim]" if raster else "[batch, heads, seq_len, dim]"
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"q, k, and v must have shape {layout}")
-    if raster:
-        q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
-    B, H, L, D = q.shape
-    T = k.shape[2]
+    seq, head = (1, 2) if raster else (2, 1)
+    B, H, D = q.shape[0], q.shape[head], q.shape[3]
+    T, Hkv = k.shape[seq], k.shape[head]
     if k.shape[0] != B or v.shape[0] != B:
         raise ValueError("q, k, and v must share the batch dimension")
-    if v.shape[1] != k.shape[1] or v.shape[2] != T:
+    if v.shape[head] != Hkv or v.shape[seq] != T:
         raise ValueError("k and v must have the same heads and sequence length")
-    if k.shape[1] == 0 and H or k.shape[1] and H % k.shape[1]:
-        raise ValueError(f"the {H} query heads must be a multiple of the {k.shape[1]} key heads")
+    if Hkv == 0 and H or Hkv and H % Hkv:
+        raise ValueError(f"the {H} query heads must be a multiple of the {Hkv} key heads")
     if k.shape[3] != D or v.shape[3] != D:
         raise ValueError("q, k, and v must have the same head dimension")
     if not 1 <= D <= 256:
@@ -124,9 +139,9 @@ def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
             key_bits = _key_bits(kv_mask if T <= 1 or kv_mask.stride(1) == 1 else kv_mask.contiguous(), kv_lengths)
         q, k, v = _usable(q), _usable(k), _usable(v)
         need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-        out = _CrossAttention.apply(q, k, v, kv_lengths, key_bits, scale) if need_grad else \
-            _forward(q, k, v, kv_lengths, key_bits, scale)[0]
-    return out.transpose(1, 2) if raster else out
+        if need_grad:
+            return _CrossAttention.apply(q, k, v, kv_lengths, key_bits, scale, raster)
+        return _forward(q, k, v, kv_lengths, key_bits, scale, raster)[0]
 
 
 def video_cross_attn(q: Tensor, k: Tensor, v: Tensor, kv_lengths: Optional[Tensor] = None, *, kv_mask: Optional[Tensor] = None,

@@ -711,7 +711,7 @@ static int check_cross(const VsaCross* a, bool backward, const char* what) {
   VSA_REQUIRE(!rows || (a->q && a->out && a->lse2), "%s: null pointer", what);
   VSA_REQUIRE(!rows || !keys || (a->k && a->v), "%s: null pointer", what);
   VSA_REQUIRE(!backward || !rows || (a->dout && a->dq && a->delta), "%s: null pointer", what);
-  VSA_REQUIRE(!backward || !keys || (a->dk && a->dv), "%s: null pointer", what);
+  VSA_REQUIRE(!backward || (a->dk == nullptr) == (a->dv == nullptr), "%s: give dk and dv, or neither", what);
   VSA_REQUIRE(a->workspace || cross_space(backward, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr).bytes == 0,
               "%s: a workspace is needed", what);
   VSA_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 16 == 0, "%s: the workspace is not 16-byte aligned", what);
@@ -769,16 +769,17 @@ int vsa_cross_bwd(const VsaCross* a, void* stream) {
   int rc = check_cross(a, true, "cross attention backward");
   if (rc || a->B == 0 || a->Hkv == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->Lq == 0 || a->H == 0) return a->Lkv == 0 ? VSA_OK : cross_sum(*a, 0, nullptr, st);       // no query: zeros
+  const bool keys = a->Lkv > 0 && a->dk != nullptr;
+  if (a->Lq == 0 || a->H == 0) return keys ? cross_sum(*a, 0, nullptr, st) : VSA_OK;       // no query: zeros
   const CrossSpace s = cross_space(true, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr);
   float* part = (float*)a->workspace;
   if (!cross_on_umma(*a, true) || a->key_bits == nullptr) {
     const bool parts = s.splits > 1;
     rc = cross_on_umma(*a, true) ? cross_bwd_umma(*a, s.splits, parts, part, st) : cross_bwd_generic(*a, s.splits, part, st);
-    return rc || !parts ? rc : cross_sum(*a, s.splits, part, st);
+    return rc || !parts || !keys ? rc : cross_sum(*a, s.splits, part, st);
   }
   VsaCross c;
-  if ((rc = compacted(*a, s, &c, st)) || (rc = cross_bwd_umma(c, s.splits, true, part, st))) return rc;
+  if ((rc = compacted(*a, s, &c, st)) || (rc = cross_bwd_umma(c, s.splits, true, part, st)) || !keys) return rc;
   return cross_sum(*a, s.splits, part, st, (const int32_t*)((uint8_t*)a->workspace + s.prefix));
 }
 

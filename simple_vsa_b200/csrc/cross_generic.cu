@@ -537,7 +537,7 @@ int bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   // dQ on tiles of 32 x 32 where tiles of 64 leave SMs without work ([1, 2, 1025, 64] x 333: 34 CTAs, 67 us; 66 CTAs, 58)
   using Small = Tile<TL::DP, 32>;
   int rc = TL::KT == 64 && a.B * a.H * ((a.Lq + 63) / 64) < 148 ? dq_pass<T, Small>(a, st) : dq_pass<T, TL>(a, st);
-  if (rc || a.Lkv == 0) return rc;
+  if (rc || a.Lkv == 0 || a.dk == nullptr) return rc;
   const int bytes = (4 * TL::floats + 2 * TL::score_floats) * 4;
   if ((rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV"))) return rc;
   cross_dkdv_generic_kernel<T, TL><<<dim3((unsigned)((a.Lkv + TL::KT - 1) / TL::KT * splits), (unsigned)a.Hkv, (unsigned)a.B), kThreads, bytes,

@@ -1213,7 +1213,7 @@ int launch_bwd(const VsaCross& a, int splits, bool parts, float* part, cudaStrea
   const int64_t sms = device_sms();
   cross_dq_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kDqThreads, DqSmem<HD>::total, st>>>(
       mq, mdo, mk, mv, mdq, a, Divisor((uint32_t)qtiles), Divisor((uint32_t)a.H), Divisor((uint32_t)(a.H / a.Hkv)), (int)items, status);
-  if ((rc = check_launch("cross_dq_umma_kernel"))) return rc;
+  if ((rc = check_launch("cross_dq_umma_kernel")) || a.dk == nullptr) return rc;
   cross_dkdv_umma_kernel<T, HD><<<(unsigned)units, kDkThreads, DkSmem<HD>::total, st>>>(mq64, mdo64, mk, mv, a, (int)ktiles, splits, parts ? part : nullptr, status);
   return check_launch("cross_dkdv_umma_kernel");
 }
@@ -1238,7 +1238,7 @@ bool cross_aligned(const VsaCross& a, bool backward) {
       !aligned(a.out, a.out_stride, a.H, a.Lq, a.B))
     return false;
   return !backward || (aligned(a.dout, a.dout_stride, a.H, a.Lq, a.B) && aligned(a.dq, a.dq_stride, a.H, a.Lq, a.B) &&
-                       aligned(a.dk, a.dk_stride, a.Hkv, a.Lkv, a.B) && aligned(a.dv, a.dv_stride, a.Hkv, a.Lkv, a.B));
+                       (a.dk == nullptr || (aligned(a.dk, a.dk_stride, a.Hkv, a.Lkv, a.B) && aligned(a.dv, a.dv_stride, a.Hkv, a.Lkv, a.B))));
 }
 
 int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {

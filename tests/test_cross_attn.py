@@ -263,6 +263,21 @@ def test_empty_extents(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float32, 24)])
+def test_gradients_of_some_operands_only(dtype, D):
+    q, k, v, dout = _inputs(2, 4, 2, 130, 140, D, dtype, 11)
+    mask = torch.ones(2, 140, dtype=torch.bool, device=DEV)
+    mask[0, 3:70] = False
+    for kw in (dict(), dict(kv_mask=mask)):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        want = torch.autograd.grad(V.video_cross_attn(*leaves, **kw), leaves, dout)
+        for need in ((0,), (1,), (2,), (0, 2)):
+            xs = [x.clone().requires_grad_(i in need) for i, x in enumerate((q, k, v))]
+            got = torch.autograd.grad(V.video_cross_attn(*xs, **kw), [xs[i] for i in need], dout)
+            assert all(torch.equal(g, want[i]) for g, i in zip(got, need))
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_device():
     q, k, v, _ = _inputs(2, 2, 2, 6, 5, 16, torch.bfloat16, 7)
     for bad, match in ((dict(k=k.half(), v=v.half()), "dtype"), (dict(kv_lengths=torch.tensor([5])), "2 integers"),
