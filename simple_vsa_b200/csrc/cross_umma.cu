@@ -514,8 +514,7 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 constexpr int kDqCols = 32;
 constexpr int kDqGroups = kRows / kDqCols;
 constexpr int kDqPoly = 3;                 // of eight pairs of exponentials, on the FMA pipe
-constexpr int kDqEwThreads = 128 * kDqGroups;
-constexpr int kDqThreads = 128 + kDqEwThreads;
+constexpr int kDqThreads = 384 + 128 * kDqGroups;      // loads and issuers of MMAs, dQ out, delta, elementwise warps
 template <int HD>
 struct DqSmem {
   static constexpr uint32_t tile = HD * 256;
@@ -524,15 +523,15 @@ struct DqSmem {
   static constexpr uint32_t d_o = q + tile;
   static constexpr uint32_t k = d_o + tile;
   static constexpr uint32_t v = k + k_stages * tile;
-  static constexpr uint32_t stage = v + v_stages * tile;          // 32 rows x 64 bytes an elementwise warp
-  static constexpr uint32_t delta = stage + 16 * 2048;            // float [2][128]
-  static constexpr uint32_t bars = delta + 1024;
+  static constexpr uint32_t stage = v + v_stages * tile;          // 32 rows x 64 bytes x HD / 32 a helper warp
+  static constexpr uint32_t stats = stage + 4 * (HD / 32) * 2048; // float2 [2][128]: delta and the statistic of a row
+  static constexpr uint32_t bars = stats + 2048;
   static constexpr uint32_t misc = bars + 32 * 8;
   static constexpr uint32_t total = misc + 16;
 };
 static_assert(DqSmem<128>::total <= 232448, "shared memory of the cross attention dQ pass");
 enum DqBar { Q_QDO_FULL = 0, Q_QDO_EMPTY = 1, Q_K_FULL = 2, Q_K_EMPTY = 5, Q_V_FULL = 8, Q_V_EMPTY = 10, Q_S_FULL = 12, Q_S_EMPTY = 14,
-             Q_DP_FULL = 16, Q_DP_EMPTY = 17, Q_DS_FULL = 18, Q_ACC_FULL = 20 };
+             Q_DP_FULL = 16, Q_DP_EMPTY = 17, Q_DS_FULL = 18, Q_ACC_FULL = 20, Q_ACC_EMPTY = 21, Q_STATS_FULL = 22, Q_STATS_EMPTY = 24 };
 
 struct DqItem {
   int b, h, row0, len, n;                       // n key tiles
@@ -566,7 +565,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   auto bar = [&](int i) -> uint32_t { return base + Sm::bars + 8u * i; };
   if (tid == 0) {
     mbar_init(bar(Q_QDO_FULL), 1);
-    mbar_init(bar(Q_QDO_EMPTY), 2 + 4 * kDqGroups);      // the last products that read them, and the warps that read dO
+    mbar_init(bar(Q_QDO_EMPTY), 2);              // the last products that read them
     for (int i = 0; i < Sm::k_stages; ++i) {
       mbar_init(bar(Q_K_FULL + i), 1);
       mbar_init(bar(Q_K_EMPTY + i), 1);
@@ -577,7 +576,10 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       mbar_init(bar(Q_S_FULL + i), 1);
       mbar_init(bar(Q_S_EMPTY + i), 1);
       mbar_init(bar(Q_DS_FULL + i), 4 * kDqGroups);
+      mbar_init(bar(Q_STATS_FULL + i), 4);
+      mbar_init(bar(Q_STATS_EMPTY + i), 4 * kDqGroups);
     }
+    mbar_init(bar(Q_ACC_EMPTY), 4);
     mbar_init(bar(Q_DP_FULL), 1);
     mbar_init(bar(Q_DP_EMPTY), 4 * kDqGroups);
     mbar_init(bar(Q_ACC_FULL), 1);
@@ -682,6 +684,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       for (int j = 0; j < it.n && ok; ++j, ++n) {
         const uint32_t s = n % Sm::k_stages, b = n & 1;
         ok = CROSS_WAIT(bar(Q_K_FULL + s), (n / Sm::k_stages) & 1) && CROSS_WAIT(bar(Q_DS_FULL + b), (n >> 1) & 1);
+        if (ok && j == 0) ok = CROSS_WAIT(bar(Q_ACC_EMPTY), (live_items++ & 1) ^ 1);      // dQ of the piece before has been read
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -694,71 +697,133 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
     }
     if (!ok && lane == 0) atomicCAS(status, 0, 84);
-  } else {
-    const int quarter = warp & 3, cg = (warp - 4) >> 2, row = quarter * 32 + lane;
-    const int c0 = cg * kDqCols, st = tid - 128;
+  } else if (warp < 8) {
+    // dQ of a piece on its way out while the elementwise warps are at the next one.
+    const int quarter = warp & 3, st = tid - 128;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const float c = a.scale * kLog2e, log_scale = log2f(fabsf(a.scale));
-    const float2 c2 = make_float2(c, c);
-    const long long lp = cross_rows(a.Lq);
-    // delta: four neighbouring threads a row, HD/4 dims each
-    const int dr = st / kDqGroups, part = st % kDqGroups;
-    constexpr int kPieces = HD / kDqGroups / 8;                  // of 8 dims
-    uint4 out_r[kPieces];
-    float lse_r = 0.f;
-    auto fetch = [&](int item) {
+    uint8_t* stage = sm + Sm::stage + quarter * (HD / 32) * 2048;
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const DqItem it(a, qtiles, heads, item);
-      const T* o = (const T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1] + (long long)(it.row0 + dr) * a.out_stride[2];
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int d = (i * kDqGroups + part) * 8;
-        out_r[i] = it.row0 + dr < a.Lq && d < a.D ? *reinterpret_cast<const uint4*>(o + d) : make_uint4(0, 0, 0, 0);
-      }
-      lse_r = a.lse2[((long long)it.b * a.H + it.h) * lp + it.row0 + row];
-    };
-    if ((int)blockIdx.x < items) fetch(blockIdx.x);
-    uint32_t pieces = 0;                                         // all pieces so far, of which live_items have key tiles
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++pieces) {
-      const DqItem it(a, qtiles, heads, item);
-      const long long bh = (long long)it.b * a.H + it.h;
-      T* dq = (T*)a.dq + it.b * a.dq_stride[0] + it.h * a.dq_stride[1] + (long long)(it.row0 + row) * a.dq_stride[2];
-      const bool there = it.row0 + row < a.Lq;
-      if (it.n == 0) {                                           // no key: zeros
-        if (part == 0) a.delta[bh * lp + it.row0 + dr] = 0.f;
-#pragma unroll
-        for (int d = c0; d < c0 + kDqCols; d += 8)
-          if (there && d < a.D) *reinterpret_cast<uint4*>(dq + d) = make_uint4(0, 0, 0, 0);
-        if (item + (int)gridDim.x < items) fetch(item + gridDim.x);
+      if (it.n == 0) {                           // no key: zeros
+        const long long stat = ((long long)it.b * a.H + it.h) * cross_rows(a.Lq) + it.row0;
+        T* dq = (T*)a.dq + it.b * a.dq_stride[0] + it.h * a.dq_stride[1] + (long long)it.row0 * a.dq_stride[2];
+        a.delta[stat + st] = 0.f;
+        for (int i = st; i < kRows * (HD / 8); i += 128) {
+          const int r = i / (HD / 8), d = i % (HD / 8) * 8;
+          if (it.row0 + r < a.Lq && d < a.D) *reinterpret_cast<uint4*>(dq + r * a.dq_stride[2] + d) = make_uint4(0, 0, 0, 0);
+        }
         continue;
       }
-      ok = CROSS_WAIT(bar(Q_QDO_FULL), live_items & 1);
+      ok = CROSS_WAIT(bar(Q_ACC_FULL), live_items & 1);
       if (!ok) break;
-      float* s_delta = reinterpret_cast<float*>(sm + Sm::delta) + (live_items & 1) * kRows;
-      {
-        float acc = 0.f;
+      ++live_items;
+      tc_fence_after();
+      if (lane == 0) bulk_wait_read();           // the boxes before have left the buffer
+      __syncwarp();
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t av[32];
+        tmem_ld(tmem_acc + lane_addr + 32 * c, av);
+        tmem_ld_wait();
+        if (c == HD / 32 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(Q_ACC_EMPTY));
+        }
+        // TMA's 64-byte swizzle (pieces xor row / 2); what lies outside the tensor is not written
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int ch = i * kDqGroups + part;                   // 16-byte piece of the row
-          const uint4 x = *reinterpret_cast<const uint4*>(sm + Sm::d_o + (ch >> 3) * kHalf + dr * 128 + (((ch ^ dr) & 7) << 4));
-          const uint32_t *p = &out_r[i].x, *q = &x.x;
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(stage + c * 2048 + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = pack8<T>(av + 8 * q);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        for (int c = 0; c < HD / 32; ++c)
+          if (it.row0 + quarter * 32 < a.Lq && 32 * c < a.D)
+            tma_store_4d(&map_dq, smem_u32(stage) + c * 2048, 32 * c, it.row0 + quarter * 32, it.h, it.b);
+        bulk_commit();
+      }
+    }
+    if (lane == 0) bulk_wait();
+    if (!ok && lane == 0) atomicCAS(status, 0, 86);
+  } else if (warp < 12) {
+    // delta and the statistics of the next piece's rows while this one is worked on
+    const int st = tid - 256;
+    const float log_scale = log2f(a.scale);      // > 0
+    const long long lp = cross_rows(a.Lq);
+    // The rows of the next piece into L2: its loads come when there is room for them, too late to wait for memory.
+    auto ask = [&](const void* p, const int64_t(&stride)[3], const DqItem& it) {
+      const T* row = (const T*)p + it.b * stride[0] + it.h * stride[1] + (long long)min(it.row0 + st, (int)a.Lq - 1) * stride[2];
+#pragma unroll
+      for (int d = 0; d < HD; d += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + min(d, a.D - 1)));
+    };
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const DqItem it(a, qtiles, heads, item);
+      if (item + (int)gridDim.x < items) {
+        const DqItem next(a, qtiles, heads, item + gridDim.x);
+        ask(a.out, a.out_stride, next);
+        ask(a.q, a.q_stride, next);
+        ask(a.dout, a.dout_stride, next);
+      }
+      if (it.n == 0) continue;
+      ok = CROSS_WAIT(bar(Q_STATS_EMPTY + (live_items & 1)), ((live_items >> 1) & 1) ^ 1);
+      if (!ok) break;
+      float2* to = reinterpret_cast<float2*>(sm + Sm::stats) + (live_items & 1) * kRows;
+      const long long stat = ((long long)it.b * a.H + it.h) * lp + it.row0;
+      const T* o = (const T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1] + (long long)it.row0 * a.out_stride[2];
+      const T* g = (const T*)a.dout + it.b * a.dout_stride[0] + it.h * a.dout_stride[1] + (long long)it.row0 * a.dout_stride[2];
+      // four neighbouring threads a row, 16-byte pieces in turn
+#pragma unroll 1
+      for (int r = st >> 2; r < kRows; r += 32) {
+        uint4 x[HD / 32], y[HD / 32];
+        const int rr = min(it.row0 + r, (int)a.Lq - 1) - it.row0;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+          const int d = min((4 * i + (st & 3)) * 8, a.D - 8);
+          x[i] = *reinterpret_cast<const uint4*>(o + rr * a.out_stride[2] + d);
+          y[i] = *reinterpret_cast<const uint4*>(g + rr * a.dout_stride[2] + d);
+        }
+        const float lse = a.lse2[stat + r];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+          if ((4 * i + (st & 3)) * 8 >= a.D) continue;
+          const uint32_t *p = &x[i].x, *q = &y[i].x;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 u = Elem<T>::unpack(p[e]), y = Elem<T>::unpack(q[e]);
-            acc = fmaf(u.x, y.x, fmaf(u.y, y.y, acc));
+            const float2 u = Elem<T>::unpack(p[e]), w = Elem<T>::unpack(q[e]);
+            sum = fmaf(u.x, w.x, fmaf(u.y, w.y, sum));
           }
         }
-#pragma unroll
-        for (int o = 1; o < kDqGroups; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-        if (part == 0) {
-          s_delta[dr] = acc;
-          a.delta[bh * lp + it.row0 + dr] = acc;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if ((st & 3) == 0) {
+          if (it.row0 + r >= a.Lq) sum = 0.f;
+          a.delta[stat + r] = sum;
+          to[r] = make_float2(sum, log_scale - lse);             // 2^(s c - lse) * scale in one exponential
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(Q_QDO_EMPTY));
-      named_barrier(1, kDqEwThreads);
-      const float dl = s_delta[row], neg_lse = log_scale - lse_r;        // 2^(s c - lse) * |scale| in one exponential
-      const float2 l2 = make_float2(neg_lse, neg_lse), d2 = make_float2(-dl, -dl);
+      if (lane == 0) mbar_arrive(bar(Q_STATS_FULL + (live_items & 1)));
+      ++live_items;
+    }
+    if (!ok && lane == 0) atomicCAS(status, 0, 87);
+  } else {
+    const int quarter = warp & 3, cg = (warp - 12) >> 2, row = quarter * 32 + lane, c0 = cg * kDqCols;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const float c = a.scale * kLog2e;
+    const float2 c2 = make_float2(c, c);
+    const float2* stats = reinterpret_cast<const float2*>(sm + Sm::stats) + row;
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const DqItem it(a, qtiles, heads, item);
+      if (it.n == 0) continue;
+      ok = CROSS_WAIT(bar(Q_STATS_FULL + (live_items & 1)), (live_items >> 1) & 1);
+      if (!ok) break;
+      const float2 row_stats = stats[(live_items & 1) * kRows];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(Q_STATS_EMPTY + (live_items & 1)));
+      ++live_items;
+      const float2 l2 = make_float2(row_stats.y, row_stats.y), d2 = make_float2(-row_stats.x, -row_stats.x);
       for (int j = 0; j < it.n; ++j, ++n) {
         const uint32_t b = n & 1;
         const int live = it.len - j * kRows;     // keys of this tile that take part, or more
@@ -766,37 +831,43 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         if (!ok) break;
         tc_fence_after();
         const uint32_t s_addr = tmem + b * 128 + lane_addr + c0;
-        uint32_t sv[kDqCols];
-        tmem_ld(s_addr, sv);
-        tmem_ld_wait();
         if (live < kRows && cg == 0) {           // rows of K that no key takes part with meet dS = 0: they must be finite (S is done)
           if (row >= live) {
             uint8_t* krow = sm + Sm::k + (n % Sm::k_stages) * Sm::tile + row * 128;
-#pragma unroll
+#pragma unroll 1
             for (int ch = 0; ch < HD / 8; ++ch)
               *reinterpret_cast<uint4*>(krow + (ch >> 3) * kHalf + ((ch ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
         float2 pf[kDqCols / 2];
+        uint32_t pk[kDqCols / 2];
 #pragma unroll
-        for (int i = 0; i < kDqCols / 2; ++i) {
-          pf[i] = exp2_pair<T>(fma2(word_pair(sv + 2 * i), c2, l2), kDqPoly > 0 && i % 8 < kDqPoly);
+        for (int h = 0; h < kDqCols; h += 16) {
+          uint32_t sv[16];
+          tmem_ld(s_addr + h, sv);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pf[h / 2 + i] = exp2_pair<T>(fma2(word_pair(sv + 2 * i), c2, l2), kDqPoly > 0 && i < kDqPoly);
         }
         ok = CROSS_WAIT(bar(Q_DP_FULL), n & 1);
         if (!ok) break;
         tc_fence_after();
-        uint32_t dv[kDqCols];
-        tmem_ld(tmem_dp + lane_addr + c0, dv);
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(Q_DP_EMPTY));
-        uint32_t pk[kDqCols / 2];
 #pragma unroll
-        for (int i = 0; i < kDqCols / 2; ++i) {
-          const float2 y = mul2(pf[i], add2(word_pair(dv + 2 * i), d2));
-          pk[i] = Elem<T>::pack(y.x, y.y);
+        for (int h = 0; h < kDqCols; h += 16) {
+          uint32_t dv[16];
+          tmem_ld(tmem_dp + lane_addr + c0 + h, dv);
+          tmem_ld_wait();
+          if (h + 16 == kDqCols) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Q_DP_EMPTY));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 y = mul2(pf[h / 2 + i], add2(word_pair(dv + 2 * i), d2));
+            pk[h / 2 + i] = Elem<T>::pack(y.x, y.y);
+          }
         }
         if (c0 + kDqCols > live) {               // what stands in a key that takes no part may be anything
 #pragma unroll
@@ -811,36 +882,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(Q_DS_FULL + b));
       }
-      if (!ok) break;
-      if (item + (int)gridDim.x < items) fetch(item + gridDim.x);
-      ok = CROSS_WAIT(bar(Q_ACC_FULL), live_items & 1);
-      if (!ok) break;
-      ++live_items;
-      tc_fence_after();
-      if (c0 < HD) {
-        uint32_t av[32];
-        tmem_ld(tmem_acc + lane_addr + c0, av);
-        tmem_ld_wait();
-        if (a.scale < 0.f) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) av[i] ^= 0x80000000u;
-        }
-        // TMA's 64-byte swizzle (pieces xor row / 2); what lies outside the tensor is not written.  Stored by the threads, 16 bytes a
-        // row and instruction, it took 3400 cycles of a piece's 17600.
-        uint8_t* stage = sm + Sm::stage + (warp - 4) * 2048;
-        if (lane == 0) bulk_wait_read();         // the box before has left the buffer
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = pack8<T>(av + 8 * q);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (it.row0 + quarter * 32 < a.Lq && c0 < a.D) tma_store_4d(&map_dq, smem_u32(stage), c0, it.row0 + quarter * 32, it.h, it.b);
-          bulk_commit();
-        }
-      }
     }
-    if (lane == 0) bulk_wait();
     if (!ok && lane == 0) atomicCAS(status, 0, 85);
   }
   tc_fence_before();
