@@ -66,7 +66,7 @@ def _forward(q, k, v, kv_lengths, key_bits, scale: float, raster: bool):
     B, H, L, D = q.shape
     if raster:
         H, L = L, H
-    out = torch.empty_like(q)
+    out = ops._like(q)
     lse = torch.empty((B * H, -(-L // 128) * 128), device=q.device, dtype=torch.float32)
     _launch("vsa_cross_fwd", 0, raster, scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits)
     return out, lse
@@ -94,9 +94,9 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, key_bits = ctx.saved_tensors
         with torch.cuda.device(q.device):
-            dq, delta = torch.empty_like(q), torch.empty_like(lse)
+            dq, delta = ops._like(q), torch.empty_like(lse)
             # the pass over the keys is left out where neither needs its gradient
-            dk, dv = (torch.empty_like(k), torch.empty_like(v)) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
+            dk, dv = (ops._like(k), ops._like(v)) if ctx.needs_input_grad[1] or ctx.needs_input_grad[2] else (None, None)
             _launch("vsa_cross_bwd", 1, ctx.raster, ctx.scale, ops._check_device_dtype(q, k, v), q, k, v, out, lse, kv_lengths, key_bits,
                     _usable(dout), dq, dk, dv, delta)
         return dq, dk, dv, None, None, None, None

@@ -101,6 +101,13 @@ def _dense(x: Tensor) -> Tensor:
     return x
 
 
+def _like(x: Tensor) -> Tensor:
+    """An empty tensor in x's order of dims, head dim contiguous.  (Rows that overlap by one element, windows of a longer one, have
+    two dims of stride 1, and ``empty_like`` may put the other one innermost.)"""
+    y = torch.empty_like(x)
+    return y if y.stride(3) == 1 or y.shape[3] <= 1 else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
 def _sizes(sizes: Tensor, device) -> Tensor:
     return sizes.to(device=device, dtype=torch.int32).contiguous()
 

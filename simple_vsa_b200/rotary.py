@@ -135,7 +135,7 @@ def rotate(xs, ys, cos, sin, interleaved: bool, inverse: bool, *, x_raster: bool
 
 def _turned(q, k, cos, sin, positions, interleaved, raster):
     xs = [_rows(x) for x in ((q,) if k is None else (q, k))]
-    ys = [torch.empty_like(x) for x in xs]
+    ys = [ops._like(x) for x in xs]
     rotate(xs, ys, cos, sin, interleaved, False, x_raster=raster, y_raster=raster, positions=positions)
     return ys[0], ys[1] if k is not None else None
 
@@ -156,7 +156,7 @@ class _Rotary(torch.autograd.Function):
         (cos, sin, positions), raster = ctx.saved_tensors, ctx.raster
         with torch.cuda.device(cos.device):
             there = [_rows(g) for g in (dq, dk) if g is not None]
-            back = [torch.empty_like(g) for g in there]
+            back = [ops._like(g) for g in there]
             if there:
                 rotate(there, back, cos, sin, ctx.interleaved, True, x_raster=raster, y_raster=raster, positions=positions)
         return back[0] if dq is not None else None, back[-1] if dk is not None else None, None, None, None, None, None

@@ -252,6 +252,21 @@ def test_strides_and_layouts(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.bfloat16, 20), (torch.float32, 64)])
+def test_windows_of_a_longer_row(dtype, D):
+    """Rows that overlap by an element: two dims of stride 1."""
+    B, H, n = 2, 3, 5
+    rows = [torch.randn(B, H, n + D - 1, generator=torch.Generator().manual_seed(20 + i)).to(dtype).to(DEV) for i in range(4)]
+    q, k, v, dout = (x.unfold(-1, D, 1) for x in rows)
+    dense = [x.contiguous() for x in (q, k, v)]
+    want = _run(*dense, dout.contiguous())
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    out = V.video_cross_attn(*leaves)
+    got = (out, *torch.autograd.grad(out, leaves, dout))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_empty_extents(dtype):
     for B, H, Hk, L, T in ((0, 2, 2, 5, 5), (2, 2, 1, 0, 5), (2, 2, 1, 5, 0), (1, 0, 0, 5, 5), (1, 0, 2, 5, 5)):

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import simple_vsa_b200 as V
+from simple_vsa_b200 import ops
 
 DEV = "cuda:0"
 
@@ -228,6 +229,32 @@ def test_strided_operands_and_gradients():
     swapped = qkv.permute(0, 3, 2, 1)[:, :32]              # head dim not contiguous: copied first
     assert torch.equal(V.video_rotary(swapped, None, V.build_rotary_metadata((3 * H,), 10)),
                        V.video_rotary(swapped.contiguous(), None, V.build_rotary_metadata((3 * H,), 10)))
+
+
+def test_outputs_keep_a_contiguous_head_dim():
+    """Windows of a longer row have two dims of stride 1; what is made like them is indexed with a contiguous head dim."""
+    for n in (5, 64, 137):
+        x = torch.zeros(2, 3, n + 63).unfold(-1, 64, 1)
+        y = ops._like(x)
+        assert y.shape == x.shape and y.stride(3) == 1 and ops._like(x.transpose(1, 2)).stride(3) == 1
+    x = torch.zeros(2, 9, 3, 64).transpose(1, 2)
+    assert ops._like(x).stride() == x.stride()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [True, False])
+def test_windows_of_a_longer_row(dtype, interleaved):
+    g = torch.Generator().manual_seed(12)
+    rot = V.build_rotary_metadata((5,), 32, device=DEV, interleaved=interleaved)
+    x = torch.randn(2, 3, 68, generator=g).to(dtype).to(DEV).unfold(-1, 64, 1)
+    want = V.video_rotary(x.contiguous(), None, rot)
+    assert torch.equal(V.video_rotary(x, None, rot), want)
+    assert torch.equal(V.video_rotary_raster(x.transpose(1, 2), None, rot), want.transpose(1, 2))
+    leaf = torch.zeros(2, 3, 5, 64, device=DEV, dtype=dtype, requires_grad=True)
+    (dx,) = torch.autograd.grad(V.video_rotary(leaf, None, rot), leaf, x)
+    (dy,) = torch.autograd.grad(V.video_rotary(leaf, None, rot), leaf, x.contiguous())
+    assert torch.equal(dx, dy)
 
 
 @pytest.mark.gpu
