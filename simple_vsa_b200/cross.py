@@ -120,9 +120,8 @@ def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
     if not 1 <= D <= 256:
         raise ValueError(f"cross attention supports head dimensions from 1 to 256, got {D}")
     ops._check_device_dtype(q, k, v)
-    if kv_lengths is not None and (kv_lengths.is_floating_point() or kv_lengths.is_complex() or kv_lengths.dtype == torch.bool
-                                   or tuple(kv_lengths.shape) != (B,)):
-        raise ValueError(f"kv_lengths must hold {B} integers, one per sample")
+    if kv_lengths is not None and (not ops._integers(kv_lengths) or tuple(kv_lengths.shape) != (B,)):
+        raise ValueError(f"kv_lengths must hold {B} integers of a signed type or uint8, one per sample")
     if kv_mask is not None and (kv_mask.dtype != torch.bool or tuple(kv_mask.shape) != (B, T)):
         raise ValueError(f"kv_mask must be a bool tensor of shape [{B}, {T}], True where a key takes part")
     scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D)

@@ -584,11 +584,12 @@ int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st,
   return a.dtype == VSA_F16 ? sum_of<__half>(a, splits, part, prefix, st) : sum_of<__nv_bfloat16>(a, splits, part, prefix, st);
 }
 int cross_compact(const VsaCross& a, int32_t* prefix, int32_t* counts, void* k, void* v, cudaStream_t st) {
+  const int64_t rows = a.B * a.Hkv * a.Lkv;
+  if (rows > 0x7fffffffLL) return fail(VSA_ERR_UNSUPPORTED, "cross attention: too many key rows for a mask");
   cross_rank_kernel<<<(unsigned)a.B, 1024, 0, st>>>(a.key_bits, (int)cross_words(a.Lkv), prefix, counts);
   const int rc = check_launch("cross_rank_kernel");
   if (rc) return rc;
   const int x = a.D <= 64 ? 8 : 16, y = 256 / x;
-  const int64_t rows = a.B * a.Hkv * a.Lkv;
   cross_compact_kernel<<<(unsigned)((rows + y - 1) / y), dim3((unsigned)x, (unsigned)y), 0, st>>>(a, prefix, counts, (uint4*)k, (uint4*)v);
   return check_launch("cross_compact_kernel");
 }

@@ -108,6 +108,11 @@ def _like(x: Tensor) -> Tensor:
     return y if y.stride(3) == 1 or y.shape[3] <= 1 else torch.empty(x.shape, device=x.device, dtype=x.dtype)
 
 
+def _integers(x: Tensor) -> bool:
+    """Whether int32 holds x's values, or int64 does and they can be clamped (uint32 and uint64 would wrap)."""
+    return x.dtype in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
 def _sizes(sizes: Tensor, device) -> Tensor:
     return sizes.to(device=device, dtype=torch.int32).contiguous()
 

@@ -178,8 +178,8 @@ def _turn(q: Tensor, k: Optional[Tensor], rotary: Dict[str, object], positions: 
         if cos.shape[0] < L:
             raise ValueError(f"the rotary table holds {cos.shape[0]} positions, the tensors hold {L} tokens")
     else:
-        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
-            raise ValueError("positions must be integers")
+        if not ops._integers(positions):
+            raise ValueError("positions must be integers of a signed type or uint8")
         if tuple(positions.shape) not in ((L,), (B, L)):
             raise ValueError(f"positions must have shape [{L}] or [{B}, {L}], got {list(positions.shape)}")
         if positions.dtype == torch.int64:           # a position beyond 32 bits stays outside the table

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import simple_vsa_b200 as V
-from simple_vsa_b200 import _lib
+from simple_vsa_b200 import _lib, ops
 
 DEV = "cuda:0"
 
@@ -372,3 +372,52 @@ def test_whole_step_replays_from_a_cuda_graph(dtype):
             torch.cuda.synchronize()
             want = _run(*leaves, dout, lengths)
             assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+def test_lengths_and_positions_of_types_that_would_wrap_are_refused():
+    for dtype in (torch.uint32, torch.uint64, torch.bool, torch.float32):
+        assert not ops._integers(torch.zeros(2, dtype=dtype))
+    for dtype in (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8):
+        assert ops._integers(torch.zeros(2, dtype=dtype))
+
+
+@pytest.mark.gpu
+def test_integer_types_of_lengths_and_positions():
+    q, k, v, _ = _inputs(2, 2, 2, 6, 5, 16, torch.bfloat16, 21)
+    rot = V.build_rotary_metadata((9,), 16, device=DEV)
+    lengths, positions = torch.tensor([5, 2]), torch.tensor([0, 8, 3, 4, 1, 2])
+    want, turned = V.video_cross_attn(q, k, v, lengths), V.video_rotary(q, None, rot, positions=positions)
+    for dtype in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        assert torch.equal(V.video_cross_attn(q, k, v, lengths.to(dtype)), want)
+        assert torch.equal(V.video_rotary(q, None, rot, positions=positions.to(dtype)), turned)
+    for dtype in (torch.uint32, torch.uint64):
+        with pytest.raises(ValueError, match="signed"):
+            V.video_cross_attn(q, k, v, lengths.to(dtype))
+        with pytest.raises(ValueError, match="signed"):
+            V.video_rotary(q, None, rot, positions=positions.to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D,L", [(torch.bfloat16, 128, 300), (torch.float16, 64, 2), (torch.bfloat16, 20, 70), (torch.float32, 64, 70)])
+def test_offsets_beyond_32_bits(dtype, D, L):
+    """Samples of one buffer more than 2^31 elements apart, and a sample's keys that reach as far."""
+    B, H, T, far, row = 2, 2, 140, (1 << 31) + (1 << 23), 1 << 24
+    pool = torch.empty(far + T * row, device=DEV, dtype=dtype)
+    dense = _inputs(B, H, H, L, T, D, dtype, 22)
+    want = _run(*dense)
+    places = [pool.as_strided((B, H, x.shape[2], D), (far, 4096, row if i == 1 else 8192, 1), 512 * i) for i, x in enumerate(dense)]
+    for p, x in zip(places, dense):
+        p.copy_(x)
+    q, k, v, dout = places
+    mask = torch.ones(B, T, dtype=torch.bool, device=DEV)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    for kw in (dict(), dict(kv_mask=mask)):
+        out = V.video_cross_attn(*leaves, **kw)
+        got = (out.detach(), *torch.autograd.grad(out, leaves, dout))
+        if not kw:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        else:                                            # keys gathered first: the same sums, up to their order
+            for a, b in zip(got, want):
+                torch.testing.assert_close(a.float(), b.float(), rtol=4 * torch.finfo(dtype).eps, atol=4 * torch.finfo(dtype).eps * b.abs().max().item())
+    rot = V.build_rotary_metadata((max(L, T),), D if D % 4 == 0 else D - D % 4, device=DEV)
+    assert torch.equal(V.video_rotary(k, None, rot), V.video_rotary(dense[1], None, rot))
