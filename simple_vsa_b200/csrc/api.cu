@@ -656,14 +656,14 @@ static int cross_fwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64
     return (int)(s < 64 ? s : 64);
   }
   if (cross_umma_shape(D, dtype)) return cross_parts(B * H * ((Lq + 255) / 256), (Lkv + 127) / 128, 4, 64);
-  const int tile = cross_generic_tile(D);
-  return cross_parts(B * H * ((Lq + tile - 1) / tile), (Lkv + tile - 1) / tile, 2, 64);
+  const CrossTile tile = cross_generic_fwd_tile(B, H, Lq, Lkv, D);
+  return cross_parts(B * H * ((Lq + tile.rows - 1) / tile.rows), (Lkv + tile.cols - 1) / tile.cols, 2, 64);
 }
 static int cross_bwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
   // a step of the tensor path is 64 query rows; a CTA's set-up and epilogue and its share of the sum weigh about ten
   if (cross_umma_shape(D, dtype)) return cross_parts(B * Hkv * ((Lkv + 127) / 128), (H / Hkv) * ((Lq + 63) / 64), 10, 64);
-  const int tile = cross_generic_tile(D);
-  return cross_parts(B * Hkv * ((Lkv + tile - 1) / tile), (H / Hkv) * ((Lq + tile - 1) / tile), 2, 64);
+  const CrossTile tile = cross_generic_bwd_tile(B, H, Hkv, Lq, Lkv, D);
+  return cross_parts(B * Hkv * ((Lkv + tile.rows - 1) / tile.rows), (H / Hkv) * ((Lq + tile.cols - 1) / tile.cols), 2, 64);
 }
 static bool cross_extents_fine(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D) {
   return B >= 0 && H >= 0 && Hkv >= 0 && Lq >= 0 && Lkv >= 0 && D >= 1 && D <= 256 && (Hkv == 0 ? H == 0 : H % Hkv == 0) && B <= 65535 &&

@@ -11,86 +11,119 @@ namespace vsa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kFwdLarge = 148, kDqLarge = 74, kDkdvLarge = 148;
 
 template <typename T> __device__ __forceinline__ float to_f(T x) { return Elem<T>::to(x); }
 template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
 template <typename T> __device__ __forceinline__ T from_f(float x) { return Elem<T>::from(x); }
 template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
 
-// DP: head dim rounded up; KT: tile edge; P: patch edge
-template <int DP_, int KT_ = (DP_ > 128 ? 32 : 64)>
+// DP: head dim rounded up; RT, CT: rows and columns of a tile of scores, PI x PJ of them a thread; OVER: the scores go over a tile of
+// operands that has been read
+template <int DP_, int RT_, int CT_ = RT_, bool OVER_ = false>
 struct Tile {
-  static constexpr int DP = DP_, KT = KT_, P = KT / 16, PITCH = DP_ + 4, SPITCH = KT + 4;
-  static constexpr int floats = KT * PITCH, score_floats = KT * SPITCH;
+  static constexpr int DP = DP_, RT = RT_, CT = CT_, PI = RT / 16, PJ = CT / 16, PITCH = DP_ + 4, SPITCH = CT + 4;
+  static constexpr int row_floats = RT * PITCH, col_floats = CT * PITCH, score_floats = RT * SPITCH;
+  static constexpr bool OVER = OVER_;
 };
 
-// Rows row0 .. of one (batch, head) slice, converted; rows from `rows` on, rows that `live` says no to and dims from D on are zeros.
-template <typename T, typename TL, typename LIVE>
+// 16 bytes global -> shared past the registers, zeros where `there` is false (src is then not read)
+__device__ __forceinline__ void copy16(float* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// ROWS rows of one (batch, head) slice, converted, as one group of copies; rows that `live` says no to and dims from D on are zeros.
+template <typename T, typename TL, int ROWS, typename LIVE>
 __device__ __forceinline__ void load_tile(float* sm, const T* __restrict__ g, long long stride, int D, bool vec, LIVE live) {
-  constexpr int C = TL::DP / 4;
-  for (int e = threadIdx.x; e < TL::KT * C; e += kThreads) {
-    const int r = e / C, c = (e % C) * 4;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live(r) && c < D) {
-      const T* p = g + r * stride + c;
-      if (sizeof(T) == 4 && vec) {
-        x = *reinterpret_cast<const float4*>(p);
-      } else {
-        x.x = to_f<T>(p[0]);
-        if (c + 1 < D) x.y = to_f<T>(p[1]);
-        if (c + 2 < D) x.z = to_f<T>(p[2]);
-        if (c + 3 < D) x.w = to_f<T>(p[3]);
+  constexpr int C = TL::DP / 4, N = ROWS * C / kThreads;
+  static_assert(ROWS * C % kThreads == 0, "whole pieces a thread");
+  if (sizeof(T) == 4 && vec) {
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+      const int e = threadIdx.x + i * kThreads, r = e / C, c = (e % C) * 4;
+      const bool there = live(r) && c < D;
+      copy16(sm + r * TL::PITCH + c, there ? g + r * stride + c : g, there);
+    }
+  } else {
+    constexpr int U = N % 4 == 0 ? 4 : 2;        // pieces whose loads fly together
+    static_assert(N % U == 0, "whole batches of pieces");
+#pragma unroll 1
+    for (int i = 0; i < N; i += U) {
+      float4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = threadIdx.x + (i + u) * kThreads, r = e / C, c = (e % C) * 4;
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (live(r) && c < D) {
+          const T* p = g + r * stride + c;
+          x[u].x = to_f<T>(p[0]);
+          if (c + 1 < D) x[u].y = to_f<T>(p[1]);
+          if (c + 2 < D) x[u].z = to_f<T>(p[2]);
+          if (c + 3 < D) x[u].w = to_f<T>(p[3]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = threadIdx.x + (i + u) * kThreads;
+        *reinterpret_cast<float4*>(sm + e / C * TL::PITCH + (e % C) * 4) = x[u];
       }
     }
-    *reinterpret_cast<float4*>(sm + r * TL::PITCH + c) = x;
   }
+  copies_commit();
 }
 
-// s[i][j] = a[P ty + i] . b[tx + 16 j], in pieces of 16 products (a chain of 16 + D/16 roundings instead of D)
+// s[i][j] = a[PI ty + i] . b[tx + 16 j].  Small patches in pieces of 16 products (a chain of 16 + D/16 roundings instead of D); a patch of
+// 8 x 8 has no registers for the pieces' sums.
 template <typename TL>
-__device__ __forceinline__ void scores(float (&s)[TL::P][TL::P], const float* a, const float* b, int tx, int ty) {
+__device__ __forceinline__ void scores(float (&s)[TL::PI][TL::PJ], const float* a, const float* b, int tx, int ty) {
+  constexpr bool pieces = TL::PI * TL::PJ < 64;
 #pragma unroll
-  for (int i = 0; i < TL::P; ++i)
+  for (int i = 0; i < TL::PI; ++i)
 #pragma unroll
-    for (int j = 0; j < TL::P; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < TL::PJ; ++j) s[i][j] = 0.f;
 #pragma unroll 1
   for (int d0 = 0; d0 < TL::DP; d0 += 16) {
-    float t[TL::P][TL::P] = {};
+    float t[TL::PI][TL::PJ];
+#pragma unroll
+    for (int i = 0; i < TL::PI; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::PJ; ++j) t[i][j] = pieces ? 0.f : s[i][j];
 #pragma unroll
     for (int d = d0; d < d0 + 16; d += 4) {
-      float4 x[TL::P], y[TL::P];
+      float4 y[TL::PJ];
 #pragma unroll
-      for (int i = 0; i < TL::P; ++i) x[i] = *reinterpret_cast<const float4*>(a + (TL::P * ty + i) * TL::PITCH + d);
+      for (int j = 0; j < TL::PJ; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * TL::PITCH + d);
 #pragma unroll
-      for (int j = 0; j < TL::P; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * TL::PITCH + d);
+      for (int i = 0; i < TL::PI; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(a + (TL::PI * ty + i) * TL::PITCH + d);
 #pragma unroll
-      for (int i = 0; i < TL::P; ++i)
-#pragma unroll
-        for (int j = 0; j < TL::P; ++j)
-          t[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, t[i][j]))));
+        for (int j = 0; j < TL::PJ; ++j) t[i][j] = fmaf(x.w, y[j].w, fmaf(x.z, y[j].z, fmaf(x.y, y[j].y, fmaf(x.x, y[j].x, t[i][j]))));
+      }
     }
 #pragma unroll
-    for (int i = 0; i < TL::P; ++i)
+    for (int i = 0; i < TL::PI; ++i)
 #pragma unroll
-      for (int j = 0; j < TL::P; ++j) s[i][j] += t[i][j];
+      for (int j = 0; j < TL::PJ; ++j) s[i][j] = pieces ? s[i][j] + t[i][j] : t[i][j];
   }
 }
 
-// acc[i][4 h + e] += sum_n p[P ty + i][n] * b[n][64 h + 4 tx + e]
+// acc[i][4 h + e] += sum_n p[PI ty + i][n] * b[n][64 h + 4 tx + e]
 template <typename TL>
-__device__ __forceinline__ void product(float (&acc)[TL::P][TL::DP / 16], const float* p, const float* b, int tx, int ty) {
+__device__ __forceinline__ void product(float (&acc)[TL::PI][TL::DP / 16], const float* p, const float* b, int tx, int ty) {
 #pragma unroll 2
-  for (int n = 0; n < TL::KT; n += 4) {
-    float4 w[TL::P];
+  for (int n = 0; n < TL::CT; n += 4) {
+    float4 w[TL::PI];
 #pragma unroll
-    for (int i = 0; i < TL::P; ++i) w[i] = *reinterpret_cast<const float4*>(p + (TL::P * ty + i) * TL::SPITCH + n);
+    for (int i = 0; i < TL::PI; ++i) w[i] = *reinterpret_cast<const float4*>(p + (TL::PI * ty + i) * TL::SPITCH + n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
 #pragma unroll
       for (int h = 0; h < TL::DP / 64; ++h) {
         const float4 x = *reinterpret_cast<const float4*>(b + (n + e) * TL::PITCH + 64 * h + 4 * tx);
 #pragma unroll
-        for (int i = 0; i < TL::P; ++i) {
+        for (int i = 0; i < TL::PI; ++i) {
           const float f = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
           acc[i][4 * h + 0] = fmaf(f, x.x, acc[i][4 * h + 0]);
           acc[i][4 * h + 1] = fmaf(f, x.y, acc[i][4 * h + 1]);
@@ -103,11 +136,11 @@ __device__ __forceinline__ void product(float (&acc)[TL::P][TL::DP / 16], const 
 }
 
 template <typename T, typename TL>
-__device__ __forceinline__ void store_rows(T* __restrict__ g, long long stride, int D, int rows, const float (&acc)[TL::P][TL::DP / 16],
-                                           const float (&mul)[TL::P], int tx, int ty) {
+__device__ __forceinline__ void store_rows(T* __restrict__ g, long long stride, int D, int rows, const float (&acc)[TL::PI][TL::DP / 16],
+                                           const float (&mul)[TL::PI], int tx, int ty) {
 #pragma unroll
-  for (int i = 0; i < TL::P; ++i) {
-    const int r = TL::P * ty + i;
+  for (int i = 0; i < TL::PI; ++i) {
+    const int r = TL::PI * ty + i;
     if (r >= rows) continue;
 #pragma unroll
     for (int h = 0; h < TL::DP / 64; ++h)
@@ -154,61 +187,65 @@ template <typename T, typename TL>
 __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __grid_constant__ VsaCross a, int splits, float* part_out, float* part_lse,
                                                                      bool vec) {
   extern __shared__ __align__(16) float sm[];
-  float *sq = sm, *sk = sq + TL::floats, *sv = sk + TL::floats, *ss = sv + TL::floats;
+  float *sq = sm, *sk = sq + TL::row_floats, *sv = sk + TL::col_floats, *ss = TL::OVER ? sk : sv + TL::col_floats;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int split = blockIdx.x % splits, qt = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
-  const int row0 = qt * TL::KT, rows = (int)min((long long)TL::KT, (long long)a.Lq - row0);
+  const int row0 = qt * TL::RT, rows = (int)min((long long)TL::RT, (long long)a.Lq - row0);
   const Ctx keys = keys_of(a, b);
-  const int tiles = (keys.len + TL::KT - 1) / TL::KT, per = (tiles + splits - 1) / splits;
+  const int tiles = (keys.len + TL::CT - 1) / TL::CT, per = (tiles + splits - 1) / splits;
   const int t0 = split * per, t1 = min(tiles, t0 + per);
   const float c = a.scale * kLog2e;
-  load_tile<T, TL>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, [&](int r) { return r < rows; });
-  float m[TL::P], l[TL::P], acc[TL::P][TL::DP / 16];
+  load_tile<T, TL, TL::RT>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, [&](int r) { return r < rows; });
+  float m[TL::PI], l[TL::PI], acc[TL::PI][TL::DP / 16];
 #pragma unroll
-  for (int i = 0; i < TL::P; ++i) {
+  for (int i = 0; i < TL::PI; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
     for (int d = 0; d < TL::DP / 16; ++d) acc[i][d] = 0.f;
   }
   for (int t = t0; t < t1; ++t) {
-    const int k0 = t * TL::KT;
+    const int k0 = t * TL::CT;
     __syncthreads();
     auto live = [&](int r) { return keys.live(k0 + r); };
-    load_tile<T, TL>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
-    load_tile<T, TL>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+    load_tile<T, TL, TL::CT>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
+    load_tile<T, TL, TL::CT>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+    copies_wait<1>();                              // Q and K; V may be on its way
     __syncthreads();
-    float s[TL::P][TL::P];
+    float s[TL::PI][TL::PJ];
     scores<TL>(s, sq, sk, tx, ty);
-    bool on[TL::P];
+    if (TL::OVER) __syncthreads();
+    bool on[TL::PJ];
 #pragma unroll
-    for (int j = 0; j < TL::P; ++j) on[j] = live(tx + 16 * j);
+    for (int j = 0; j < TL::PJ; ++j) on[j] = live(tx + 16 * j);
 #pragma unroll
-    for (int i = 0; i < TL::P; ++i) {
+    for (int i = 0; i < TL::PI; ++i) {
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < TL::P; ++j)
+      for (int j = 0; j < TL::PJ; ++j)
         if (on[j]) top = fmaxf(top, s[i][j] * c);
       const float mn = fmaxf(m[i], lanes16_max(top)), shift = mn == -INFINITY ? 0.f : mn;
       const float keep = exp2f(m[i] - shift);
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < TL::P; ++j) {
+      for (int j = 0; j < TL::PJ; ++j) {
         const float p = on[j] ? exp2f(fmaf(s[i][j], c, -shift)) : 0.f;
         sum += p;
-        ss[(TL::P * ty + i) * TL::SPITCH + tx + 16 * j] = p;
+        ss[(TL::PI * ty + i) * TL::SPITCH + tx + 16 * j] = p;
       }
       l[i] = l[i] * keep + lanes16_sum(sum);
       m[i] = mn;
 #pragma unroll
       for (int d = 0; d < TL::DP / 16; ++d) acc[i][d] *= keep;
     }
+    copies_wait<0>();
     __syncthreads();
     product<TL>(acc, ss, sv, tx, ty);
   }
-  float mul[TL::P];
+  copies_wait<0>();
+  float mul[TL::PI];
 #pragma unroll
-  for (int i = 0; i < TL::P; ++i) mul[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+  for (int i = 0; i < TL::PI; ++i) mul[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
   const long long bh = (long long)b * a.H + h, lp = cross_rows(a.Lq);
   if (splits == 1) {
     store_rows<T, TL>(slice<T>(a.out, a.out_stride, b, h) + row0 * a.out_stride[2], a.out_stride[2], a.D, rows, acc, mul, tx, ty);
@@ -218,8 +255,8 @@ __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __gri
   }
   if (tx == 0) {
 #pragma unroll
-    for (int i = 0; i < TL::P; ++i) {
-      const int r = TL::P * ty + i;
+    for (int i = 0; i < TL::PI; ++i) {
+      const int r = TL::PI * ty + i;
       const float lse = l[i] == 0.f ? (splits == 1 ? INFINITY : -INFINITY) : m[i] + log2f(l[i]);
       if (splits > 1) {
         if (r < rows) part_lse[(split * (long long)a.B * a.H + bh) * a.Lq + row0 + r] = lse;
@@ -228,31 +265,33 @@ __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __gri
       }
     }
   }
-  if (splits == 1 && row0 + TL::KT >= a.Lq)
-    for (long long r = row0 + TL::KT + tid; r < lp; r += kThreads) a.lse2[bh * lp + r] = INFINITY;
+  if (splits == 1 && row0 + TL::RT >= a.Lq)
+    for (long long r = row0 + TL::RT + tid; r < lp; r += kThreads) a.lse2[bh * lp + r] = INFINITY;
 }
 
 // ---- backward: dQ (and delta) of one tile of query rows -----------------------------------------------------------
 template <typename T, typename TL>
 __global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid_constant__ VsaCross a, bool vec) {
   extern __shared__ __align__(16) float sm[];
-  float *sq = sm, *sdo = sq + TL::floats, *sk = sdo + TL::floats, *sv = sk + TL::floats, *ss = sv + TL::floats;
+  float *sq = sm, *sdo = sq + TL::row_floats, *sk = sdo + TL::row_floats, *sv = sk + TL::col_floats, *ss = TL::OVER ? sv : sv + TL::col_floats;
+  static_assert(TL::RT <= 2 * TL::CT, "the rows of out pass through the tiles of K and V");
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int qt = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
-  const int row0 = qt * TL::KT, rows = (int)min((long long)TL::KT, (long long)a.Lq - row0);
+  const int row0 = qt * TL::RT, rows = (int)min((long long)TL::RT, (long long)a.Lq - row0);
   const Ctx keys = keys_of(a, b);
-  const int tiles = (keys.len + TL::KT - 1) / TL::KT;
+  const int tiles = (keys.len + TL::CT - 1) / TL::CT;
   const float c = a.scale * kLog2e;
   const long long bh = (long long)b * a.H + h, lp = cross_rows(a.Lq);
   auto there = [&](int r) { return r < rows; };
-  load_tile<T, TL>(sk, slice<T>((const void*)a.out, a.out_stride, b, h) + row0 * a.out_stride[2], a.out_stride[2], a.D, vec, there);
-  load_tile<T, TL>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, there);
-  load_tile<T, TL>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
+  load_tile<T, TL, TL::RT>(sk, slice<T>((const void*)a.out, a.out_stride, b, h) + row0 * a.out_stride[2], a.out_stride[2], a.D, vec, there);
+  load_tile<T, TL, TL::RT>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, there);
+  load_tile<T, TL, TL::RT>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
+  copies_wait<0>();
   __syncthreads();
-  float lse[TL::P], delta[TL::P], acc[TL::P][TL::DP / 16], mul[TL::P];
+  float lse[TL::PI], delta[TL::PI], acc[TL::PI][TL::DP / 16], mul[TL::PI];
 #pragma unroll
-  for (int i = 0; i < TL::P; ++i) {
-    const int r = TL::P * ty + i;
+  for (int i = 0; i < TL::PI; ++i) {
+    const int r = TL::PI * ty + i;
     float d = 0.f;
     for (int e = tx; e < TL::DP; e += 16) d = fmaf(sk[r * TL::PITCH + e], sdo[r * TL::PITCH + e], d);
     delta[i] = lanes16_sum(d);
@@ -263,27 +302,31 @@ __global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid
     for (int e = 0; e < TL::DP / 16; ++e) acc[i][e] = 0.f;
   }
   for (int t = 0; t < tiles; ++t) {
-    const int k0 = t * TL::KT;
+    const int k0 = t * TL::CT;
     __syncthreads();
     auto live = [&](int r) { return keys.live(k0 + r); };
-    load_tile<T, TL>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
-    load_tile<T, TL>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+    load_tile<T, TL, TL::CT>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
+    load_tile<T, TL, TL::CT>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+    copies_wait<1>();                              // K; V may be on its way
     __syncthreads();
-    float s[TL::P][TL::P], dp[TL::P][TL::P];
+    float s[TL::PI][TL::PJ], dp[TL::PI][TL::PJ];
     scores<TL>(s, sq, sk, tx, ty);
+    copies_wait<0>();
+    __syncthreads();
     scores<TL>(dp, sdo, sv, tx, ty);
+    if (TL::OVER) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < TL::P; ++j) {
+    for (int j = 0; j < TL::PJ; ++j) {
       const bool on = live(tx + 16 * j);
 #pragma unroll
-      for (int i = 0; i < TL::P; ++i)
-        ss[(TL::P * ty + i) * TL::SPITCH + tx + 16 * j] = on ? exp2f(fmaf(s[i][j], c, -lse[i])) * (dp[i][j] - delta[i]) : 0.f;
+      for (int i = 0; i < TL::PI; ++i)
+        ss[(TL::PI * ty + i) * TL::SPITCH + tx + 16 * j] = on ? exp2f(fmaf(s[i][j], c, -lse[i])) * (dp[i][j] - delta[i]) : 0.f;
     }
     __syncthreads();
     product<TL>(acc, ss, sk, tx, ty);
   }
-  if (row0 + TL::KT >= a.Lq)
-    for (long long r = row0 + TL::KT + tid; r < lp; r += kThreads) a.delta[bh * lp + r] = 0.f;
+  if (row0 + TL::RT >= a.Lq)
+    for (long long r = row0 + TL::RT + tid; r < lp; r += kThreads) a.delta[bh * lp + r] = 0.f;
   store_rows<T, TL>(slice<T>(a.dq, a.dq_stride, b, h) + row0 * a.dq_stride[2], a.dq_stride[2], a.D, rows, acc, mul, tx, ty);
 }
 
@@ -291,55 +334,73 @@ __global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid
 template <typename T, typename TL>
 __global__ void __launch_bounds__(kThreads) cross_dkdv_generic_kernel(const __grid_constant__ VsaCross a, int splits, float* part, bool vec) {
   extern __shared__ __align__(16) float sm[];
-  float *sk = sm, *sv = sk + TL::floats, *sq = sv + TL::floats, *sdo = sq + TL::floats, *sp = sdo + TL::floats, *sds = sp + TL::score_floats;
+  float *sk = sm, *sv = sk + TL::row_floats, *sq = sv + TL::row_floats, *sdo = sq + TL::col_floats, *sp = sdo + TL::col_floats;
+  float* sds = TL::OVER ? sp : sp + TL::score_floats;      // dS after P, or beside it
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int split = blockIdx.x % splits, kt = blockIdx.x / splits, hk = blockIdx.y, b = blockIdx.z, group = (int)(a.H / a.Hkv);
-  const int k0 = kt * TL::KT, krows = (int)min((long long)TL::KT, (long long)a.Lkv - k0);
+  const int k0 = kt * TL::RT, krows = (int)min((long long)TL::RT, (long long)a.Lkv - k0);
   const Ctx keys = keys_of(a, b);
   const float c = a.scale * kLog2e;
   auto live = [&](int r) { return keys.live(k0 + r); };
-  load_tile<T, TL>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
-  load_tile<T, TL>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
-  float dk[TL::P][TL::DP / 16], dv[TL::P][TL::DP / 16], mul_k[TL::P], mul_v[TL::P];
+  load_tile<T, TL, TL::RT>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
+  load_tile<T, TL, TL::RT>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
+  float dk[TL::PI][TL::DP / 16], dv[TL::PI][TL::DP / 16], mul_k[TL::PI], mul_v[TL::PI];
 #pragma unroll
-  for (int i = 0; i < TL::P; ++i) {
-    const bool on = live(TL::P * ty + i);
+  for (int i = 0; i < TL::PI; ++i) {
+    const bool on = live(TL::PI * ty + i);
     mul_k[i] = on ? a.scale : 0.f;
     mul_v[i] = on ? 1.f : 0.f;
 #pragma unroll
     for (int e = 0; e < TL::DP / 16; ++e) dk[i][e] = dv[i][e] = 0.f;
   }
-  const int qtiles = (int)((a.Lq + TL::KT - 1) / TL::KT);
+  const int qtiles = (int)((a.Lq + TL::CT - 1) / TL::CT);
   const long long total = (long long)qtiles * group, per = (total + splits - 1) / splits;
   const long long t1 = k0 < keys.len ? min(total, (split + 1) * per) : 0, lp = cross_rows(a.Lq);
   for (long long t = split * per; t < t1; ++t) {
-    const int h = hk * group + (int)(t / qtiles), row0 = (int)(t % qtiles) * TL::KT;
-    const int rows = (int)min((long long)TL::KT, (long long)a.Lq - row0);
+    const int h = hk * group + (int)(t / qtiles), row0 = (int)(t % qtiles) * TL::CT;
+    const int rows = (int)min((long long)TL::CT, (long long)a.Lq - row0);
     const long long stat = ((long long)b * a.H + h) * lp + row0;
     auto there = [&](int r) { return r < rows; };
     __syncthreads();
-    load_tile<T, TL>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, there);
-    load_tile<T, TL>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
+    load_tile<T, TL, TL::CT>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, there);
+    load_tile<T, TL, TL::CT>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
+    float lse[TL::PJ], delta[TL::PJ];
+#pragma unroll
+    for (int j = 0; j < TL::PJ; ++j) {
+      const int r = tx + 16 * j;
+      lse[j] = there(r) ? a.lse2[stat + r] : INFINITY;
+      delta[j] = there(r) ? a.delta[stat + r] : 0.f;
+    }
+    copies_wait<1>();                              // K, V and Q; dO may be on its way
     __syncthreads();
-    float s[TL::P][TL::P], dp[TL::P][TL::P];
+    float s[TL::PI][TL::PJ], dp[TL::PI][TL::PJ];
     scores<TL>(s, sk, sq, tx, ty);
+    copies_wait<0>();
+    __syncthreads();
     scores<TL>(dp, sv, sdo, tx, ty);
 #pragma unroll
-    for (int j = 0; j < TL::P; ++j) {
-      const int r = tx + 16 * j;
-      const float lse = there(r) ? a.lse2[stat + r] : INFINITY, delta = there(r) ? a.delta[stat + r] : 0.f;
+    for (int j = 0; j < TL::PJ; ++j)
 #pragma unroll
-      for (int i = 0; i < TL::P; ++i) {
-        const int at = (TL::P * ty + i) * TL::SPITCH + r;
-        const float p = exp2f(fmaf(s[i][j], c, -lse));
+      for (int i = 0; i < TL::PI; ++i) {
+        const int at = (TL::PI * ty + i) * TL::SPITCH + tx + 16 * j;
+        const float p = exp2f(fmaf(s[i][j], c, -lse[j]));
         sp[at] = p;
-        sds[at] = p * (dp[i][j] - delta);
+        s[i][j] = p * (dp[i][j] - delta[j]);
+        if (!TL::OVER) sds[at] = s[i][j];
       }
-    }
     __syncthreads();
     product<TL>(dv, sp, sdo, tx, ty);
+    if (TL::OVER) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < TL::PJ; ++j)
+#pragma unroll
+        for (int i = 0; i < TL::PI; ++i) sds[(TL::PI * ty + i) * TL::SPITCH + tx + 16 * j] = s[i][j];
+      __syncthreads();
+    }
     product<TL>(dk, sds, sq, tx, ty);
   }
+  copies_wait<0>();
   if (splits == 1) {
     store_rows<T, TL>(slice<T>(a.dk, a.dk_stride, b, hk) + k0 * a.dk_stride[2], a.dk_stride[2], a.D, krows, dk, mul_k, tx, ty);
     store_rows<T, TL>(slice<T>(a.dv, a.dv_stride, b, hk) + k0 * a.dv_stride[2], a.dv_stride[2], a.D, krows, dv, mul_v, tx, ty);
@@ -515,48 +576,80 @@ int reserve(Kern kern, int bytes, const char* what) {
 
 template <typename T, typename TL>
 int fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
-  const int bytes = (3 * TL::floats + TL::score_floats) * 4;
+  const int bytes = (TL::row_floats + 2 * TL::col_floats + (TL::OVER ? 0 : TL::score_floats)) * 4;
+  static_assert(!TL::OVER || TL::score_floats <= TL::col_floats, "P goes over K");
   int rc = reserve(cross_fwd_generic_kernel<T, TL>, bytes, "cross attention forward");
   if (rc) return rc;
-  const int64_t tiles = (a.Lq + TL::KT - 1) / TL::KT;
+  const int64_t tiles = (a.Lq + TL::RT - 1) / TL::RT;
   cross_fwd_generic_kernel<T, TL><<<dim3((unsigned)(tiles * splits), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
       a, splits, part_out, part_lse, vec4(a, false));
   return check_launch("cross_fwd_generic_kernel");
 }
 template <typename T, typename TL>
 int dq_pass(const VsaCross& a, cudaStream_t st) {
-  const int bytes = (4 * TL::floats + TL::score_floats) * 4;
+  constexpr int last = TL::OVER ? (TL::score_floats > TL::col_floats ? TL::score_floats : TL::col_floats) : TL::col_floats + TL::score_floats;
+  const int bytes = (2 * TL::row_floats + TL::col_floats + last) * 4;
   const int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
   if (rc) return rc;
-  cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::KT - 1) / TL::KT), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
+  cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::RT - 1) / TL::RT), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
       a, vec4(a, true));
   return check_launch("cross_dq_generic_kernel");
 }
 template <typename T, typename TL>
-int bwd(const VsaCross& a, int splits, float* part, cudaStream_t st) {
-  // dQ on tiles of 32 x 32 where tiles of 64 leave SMs without work ([1, 2, 1025, 64] x 333: 34 CTAs, 67 us; 66 CTAs, 58)
-  using Small = Tile<TL::DP, 32>;
-  int rc = TL::KT == 64 && a.B * a.H * ((a.Lq + 63) / 64) < 148 ? dq_pass<T, Small>(a, st) : dq_pass<T, TL>(a, st);
-  if (rc || a.Lkv == 0 || a.dk == nullptr) return rc;
-  const int bytes = (4 * TL::floats + 2 * TL::score_floats) * 4;
-  if ((rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV"))) return rc;
-  cross_dkdv_generic_kernel<T, TL><<<dim3((unsigned)((a.Lkv + TL::KT - 1) / TL::KT * splits), (unsigned)a.Hkv, (unsigned)a.B), kThreads, bytes,
+int dkdv_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  const int bytes = (2 * TL::row_floats + 2 * TL::col_floats + (TL::OVER ? 1 : 2) * TL::score_floats) * 4;
+  const int rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV");
+  if (rc) return rc;
+  cross_dkdv_generic_kernel<T, TL><<<dim3((unsigned)((a.Lkv + TL::RT - 1) / TL::RT * splits), (unsigned)a.Hkv, (unsigned)a.B), kThreads, bytes,
                                      st>>>(a, splits, part, vec4(a, true));
   return check_launch("cross_dkdv_generic_kernel");
 }
 
+template <typename T>
+int fwd_by_dim(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
+  const bool large = cross_generic_fwd_tile(a.B, a.H, a.Lq, a.Lkv, a.D).large;
+  if (a.D <= 64) return large ? fwd<T, Tile<64, 128>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<64, 64>>(a, splits, part_out, part_lse, st);
+  if (a.D <= 128)
+    return large ? fwd<T, Tile<128, 128, 128, true>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<128, 64>>(a, splits, part_out, part_lse, st);
+  return large ? fwd<T, Tile<256, 64>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<256, 32>>(a, splits, part_out, part_lse, st);
+}
+template <typename T>
+int bwd_by_dim(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  // dQ has no cut over the keys: its tiles shrink with the rows that there are
+  const int64_t heads = a.B * a.H, edge = a.D <= 128 ? 128 : 64;
+  const bool most = heads * ((a.Lq + edge - 1) / edge) >= kDqLarge, few = heads * ((a.Lq + 63) / 64) < 148;
+  int rc;
+  if (a.D <= 64) rc = most ? dq_pass<T, Tile<64, 128>>(a, st) : few ? dq_pass<T, Tile<64, 32>>(a, st) : dq_pass<T, Tile<64, 64>>(a, st);
+  else if (a.D <= 128) rc = most ? dq_pass<T, Tile<128, 128, 64, true>>(a, st) : few ? dq_pass<T, Tile<128, 32>>(a, st) : dq_pass<T, Tile<128, 64>>(a, st);
+  else rc = most ? dq_pass<T, Tile<256, 64, 32>>(a, st) : dq_pass<T, Tile<256, 32>>(a, st);
+  if (rc || a.Lkv == 0 || a.dk == nullptr) return rc;
+  const bool large = cross_generic_bwd_tile(a.B, a.H, a.Hkv, a.Lq, a.Lkv, a.D).large;
+  if (a.D <= 64) return large ? dkdv_pass<T, Tile<64, 128, 128, true>>(a, splits, part, st) : dkdv_pass<T, Tile<64, 64>>(a, splits, part, st);
+  if (a.D <= 128) return large ? dkdv_pass<T, Tile<128, 96, 64, true>>(a, splits, part, st) : dkdv_pass<T, Tile<128, 64>>(a, splits, part, st);
+  return large ? dkdv_pass<T, Tile<256, 64, 32, true>>(a, splits, part, st) : dkdv_pass<T, Tile<256, 32>>(a, splits, part, st);
+}
+
 }  // namespace
 
-#define VSA_CROSS_BY_DIM(T_, call_) (a.D <= 64 ? call_<T_, Tile<64>> : a.D <= 128 ? call_<T_, Tile<128>> : call_<T_, Tile<256>>)
-#define VSA_CROSS_BY_TYPE(call_) \
-  (a.dtype == VSA_F32 ? VSA_CROSS_BY_DIM(float, call_) : a.dtype == VSA_F16 ? VSA_CROSS_BY_DIM(__half, call_) : VSA_CROSS_BY_DIM(__nv_bfloat16, call_))
-
-int cross_generic_tile(int D) { return D > 128 ? 32 : 64; }
+CrossTile cross_generic_fwd_tile(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D) {
+  const int edge = D <= 128 ? 128 : 64, small = D <= 128 ? 64 : 32;
+  if (B * H * ((Lq + edge - 1) / edge) * ((Lkv + edge - 1) / edge) >= kFwdLarge) return {edge, edge, true};
+  return {small, small, false};
+}
+CrossTile cross_generic_bwd_tile(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D) {
+  const int rows = D <= 64 ? 128 : D <= 128 ? 96 : 64, cols = D <= 64 ? 128 : D <= 128 ? 64 : 32, small = D <= 128 ? 64 : 32;
+  if (B * H * ((Lq + cols - 1) / cols) * ((Lkv + rows - 1) / rows) >= kDkdvLarge) return {rows, cols, true};
+  return {small, small, false};
+}
 
 int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
-  return VSA_CROSS_BY_TYPE(fwd)(a, splits, part_out, part_lse, st);
+  if (a.dtype == VSA_F32) return fwd_by_dim<float>(a, splits, part_out, part_lse, st);
+  return a.dtype == VSA_F16 ? fwd_by_dim<__half>(a, splits, part_out, part_lse, st) : fwd_by_dim<__nv_bfloat16>(a, splits, part_out, part_lse, st);
 }
-int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st) { return VSA_CROSS_BY_TYPE(bwd)(a, splits, part, st); }
+int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st) {
+  if (a.dtype == VSA_F32) return bwd_by_dim<float>(a, splits, part, st);
+  return a.dtype == VSA_F16 ? bwd_by_dim<__half>(a, splits, part, st) : bwd_by_dim<__nv_bfloat16>(a, splits, part, st);
+}
 
 int cross_join(const VsaCross& a, int splits, const float* part_out, const float* part_lse, cudaStream_t st) {
   const unsigned blocks = (unsigned)((a.B * a.H * a.Lq + 7) / 8);

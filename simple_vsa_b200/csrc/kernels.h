@@ -74,7 +74,12 @@ __device__ __forceinline__ int cross_length(const VsaCross& a, int b) {
   return n < 0 ? 0 : n > a.Lkv ? (int)a.Lkv : n;
 }
 #endif
-int cross_generic_tile(int D);
+struct CrossTile {
+  int rows, cols;      // query rows and keys of the forward, keys and query rows of dK/dV
+  bool large;
+};
+CrossTile cross_generic_fwd_tile(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D);
+CrossTile cross_generic_bwd_tile(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D);
 // tensor path (cross_umma.cu), lengths only (key_bits is not looked at): by head dim and type; with pointers and strides
 bool cross_umma_shape(int D, int dtype);
 bool cross_aligned(const VsaCross& a, bool backward);
