@@ -665,6 +665,12 @@ static int cross_bwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64
   const CrossTile tile = cross_generic_bwd_tile(B, H, Hkv, Lq, Lkv, D);
   return cross_parts(B * Hkv * ((Lkv + tile.rows - 1) / tile.rows), (H / Hkv) * ((Lq + tile.cols - 1) / tile.cols), 2, 64);
 }
+// The CUDA-core kernels' dQ over ranges of the keys (a cut costs a launch and a pass over the parts).
+static int cross_dq_splits(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  if (cross_umma_shape(D, dtype)) return 1;
+  const CrossTile tile = cross_generic_dq_tile(B, H, Lq, D);
+  return tile.large ? 1 : cross_parts(B * H * ((Lq + tile.rows - 1) / tile.rows), (Lkv + tile.cols - 1) / tile.cols, 2, 16);
+}
 static bool cross_extents_fine(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D) {
   return B >= 0 && H >= 0 && Hkv >= 0 && Lq >= 0 && Lkv >= 0 && D >= 1 && D <= 256 && (Hkv == 0 ? H == 0 : H % Hkv == 0) && B <= 65535 &&
          H <= 65535 && Lq <= 0x3fffffff && Lkv <= 0x3fffffff;
@@ -674,16 +680,19 @@ int64_t vsa_cross_words(int64_t Lkv) { return Lkv < 0 ? -1 : cross_words(Lkv); }
 
 // The workspace: partial results, then what a compaction of the keys needs (16-bit types with a mask).
 struct CrossSpace {
-  int splits;
+  int splits, dq_splits;
   int64_t parts, prefix, counts, k, v, bytes;      // byte offsets behind the partial results, which begin at 0
 };
 static CrossSpace cross_space(bool backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype, bool mask) {
-  CrossSpace s{1, 0, 0, 0, 0, 0, 0};
+  CrossSpace s{1, 1, 0, 0, 0, 0, 0, 0};
   if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return s;
   const bool compact = mask && cross_umma_shape(D, dtype) && (backward || !cross_few_rows(H, Hkv, Lq, D, dtype));
   s.splits = backward ? cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype) : cross_fwd_splits(B, H, Hkv, Lq, Lkv, D, dtype);
   if (!backward) s.parts = s.splits == 1 ? 0 : s.splits * B * H * Lq * (int64_t)(D + 1) * 4;
   else s.parts = s.splits == 1 && !compact ? 0 : s.splits * 2 * B * Hkv * Lkv * (int64_t)D * 4;
+  s.dq_splits = backward ? cross_dq_splits(B, H, Lq, Lkv, D, dtype) : 1;
+  const int64_t dq_parts = s.dq_splits == 1 ? 0 : s.dq_splits * B * H * Lq * (int64_t)D * 4;      // before dK/dV, in the same place
+  if (dq_parts > s.parts) s.parts = dq_parts;
   s.parts = (s.parts + 15) / 16 * 16;
   s.prefix = s.parts;
   s.counts = s.prefix + (compact ? B * cross_words(Lkv) * 4 : 0);
@@ -775,7 +784,7 @@ int vsa_cross_bwd(const VsaCross* a, void* stream) {
   float* part = (float*)a->workspace;
   if (!cross_on_umma(*a, true) || a->key_bits == nullptr) {
     const bool parts = s.splits > 1;
-    rc = cross_on_umma(*a, true) ? cross_bwd_umma(*a, s.splits, parts, part, st) : cross_bwd_generic(*a, s.splits, part, st);
+    rc = cross_on_umma(*a, true) ? cross_bwd_umma(*a, s.splits, parts, part, st) : cross_bwd_generic(*a, s.splits, s.dq_splits, part, st);
     return rc || !parts || !keys ? rc : cross_sum(*a, s.splits, part, st);
   }
   VsaCross c;

@@ -2,8 +2,12 @@
 // cross attention share: the packed key mask, the join of a forward split over the keys, the sum of partial dK and dV.
 //
 // out_i = sum_j p_ij v_j with p_i the softmax of scale q_i.k_j over the live keys j of the sample; a row without one gets zeros.
-// Tiles of 64 query rows x 64 keys (32 x 32 above head dim 128), 256 threads, a 4 x 4 patch of scores each, everything in fp32 and one
-// rounding at the end.  Bound by the FP32 pipe and by shared-memory reads (a 16-byte read feeds 8 to 16 multiply-adds).
+// Tiles of 128 query rows x 64 keys, 64 x 64 where there are few (64 x 64 and 32 x 32 above head dim 128; dK/dV up to 128 keys x 64 query
+// rows), 256 threads, a patch of 8 x 4 scores each, everything in fp32 and one rounding at the end.  Bound by the FP32 pipe and the
+// shared-memory reads that feed it (12 of 16 bytes for 128 multiply-adds in the scores, 16 for 256 in the products): at
+// [1, 12, 4096, 128] x 2048 the forward takes 1386 us (37 of 72 TFLOP/s; pipe 64 % busy, reads 50 %), the backward 4470 (its seven products at
+// 40).  8 x 8 scores a thread spill (1448 us); chains without pairs are slower in the backward (4954), two CTAs an SM at head dim 64
+// spill too (874 us for 830).  With few query rows a pass is cut over the keys, with few keys dK/dV is over the query rows.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -11,7 +15,6 @@ namespace vsa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kFwdLarge = 148, kDqLarge = 74, kDkdvLarge = 148;
 
 template <typename T> __device__ __forceinline__ float to_f(T x) { return Elem<T>::to(x); }
 template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
@@ -74,61 +77,54 @@ __device__ __forceinline__ void load_tile(float* sm, const T* __restrict__ g, lo
   copies_commit();
 }
 
-// s[i][j] = a[PI ty + i] . b[tx + 16 j].  Small patches in pieces of 16 products (a chain of 16 + D/16 roundings instead of D); a patch of
-// 8 x 8 has no registers for the pieces' sums.
+// s[i][j] = a[PI ty + i] . b[tx + 16 j], even and odd dims in two chains that one instruction advances
 template <typename TL>
 __device__ __forceinline__ void scores(float (&s)[TL::PI][TL::PJ], const float* a, const float* b, int tx, int ty) {
-  constexpr bool pieces = TL::PI * TL::PJ < 64;
+  float2 t[TL::PI][TL::PJ];
 #pragma unroll
   for (int i = 0; i < TL::PI; ++i)
 #pragma unroll
-    for (int j = 0; j < TL::PJ; ++j) s[i][j] = 0.f;
-#pragma unroll 1
-  for (int d0 = 0; d0 < TL::DP; d0 += 16) {
-    float t[TL::PI][TL::PJ];
+    for (int j = 0; j < TL::PJ; ++j) t[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
+  for (int d = 0; d < TL::DP; d += 4) {
+    float4 y[TL::PJ];
 #pragma unroll
-    for (int i = 0; i < TL::PI; ++i)
+    for (int j = 0; j < TL::PJ; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * TL::PITCH + d);
 #pragma unroll
-      for (int j = 0; j < TL::PJ; ++j) t[i][j] = pieces ? 0.f : s[i][j];
+    for (int i = 0; i < TL::PI; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(a + (TL::PI * ty + i) * TL::PITCH + d);
 #pragma unroll
-    for (int d = d0; d < d0 + 16; d += 4) {
-      float4 y[TL::PJ];
-#pragma unroll
-      for (int j = 0; j < TL::PJ; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * TL::PITCH + d);
-#pragma unroll
-      for (int i = 0; i < TL::PI; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(a + (TL::PI * ty + i) * TL::PITCH + d);
-#pragma unroll
-        for (int j = 0; j < TL::PJ; ++j) t[i][j] = fmaf(x.w, y[j].w, fmaf(x.z, y[j].z, fmaf(x.y, y[j].y, fmaf(x.x, y[j].x, t[i][j]))));
-      }
+      for (int j = 0; j < TL::PJ; ++j)
+        t[i][j] = fma2(make_float2(x.z, x.w), make_float2(y[j].z, y[j].w), fma2(make_float2(x.x, x.y), make_float2(y[j].x, y[j].y), t[i][j]));
     }
-#pragma unroll
-    for (int i = 0; i < TL::PI; ++i)
-#pragma unroll
-      for (int j = 0; j < TL::PJ; ++j) s[i][j] = pieces ? s[i][j] + t[i][j] : t[i][j];
   }
+#pragma unroll
+  for (int i = 0; i < TL::PI; ++i)
+#pragma unroll
+    for (int j = 0; j < TL::PJ; ++j) s[i][j] = t[i][j].x + t[i][j].y;
 }
 
-// acc[i][4 h + e] += sum_n p[PI ty + i][n] * b[n][64 h + 4 tx + e]
+// acc[i][2 h + f] += sum_n p[PI ty + i][n] * b[n][64 h + 4 tx + 2 f ..]
 template <typename TL>
-__device__ __forceinline__ void product(float (&acc)[TL::PI][TL::DP / 16], const float* p, const float* b, int tx, int ty) {
-#pragma unroll 2
+__device__ __forceinline__ void product(float2 (&acc)[TL::PI][TL::DP / 32], const float* p, const float* b, int tx, int ty) {
+#pragma unroll 1
   for (int n = 0; n < TL::CT; n += 4) {
     float4 w[TL::PI];
 #pragma unroll
     for (int i = 0; i < TL::PI; ++i) w[i] = *reinterpret_cast<const float4*>(p + (TL::PI * ty + i) * TL::SPITCH + n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
+      float4 x[TL::DP / 64];
 #pragma unroll
-      for (int h = 0; h < TL::DP / 64; ++h) {
-        const float4 x = *reinterpret_cast<const float4*>(b + (n + e) * TL::PITCH + 64 * h + 4 * tx);
+      for (int h = 0; h < TL::DP / 64; ++h) x[h] = *reinterpret_cast<const float4*>(b + (n + e) * TL::PITCH + 64 * h + 4 * tx);
 #pragma unroll
-        for (int i = 0; i < TL::PI; ++i) {
-          const float f = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-          acc[i][4 * h + 0] = fmaf(f, x.x, acc[i][4 * h + 0]);
-          acc[i][4 * h + 1] = fmaf(f, x.y, acc[i][4 * h + 1]);
-          acc[i][4 * h + 2] = fmaf(f, x.z, acc[i][4 * h + 2]);
-          acc[i][4 * h + 3] = fmaf(f, x.w, acc[i][4 * h + 3]);
+      for (int i = 0; i < TL::PI; ++i) {
+        const float f = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+        const float2 f2 = make_float2(f, f);
+#pragma unroll
+        for (int h = 0; h < TL::DP / 64; ++h) {
+          acc[i][2 * h] = fma2(f2, make_float2(x[h].x, x[h].y), acc[i][2 * h]);
+          acc[i][2 * h + 1] = fma2(f2, make_float2(x[h].z, x[h].w), acc[i][2 * h + 1]);
         }
       }
     }
@@ -136,7 +132,7 @@ __device__ __forceinline__ void product(float (&acc)[TL::PI][TL::DP / 16], const
 }
 
 template <typename T, typename TL>
-__device__ __forceinline__ void store_rows(T* __restrict__ g, long long stride, int D, int rows, const float (&acc)[TL::PI][TL::DP / 16],
+__device__ __forceinline__ void store_rows(T* __restrict__ g, long long stride, int D, int rows, const float2 (&acc)[TL::PI][TL::DP / 32],
                                            const float (&mul)[TL::PI], int tx, int ty) {
 #pragma unroll
   for (int i = 0; i < TL::PI; ++i) {
@@ -147,7 +143,8 @@ __device__ __forceinline__ void store_rows(T* __restrict__ g, long long stride, 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = 64 * h + 4 * tx + e;
-        if (d < D) g[r * stride + d] = from_f<T>(mul[i] == 0.f ? 0.f : acc[i][4 * h + e] * mul[i]);
+        const float2 x = acc[i][2 * h + e / 2];
+        if (d < D) g[r * stride + d] = from_f<T>(mul[i] == 0.f ? 0.f : (e & 1 ? x.y : x.x) * mul[i]);
       }
   }
 }
@@ -187,7 +184,7 @@ template <typename T, typename TL>
 __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __grid_constant__ VsaCross a, int splits, float* part_out, float* part_lse,
                                                                      bool vec) {
   extern __shared__ __align__(16) float sm[];
-  float *sq = sm, *sk = sq + TL::row_floats, *sv = sk + TL::col_floats, *ss = TL::OVER ? sk : sv + TL::col_floats;
+  float *sq = sm, *sk = sq + TL::row_floats, *sv = sk + TL::col_floats, *ss = sv + TL::col_floats;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int split = blockIdx.x % splits, qt = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
   const int row0 = qt * TL::RT, rows = (int)min((long long)TL::RT, (long long)a.Lq - row0);
@@ -196,13 +193,14 @@ __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __gri
   const int t0 = split * per, t1 = min(tiles, t0 + per);
   const float c = a.scale * kLog2e;
   load_tile<T, TL, TL::RT>(sq, slice<T>(a.q, a.q_stride, b, h) + row0 * a.q_stride[2], a.q_stride[2], a.D, vec, [&](int r) { return r < rows; });
-  float m[TL::PI], l[TL::PI], acc[TL::PI][TL::DP / 16];
+  float m[TL::PI], l[TL::PI];
+  float2 acc[TL::PI][TL::DP / 32];
 #pragma unroll
   for (int i = 0; i < TL::PI; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int d = 0; d < TL::DP / 16; ++d) acc[i][d] = 0.f;
+    for (int d = 0; d < TL::DP / 32; ++d) acc[i][d] = make_float2(0.f, 0.f);
   }
   for (int t = t0; t < t1; ++t) {
     const int k0 = t * TL::CT;
@@ -214,7 +212,6 @@ __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __gri
     __syncthreads();
     float s[TL::PI][TL::PJ];
     scores<TL>(s, sq, sk, tx, ty);
-    if (TL::OVER) __syncthreads();
     bool on[TL::PJ];
 #pragma unroll
     for (int j = 0; j < TL::PJ; ++j) on[j] = live(tx + 16 * j);
@@ -236,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __gri
       l[i] = l[i] * keep + lanes16_sum(sum);
       m[i] = mn;
 #pragma unroll
-      for (int d = 0; d < TL::DP / 16; ++d) acc[i][d] *= keep;
+      for (int d = 0; d < TL::DP / 32; ++d) acc[i][d] = mul2(acc[i][d], make_float2(keep, keep));
     }
     copies_wait<0>();
     __syncthreads();
@@ -269,17 +266,17 @@ __global__ void __launch_bounds__(kThreads) cross_fwd_generic_kernel(const __gri
     for (long long r = row0 + TL::RT + tid; r < lp; r += kThreads) a.lse2[bh * lp + r] = INFINITY;
 }
 
-// ---- backward: dQ (and delta) of one tile of query rows -----------------------------------------------------------
+// ---- backward: dQ (and delta) of one tile of query rows, one range of key tiles -----------------------------------------------------------
 template <typename T, typename TL>
-__global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid_constant__ VsaCross a, bool vec) {
+__global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid_constant__ VsaCross a, int splits, float* part, bool vec) {
   extern __shared__ __align__(16) float sm[];
   float *sq = sm, *sdo = sq + TL::row_floats, *sk = sdo + TL::row_floats, *sv = sk + TL::col_floats, *ss = TL::OVER ? sv : sv + TL::col_floats;
   static_assert(TL::RT <= 2 * TL::CT, "the rows of out pass through the tiles of K and V");
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int qt = blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
+  const int split = blockIdx.x % splits, qt = blockIdx.x / splits, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(a.H / a.Hkv);
   const int row0 = qt * TL::RT, rows = (int)min((long long)TL::RT, (long long)a.Lq - row0);
   const Ctx keys = keys_of(a, b);
-  const int tiles = (keys.len + TL::CT - 1) / TL::CT;
+  const int tiles = (keys.len + TL::CT - 1) / TL::CT, per = (tiles + splits - 1) / splits, t1 = min(tiles, (split + 1) * per);
   const float c = a.scale * kLog2e;
   const long long bh = (long long)b * a.H + h, lp = cross_rows(a.Lq);
   auto there = [&](int r) { return r < rows; };
@@ -288,7 +285,8 @@ __global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid
   load_tile<T, TL, TL::RT>(sdo, slice<T>(a.dout, a.dout_stride, b, h) + row0 * a.dout_stride[2], a.dout_stride[2], a.D, vec, there);
   copies_wait<0>();
   __syncthreads();
-  float lse[TL::PI], delta[TL::PI], acc[TL::PI][TL::DP / 16], mul[TL::PI];
+  float lse[TL::PI], delta[TL::PI], mul[TL::PI];
+  float2 acc[TL::PI][TL::DP / 32];
 #pragma unroll
   for (int i = 0; i < TL::PI; ++i) {
     const int r = TL::PI * ty + i;
@@ -296,12 +294,12 @@ __global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid
     for (int e = tx; e < TL::DP; e += 16) d = fmaf(sk[r * TL::PITCH + e], sdo[r * TL::PITCH + e], d);
     delta[i] = lanes16_sum(d);
     lse[i] = row0 + r < lp ? a.lse2[bh * lp + row0 + r] : INFINITY;
-    if (tx == 0 && row0 + r < lp) a.delta[bh * lp + row0 + r] = r < rows ? delta[i] : 0.f;
+    if (tx == 0 && split == 0 && row0 + r < lp) a.delta[bh * lp + row0 + r] = r < rows ? delta[i] : 0.f;
     mul[i] = a.scale;
 #pragma unroll
-    for (int e = 0; e < TL::DP / 16; ++e) acc[i][e] = 0.f;
+    for (int e = 0; e < TL::DP / 32; ++e) acc[i][e] = make_float2(0.f, 0.f);
   }
-  for (int t = 0; t < tiles; ++t) {
+  for (int t = split * per; t < t1; ++t) {
     const int k0 = t * TL::CT;
     __syncthreads();
     auto live = [&](int r) { return keys.live(k0 + r); };
@@ -325,9 +323,25 @@ __global__ void __launch_bounds__(kThreads) cross_dq_generic_kernel(const __grid
     __syncthreads();
     product<TL>(acc, ss, sk, tx, ty);
   }
-  if (row0 + TL::RT >= a.Lq)
+  if (split == 0 && row0 + TL::RT >= a.Lq)
     for (long long r = row0 + TL::RT + tid; r < lp; r += kThreads) a.delta[bh * lp + r] = 0.f;
+  if (splits > 1) {
+    store_rows<float, TL>(part + ((split * (long long)a.B * a.H + bh) * a.Lq + row0) * a.D, a.D, a.D, rows, acc, mul, tx, ty);
+    return;
+  }
   store_rows<T, TL>(slice<T>(a.dq, a.dq_stride, b, h) + row0 * a.dq_stride[2], a.dq_stride[2], a.D, rows, acc, mul, tx, ty);
+}
+
+// The parts of dQ, added in the order of the splits.
+template <typename T>
+__global__ void __launch_bounds__(256) cross_dq_sum_kernel(const __grid_constant__ VsaCross a, int splits, const float* __restrict__ part) {
+  const long long one = (long long)a.B * a.H * a.Lq * a.D, at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= one) return;
+  const long long row = at / a.D, bh = row / a.Lq, b = bh / a.H;
+  float x = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) x += part[s * one + at];
+  ((T*)a.dq)[b * a.dq_stride[0] + (bh - b * a.H) * a.dq_stride[1] + (row - bh * a.Lq) * a.dq_stride[2] + (at - row * a.D)] = from_f<T>(x);
 }
 
 // ---- backward: dK, dV of one tile of keys, one range of the query tiles of all heads that share them ------------------
@@ -344,14 +358,15 @@ __global__ void __launch_bounds__(kThreads) cross_dkdv_generic_kernel(const __gr
   auto live = [&](int r) { return keys.live(k0 + r); };
   load_tile<T, TL, TL::RT>(sk, slice<T>(a.k, a.k_stride, b, hk) + k0 * a.k_stride[2], a.k_stride[2], a.D, vec, live);
   load_tile<T, TL, TL::RT>(sv, slice<T>(a.v, a.v_stride, b, hk) + k0 * a.v_stride[2], a.v_stride[2], a.D, vec, live);
-  float dk[TL::PI][TL::DP / 16], dv[TL::PI][TL::DP / 16], mul_k[TL::PI], mul_v[TL::PI];
+  float2 dk[TL::PI][TL::DP / 32], dv[TL::PI][TL::DP / 32];
+  float mul_k[TL::PI], mul_v[TL::PI];
 #pragma unroll
   for (int i = 0; i < TL::PI; ++i) {
     const bool on = live(TL::PI * ty + i);
     mul_k[i] = on ? a.scale : 0.f;
     mul_v[i] = on ? 1.f : 0.f;
 #pragma unroll
-    for (int e = 0; e < TL::DP / 16; ++e) dk[i][e] = dv[i][e] = 0.f;
+    for (int e = 0; e < TL::DP / 32; ++e) dk[i][e] = dv[i][e] = make_float2(0.f, 0.f);
   }
   const int qtiles = (int)((a.Lq + TL::CT - 1) / TL::CT);
   const long long total = (long long)qtiles * group, per = (total + splits - 1) / splits;
@@ -576,8 +591,7 @@ int reserve(Kern kern, int bytes, const char* what) {
 
 template <typename T, typename TL>
 int fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
-  const int bytes = (TL::row_floats + 2 * TL::col_floats + (TL::OVER ? 0 : TL::score_floats)) * 4;
-  static_assert(!TL::OVER || TL::score_floats <= TL::col_floats, "P goes over K");
+  const int bytes = (TL::row_floats + 2 * TL::col_floats + TL::score_floats) * 4;
   int rc = reserve(cross_fwd_generic_kernel<T, TL>, bytes, "cross attention forward");
   if (rc) return rc;
   const int64_t tiles = (a.Lq + TL::RT - 1) / TL::RT;
@@ -586,14 +600,16 @@ int fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStr
   return check_launch("cross_fwd_generic_kernel");
 }
 template <typename T, typename TL>
-int dq_pass(const VsaCross& a, cudaStream_t st) {
+int dq_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   constexpr int last = TL::OVER ? (TL::score_floats > TL::col_floats ? TL::score_floats : TL::col_floats) : TL::col_floats + TL::score_floats;
   const int bytes = (2 * TL::row_floats + TL::col_floats + last) * 4;
-  const int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
+  int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
   if (rc) return rc;
-  cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::RT - 1) / TL::RT), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
-      a, vec4(a, true));
-  return check_launch("cross_dq_generic_kernel");
+  cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::RT - 1) / TL::RT * splits), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
+      a, splits, part, vec4(a, true));
+  if ((rc = check_launch("cross_dq_generic_kernel")) || splits == 1) return rc;
+  cross_dq_sum_kernel<T><<<(unsigned)((a.B * a.H * a.Lq * a.D + 255) / 256), 256, 0, st>>>(a, splits, part);
+  return check_launch("cross_dq_sum_kernel");
 }
 template <typename T, typename TL>
 int dkdv_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
@@ -608,47 +624,55 @@ int dkdv_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
 template <typename T>
 int fwd_by_dim(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
   const bool large = cross_generic_fwd_tile(a.B, a.H, a.Lq, a.Lkv, a.D).large;
-  if (a.D <= 64) return large ? fwd<T, Tile<64, 128>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<64, 64>>(a, splits, part_out, part_lse, st);
+  if (a.D <= 64) return large ? fwd<T, Tile<64, 128, 64>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<64, 64>>(a, splits, part_out, part_lse, st);
   if (a.D <= 128)
-    return large ? fwd<T, Tile<128, 128, 128, true>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<128, 64>>(a, splits, part_out, part_lse, st);
+    return large ? fwd<T, Tile<128, 128, 64>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<128, 64>>(a, splits, part_out, part_lse, st);
   return large ? fwd<T, Tile<256, 64>>(a, splits, part_out, part_lse, st) : fwd<T, Tile<256, 32>>(a, splits, part_out, part_lse, st);
 }
 template <typename T>
-int bwd_by_dim(const VsaCross& a, int splits, float* part, cudaStream_t st) {
-  // dQ has no cut over the keys: its tiles shrink with the rows that there are
-  const int64_t heads = a.B * a.H, edge = a.D <= 128 ? 128 : 64;
-  const bool most = heads * ((a.Lq + edge - 1) / edge) >= kDqLarge, few = heads * ((a.Lq + 63) / 64) < 148;
+int bwd_by_dim(const VsaCross& a, int splits, int dq_splits, float* part, cudaStream_t st) {
+  const bool most = cross_generic_dq_tile(a.B, a.H, a.Lq, a.D).large;
   int rc;
-  if (a.D <= 64) rc = most ? dq_pass<T, Tile<64, 128>>(a, st) : few ? dq_pass<T, Tile<64, 32>>(a, st) : dq_pass<T, Tile<64, 64>>(a, st);
-  else if (a.D <= 128) rc = most ? dq_pass<T, Tile<128, 128, 64, true>>(a, st) : few ? dq_pass<T, Tile<128, 32>>(a, st) : dq_pass<T, Tile<128, 64>>(a, st);
-  else rc = most ? dq_pass<T, Tile<256, 64, 32>>(a, st) : dq_pass<T, Tile<256, 32>>(a, st);
+  if (a.D <= 64) rc = most ? dq_pass<T, Tile<64, 128, 64>>(a, dq_splits, part, st) : dq_pass<T, Tile<64, 64>>(a, dq_splits, part, st);
+  else if (a.D <= 128) rc = most ? dq_pass<T, Tile<128, 128, 64, true>>(a, dq_splits, part, st) : dq_pass<T, Tile<128, 64>>(a, dq_splits, part, st);
+  else rc = most ? dq_pass<T, Tile<256, 64, 32>>(a, dq_splits, part, st) : dq_pass<T, Tile<256, 32>>(a, dq_splits, part, st);
   if (rc || a.Lkv == 0 || a.dk == nullptr) return rc;
   const bool large = cross_generic_bwd_tile(a.B, a.H, a.Hkv, a.Lq, a.Lkv, a.D).large;
-  if (a.D <= 64) return large ? dkdv_pass<T, Tile<64, 128, 128, true>>(a, splits, part, st) : dkdv_pass<T, Tile<64, 64>>(a, splits, part, st);
+  if (a.D <= 64) return large ? dkdv_pass<T, Tile<64, 128, 64, true>>(a, splits, part, st) : dkdv_pass<T, Tile<64, 64>>(a, splits, part, st);
   if (a.D <= 128) return large ? dkdv_pass<T, Tile<128, 96, 64, true>>(a, splits, part, st) : dkdv_pass<T, Tile<128, 64>>(a, splits, part, st);
   return large ? dkdv_pass<T, Tile<256, 64, 32, true>>(a, splits, part, st) : dkdv_pass<T, Tile<256, 32>>(a, splits, part, st);
 }
 
 }  // namespace
 
+// Rows of `large` edge where tiles of them do not compute a quarter more than those of `small` would, and there are enough tiles of scores
+// to fill the SMs: us of the large and the small ones, forward [1, 8, 1600, 128] x 150 (312 tiles) 49 / 59, [1, 1, 1500, 128] x 1500 (288)
+// 53 / 46; dK/dV [1, 1, 1500, 128] x 1500 (384) 69 / 72, [1, 2, 1500, 128] x 300 (192) 49 / 40.
+static bool large_tiles(int64_t rows, int64_t large, int64_t small, int64_t others, int64_t enough) {
+  const int64_t n = (rows + large - 1) / large;
+  return n * large * 4 <= (rows + small - 1) / small * small * 5 && n * others >= enough;
+}
 CrossTile cross_generic_fwd_tile(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D) {
-  const int edge = D <= 128 ? 128 : 64, small = D <= 128 ? 64 : 32;
-  if (B * H * ((Lq + edge - 1) / edge) * ((Lkv + edge - 1) / edge) >= kFwdLarge) return {edge, edge, true};
-  return {small, small, false};
+  if (D > 128) return large_tiles(Lq, 64, 32, B * H * ((Lkv + 63) / 64), 300) ? CrossTile{64, 64, true} : CrossTile{32, 32, false};
+  return large_tiles(Lq, 128, 64, B * H * ((Lkv + 63) / 64), 300) ? CrossTile{128, 64, true} : CrossTile{64, 64, false};
+}
+CrossTile cross_generic_dq_tile(int64_t B, int64_t H, int64_t Lq, int D) {
+  if (D > 128) return large_tiles(Lq, 64, 32, B * H, 74) ? CrossTile{64, 32, true} : CrossTile{32, 32, false};
+  return large_tiles(Lq, 128, 64, B * H, 74) ? CrossTile{128, 64, true} : CrossTile{64, 64, false};
 }
 CrossTile cross_generic_bwd_tile(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D) {
-  const int rows = D <= 64 ? 128 : D <= 128 ? 96 : 64, cols = D <= 64 ? 128 : D <= 128 ? 64 : 32, small = D <= 128 ? 64 : 32;
-  if (B * H * ((Lq + cols - 1) / cols) * ((Lkv + rows - 1) / rows) >= kDkdvLarge) return {rows, cols, true};
-  return {small, small, false};
+  if (D > 128) return large_tiles(Lkv, 64, 32, B * H * ((Lq + 31) / 32), 300) ? CrossTile{64, 32, true} : CrossTile{32, 32, false};
+  const int rows = D <= 64 ? 128 : 96;
+  return large_tiles(Lkv, rows, 64, B * H * ((Lq + 63) / 64), 300) ? CrossTile{rows, 64, true} : CrossTile{64, 64, false};
 }
 
 int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
   if (a.dtype == VSA_F32) return fwd_by_dim<float>(a, splits, part_out, part_lse, st);
   return a.dtype == VSA_F16 ? fwd_by_dim<__half>(a, splits, part_out, part_lse, st) : fwd_by_dim<__nv_bfloat16>(a, splits, part_out, part_lse, st);
 }
-int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st) {
-  if (a.dtype == VSA_F32) return bwd_by_dim<float>(a, splits, part, st);
-  return a.dtype == VSA_F16 ? bwd_by_dim<__half>(a, splits, part, st) : bwd_by_dim<__nv_bfloat16>(a, splits, part, st);
+int cross_bwd_generic(const VsaCross& a, int splits, int dq_splits, float* part, cudaStream_t st) {
+  if (a.dtype == VSA_F32) return bwd_by_dim<float>(a, splits, dq_splits, part, st);
+  return a.dtype == VSA_F16 ? bwd_by_dim<__half>(a, splits, dq_splits, part, st) : bwd_by_dim<__nv_bfloat16>(a, splits, dq_splits, part, st);
 }
 
 int cross_join(const VsaCross& a, int splits, const float* part_out, const float* part_lse, cudaStream_t st) {

@@ -79,6 +79,7 @@ struct CrossTile {
   bool large;
 };
 CrossTile cross_generic_fwd_tile(int64_t B, int64_t H, int64_t Lq, int64_t Lkv, int D);
+CrossTile cross_generic_dq_tile(int64_t B, int64_t H, int64_t Lq, int D);
 CrossTile cross_generic_bwd_tile(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D);
 // tensor path (cross_umma.cu), lengths only (key_bits is not looked at): by head dim and type; with pointers and strides
 bool cross_umma_shape(int D, int dtype);
@@ -92,7 +93,7 @@ int cross_bwd_umma(const VsaCross& a, int splits, bool parts, float* part, cudaS
 // splits > 1: partial outputs [splits][B*H][Lq][D] and statistics [splits][B*H][Lq] (-inf: no live key), for cross_join
 int cross_fwd_generic(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 // splits > 1: partial dK and dV [splits][2][B*Hkv][Lkv][D], for cross_sum
-int cross_bwd_generic(const VsaCross& a, int splits, float* part, cudaStream_t st);
+int cross_bwd_generic(const VsaCross& a, int splits, int dq_splits, float* part, cudaStream_t st);
 int cross_join(const VsaCross& a, int splits, const float* part_out, const float* part_lse, cudaStream_t st);
 int cross_sum(const VsaCross& a, int splits, const float* part, cudaStream_t st, const int32_t* prefix = nullptr);
 // live rows of K and V (16-bit types) to the front, zeros behind: k, v dense [B][Hkv][Lkv][D]; prefix [B][cross_words(Lkv)], counts [B]
