@@ -8,6 +8,8 @@
 // [1, 12, 4096, 128] x 2048 the forward takes 1386 us (37 of 72 TFLOP/s; pipe 64 % busy, reads 50 %), the backward 4470 (its seven products at
 // 40).  8 x 8 scores a thread spill (1448 us); chains without pairs are slower in the backward (4954), two CTAs an SM at head dim 64
 // spill too (874 us for 830).  With few query rows a pass is cut over the keys, with few keys dK/dV is over the query rows.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -583,16 +585,24 @@ bool vec4(const VsaCross& a, bool backward) {      // 16-byte reads of fp32 rows
          (!backward || (fine(a.out, a.out_stride) && fine(a.dout, a.dout_stride)));
 }
 
+// The kernel's shared memory, once per device: `ready` has a bit for each.
 template <typename Kern>
-int reserve(Kern kern, int bytes, const char* what) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == cudaSuccess ? VSA_OK : fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
+int reserve(Kern kern, int bytes, const char* what, std::atomic<uint64_t>& ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && dev < 64 && (ready.load(std::memory_order_relaxed) & bit)) return VSA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(VSA_ERR_LAUNCH, "%s: shared memory: %s", what, cudaGetErrorString(e));
+  if (dev < 64) ready.fetch_or(bit, std::memory_order_relaxed);
+  return VSA_OK;
 }
 
 template <typename T, typename TL>
 int fwd(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st) {
   const int bytes = (TL::row_floats + 2 * TL::col_floats + TL::score_floats) * 4;
-  int rc = reserve(cross_fwd_generic_kernel<T, TL>, bytes, "cross attention forward");
+  static std::atomic<uint64_t> ready{0};
+  int rc = reserve(cross_fwd_generic_kernel<T, TL>, bytes, "cross attention forward", ready);
   if (rc) return rc;
   const int64_t tiles = (a.Lq + TL::RT - 1) / TL::RT;
   cross_fwd_generic_kernel<T, TL><<<dim3((unsigned)(tiles * splits), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
@@ -603,7 +613,8 @@ template <typename T, typename TL>
 int dq_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   constexpr int last = TL::OVER ? (TL::score_floats > TL::col_floats ? TL::score_floats : TL::col_floats) : TL::col_floats + TL::score_floats;
   const int bytes = (2 * TL::row_floats + TL::col_floats + last) * 4;
-  int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ");
+  static std::atomic<uint64_t> ready{0};
+  int rc = reserve(cross_dq_generic_kernel<T, TL>, bytes, "cross attention dQ", ready);
   if (rc) return rc;
   cross_dq_generic_kernel<T, TL><<<dim3((unsigned)((a.Lq + TL::RT - 1) / TL::RT * splits), (unsigned)a.H, (unsigned)a.B), kThreads, bytes, st>>>(
       a, splits, part, vec4(a, true));
@@ -614,7 +625,8 @@ int dq_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
 template <typename T, typename TL>
 int dkdv_pass(const VsaCross& a, int splits, float* part, cudaStream_t st) {
   const int bytes = (2 * TL::row_floats + 2 * TL::col_floats + (TL::OVER ? 1 : 2) * TL::score_floats) * 4;
-  const int rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV");
+  static std::atomic<uint64_t> ready{0};
+  const int rc = reserve(cross_dkdv_generic_kernel<T, TL>, bytes, "cross attention dK/dV", ready);
   if (rc) return rc;
   cross_dkdv_generic_kernel<T, TL><<<dim3((unsigned)((a.Lkv + TL::RT - 1) / TL::RT * splits), (unsigned)a.Hkv, (unsigned)a.B), kThreads, bytes,
                                      st>>>(a, splits, part, vec4(a, true));

@@ -140,7 +140,8 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
 // asks for), 1250 of shared-memory traffic (160 KB at 128 B/clk), 1024 of exponentials before a quarter of them moved to the FMA pipe;
 // what bounds it is a softmax group's chain (scores from tensor memory, maximum, exponentials, P back), which two groups overlap.
 // More warps were slower: eight a tile sharing its rows, and four groups on alternating steps with the maximum handed on (982 for
-// 860 us).  A piece's end (O out, the next piece's set-up) is some 3000 of 16000 cycles at 512 keys.
+// 860 us).  A piece's end (O out, the next piece's set-up) is some 3000 of 16000 cycles at 512 keys, but the other tile's group works
+// under it: four warps that write O while both groups go on brought nothing (880 -> 891 us, at eight heads 181 -> 188).
 constexpr int kFwdThreads = 256 + 256;     // loads and four issuers of MMAs (eight warps), two softmax groups
 constexpr int kKeys = 64;                  // keys of a step
 constexpr int kFwdPoly = 2;                // of eight pairs of exponentials, on the FMA pipe
@@ -502,15 +503,15 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // ------------------------------------------------------------------------------------------------------
 // dQ (and delta)
 // ------------------------------------------------------------------------------------------------------
-// A piece of work is 128 query rows of one head: S = Q K^T, dP = dO V^T, dQ += dS K per key tile.  All sixteen elementwise warps
-// share a tile, 32 score columns a thread; S (later dS) in two accumulators, dP in one that is free again as soon as it has been read.
-// delta = rowsum(out * dout) takes dout from its tile in shared memory and out from registers that were filled while the piece before
-// was finished.
+// A piece of work is 128 query rows of one head: S = Q K^T, dP = dO V^T, dQ += dS K per key tile.  Sixteen elementwise warps share a
+// tile, 32 score columns a thread; S (later dS) in two accumulators, dP in one that is free again as soon as it has been read.  Four warps
+// form delta = rowsum(out * dout) and the statistics of the next piece's rows from memory, into two buffers, and ask L2 for the rows
+// of the piece after it; four more write a finished dQ while the elementwise warps are at the next piece.
 //
-// [1, 8, 92160, 128] x 512 keys: 268 us, 1080 TFLOP/s.  A piece of four key tiles takes 12,000 cycles: 1700 to 1800 a tile (1536 of MMAs,
-// 1024 of exponentials before three of eight moved to the FMA pipe) and 5000 around them (delta, the wait for the last product, dQ out,
-// the next piece's rows): sixteen warps that all do the same at the same time.  Reading dQ under the next piece's first tile instead
-// of behind the last one changed nothing.
+// [1, 8, 92160, 128] x 512 keys: 236 us, 1230 TFLOP/s (where dK/dV takes 257).  A piece of four key tiles takes some 8800 cycles: 1700 to
+// 1800 a tile (1536 of MMAs, 1024 of exponentials before three of eight moved to the FMA pipe), then the elementwise warps wait 500 to
+// 800 for the delta warps, whose 8800 cycles are loads of 64 KB.  With delta and dQ done by the elementwise warps the tiles' 7000 cycles had
+// 5000 of them around (268 us).  Loads of two delta rows in flight, and Q and dO on barriers of their own, changed nothing.
 constexpr int kDqCols = 32;
 constexpr int kDqGroups = kRows / kDqCols;
 constexpr int kDqPoly = 3;                 // of eight pairs of exponentials, on the FMA pipe
