@@ -421,3 +421,48 @@ def test_offsets_beyond_32_bits(dtype, D, L):
                 torch.testing.assert_close(a.float(), b.float(), rtol=4 * torch.finfo(dtype).eps, atol=4 * torch.finfo(dtype).eps * b.abs().max().item())
     rot = V.build_rotary_metadata((max(L, T),), D if D % 4 == 0 else D - D % 4, device=DEV)
     assert torch.equal(V.video_rotary(k, None, rot), V.video_rotary(dense[1], None, rot))
+
+
+def _cuda_core_tiles(D):
+    """Which passes of [2, 4 + 2, 1300, D] x 333 run on the large tiles of the CUDA-core kernels: at least 300 tiles of scores
+    (forward, dK/dV), 74 of query rows (dQ), and no more than a quarter of padding."""
+    heads, Lq, Lkv = 8, 1300, 333
+    tiles = lambda n, edge: -(-n // edge)
+    rows, cols, keys, queries = (64, 64, 64, 32) if D > 128 else (128, 64, 128 if D <= 64 else 96, 64)
+    fits = lambda n, large, small: 4 * tiles(n, large) * large <= 5 * tiles(n, small) * small
+    small = 32 if D > 128 else 64
+    return (fits(Lq, rows, small) and heads * tiles(Lq, rows) * tiles(Lkv, cols) >= 300, fits(Lq, rows, small) and heads * tiles(Lq, rows) >= 74,
+            fits(Lkv, keys, small) and heads * tiles(Lkv, keys) * tiles(Lq, queries) >= 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 128), (torch.float32, 256), (torch.float32, 61), (torch.bfloat16, 100),
+                                     (torch.float16, 200)])
+def test_large_tiles_of_the_cuda_core_kernels(dtype, D):
+    """Problems that fill the GPU with large tiles; lengths and masks, values that must not be read."""
+    assert all(_cuda_core_tiles(D))
+    B, H, Hk, L, T = 2, 4, 2, 1300, 333
+    q, k, v, dout = _inputs(B, H, Hk, L, T, D, dtype, D)
+    lengths = torch.tensor([T, 190])
+    mask = torch.rand(B, T, generator=torch.Generator().manual_seed(1)) < 0.7
+    for ln, mk in ((None, None), (lengths, None), (lengths, mask)):
+        live = _live(B, T, ln, mk)
+        kk, vv = k.clone(), v.clone()
+        dead = ~live[:, None, :, None].to(DEV).expand_as(kk)
+        kk[dead], vv[dead] = math.nan, math.inf
+        got = _run(q, kk, vv, dout, None if ln is None else ln.to(DEV), None if mk is None else mk.to(DEV))
+        _compare(got, _exact(q, k, v, live, 1 / math.sqrt(D), dout), dtype)
+        assert not got[2][dead].any() and not got[3][dead].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 200])
+def test_few_rows_of_queries_against_long_states_in_fp32(D):
+    """dQ cut over the keys: parts without a live key, and a sample without one."""
+    B, H, Hk, L, T = 2, 1, 1, 70, 1900
+    q, k, v, dout = _inputs(B, H, Hk, L, T, D, torch.float32, D + 1)
+    for lengths in (None, torch.tensor([1900, 100]), torch.tensor([0, 65])):
+        live = _live(B, T, lengths, None)
+        got = _run(q, k, v, dout, None if lengths is None else lengths.to(DEV))
+        _compare(got, _exact(q, k, v, live, 1 / math.sqrt(D), dout), torch.float32)
+        assert all(torch.equal(a, b) for a, b in zip(got, _run(q, k, v, dout, None if lengths is None else lengths.to(DEV))))
