@@ -1153,10 +1153,10 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
     if (!ok && lane == 0) atomicCAS(status, 0, 95);
     if (ok) ok = CROSS_WAIT(bar(K_ACC_FULL), 0);
+    uint8_t* stage_k = sm + Sm::k;            // every MMA is done: dK over K, dV over V
+    uint8_t* stage_v = sm + Sm::v;
     if (ok) {
       tc_fence_after();
-      uint8_t* stage_k = sm + Sm::k;          // every MMA is done: dK over K, dV over V
-      uint8_t* stage_v = sm + Sm::v;
       for (int j = cg; j < 2 * (HD / 32); j += kDkGroups) {
         const bool is_k = j < HD / 32;
         const int jj = is_k ? j : j - HD / 32;
@@ -1177,17 +1177,17 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             if (32 * jj + i < a.D) *reinterpret_cast<uint4*>(dst + i) = make_uint4(av[i], av[i + 1], av[i + 2], av[i + 3]);
         }
       }
-      if (part == nullptr) {
-        named_barrier(1, kDkEwThreads);
-        for (int i = st; i < kRows * HD / 8; i += kDkEwThreads) {
-          const int r = i / (HD / 8), ch = i % (HD / 8);
-          if (krow0 + r >= a.Lkv || ch * 8 >= a.D) continue;
-          const uint32_t off = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>((T*)a.dk + b * a.dk_stride[0] + hk * a.dk_stride[1] + (krow0 + r) * a.dk_stride[2] + ch * 8) =
-              *reinterpret_cast<const uint4*>(stage_k + off);
-          *reinterpret_cast<uint4*>((T*)a.dv + b * a.dv_stride[0] + hk * a.dv_stride[1] + (krow0 + r) * a.dv_stride[2] + ch * 8) =
-              *reinterpret_cast<const uint4*>(stage_v + off);
-        }
+    }
+    if (part == nullptr) {
+      named_barrier(1, kDkEwThreads);          // of every warp: one whose wait ran out must not leave the others in it
+      for (int i = st; i < kRows * HD / 8 && ok; i += kDkEwThreads) {
+        const int r = i / (HD / 8), ch = i % (HD / 8);
+        if (krow0 + r >= a.Lkv || ch * 8 >= a.D) continue;
+        const uint32_t off = r * (HD * 2) + ((ch ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>((T*)a.dk + b * a.dk_stride[0] + hk * a.dk_stride[1] + (krow0 + r) * a.dk_stride[2] + ch * 8) =
+            *reinterpret_cast<const uint4*>(stage_k + off);
+        *reinterpret_cast<uint4*>((T*)a.dv + b * a.dv_stride[0] + hk * a.dv_stride[1] + (krow0 + r) * a.dv_stride[2] + ch * 8) =
+            *reinterpret_cast<const uint4*>(stage_v + off);
       }
     }
   }
