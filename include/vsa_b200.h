@@ -479,12 +479,15 @@ int vsa_rotary(const VsaRotary* a, void* stream);
  *   lse2      [B * H, Lq rounded up to 128] fp32: base-2 log-sum-exp of the scaled scores, +inf for rows without a live key and
  *             for the padding; written by the forward, read by the backward
  *   delta     the same shape, scratch of the backward
+ *   bounds    [B * Hkv, VSA_CROSS_BOUNDS] fp32, scratch of the backward in fp16 with head dims that are multiples of 8 up to 128, else
+ *             not looked at: norms that keep its 16-bit operands within the type's range
  *   dk, dv    both NULL: the pass over the keys is left out
  *   workspace vsa_cross_workspace_bytes(backward, ..., key_bits != NULL) bytes (0: may be NULL), 16-byte aligned, free again after the
  *             call
  * bf16 and fp16 with head dims that are multiples of 8 up to 128, 16-byte aligned pointers and strides of multiples of 8 run on
  * tcgen05 kernels (vsa_cross_on_tensor_cores), everything else up to head dim 256 on CUDA cores in fp32.  Results do not
  * depend on the order in which blocks run.  No reference counterpart (its operator is self-attention over one token grid). */
+#define VSA_CROSS_BOUNDS 33
 typedef struct VsaCross {
   const void *q, *k, *v, *dout;
   void *out, *dq, *dk, *dv;                    /* dout, dq, dk, dv, delta: backward only */
@@ -492,6 +495,7 @@ typedef struct VsaCross {
   const int32_t* kv_lengths;
   const uint32_t* key_bits;
   void* workspace;
+  float* bounds;
   int64_t B, H, Hkv, Lq, Lkv;
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
   float scale;

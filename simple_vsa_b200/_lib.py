@@ -50,9 +50,10 @@ class Rotary(ctypes.Structure):
 
 class Cross(ctypes.Structure):
     """``VsaCross`` of the header; ``PACK`` as in ``Rotary``."""
-    PACK = struct.Struct("@13P5q24qf2i0q")
+    PACK = struct.Struct("@14P5q24qf2i0q")
+    BOUNDS = 33
     _fields_ = [(n, P) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "lse2", "delta", "kv_lengths", "key_bits",
-                                 "workspace")] + \
+                                 "workspace", "bounds")] + \
                [(n, L) for n in ("B", "H", "Hkv", "Lq", "Lkv")] + \
                [(n + "_stride", L * 3) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + \
                [("scale", F), ("D", I), ("dtype", I)]

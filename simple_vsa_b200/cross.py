@@ -54,10 +54,11 @@ def _launch(name: str, backward: int, raster: bool, scale: float, dt: int, q, k,
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     n = _lib.lib.vsa_cross_workspace_bytes(backward, B, H, Hkv, Lq, Lkv, D, dt, key_bits is not None)
     ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n > 0 else None
+    bounds = torch.empty(B * Hkv * _lib.Cross.BOUNDS, device=q.device, dtype=torch.float32) if backward and dt == _lib.VSA_F16 else None
     grads = (*_steps(dout, raster), *_steps(dq, raster), *_steps(dk, raster), *_steps(dv, raster)) if backward else _NO_STRIDES * 4
     a = _ARGUMENTS(_PACK(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(dout), out.data_ptr(), ptr(dq), ptr(dk), ptr(dv), lse.data_ptr(), ptr(delta),
-        ptr(kv_lengths), ptr(key_bits), ptr(ws), B, H, Hkv, Lq, Lkv, *_steps(q, raster), *_steps(k, raster), *_steps(v, raster),
+        ptr(kv_lengths), ptr(key_bits), ptr(ws), ptr(bounds), B, H, Hkv, Lq, Lkv, *_steps(q, raster), *_steps(k, raster), *_steps(v, raster),
         *_steps(out, raster), *grads, scale, D, dt))
     call(name, a, ops._stream(q.device))
 

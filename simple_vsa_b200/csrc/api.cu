@@ -720,6 +720,7 @@ static int check_cross(const VsaCross* a, bool backward, const char* what) {
   VSA_REQUIRE(!rows || (a->q && a->out && a->lse2), "%s: null pointer", what);
   VSA_REQUIRE(!rows || !keys || (a->k && a->v), "%s: null pointer", what);
   VSA_REQUIRE(!backward || !rows || (a->dout && a->dq && a->delta), "%s: null pointer", what);
+  VSA_REQUIRE(!backward || !rows || !keys || a->dtype != VSA_F16 || !cross_umma_shape(a->D, a->dtype) || a->bounds, "%s: fp16 needs bounds", what);
   VSA_REQUIRE(!backward || (a->dk == nullptr) == (a->dv == nullptr), "%s: give dk and dv, or neither", what);
   VSA_REQUIRE(a->workspace || cross_space(backward, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr).bytes == 0,
               "%s: a workspace is needed", what);

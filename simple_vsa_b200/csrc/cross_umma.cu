@@ -124,6 +124,21 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
   return poly ? poly_exp2<T>(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
 }
 
+// fp16 holds numbers from 2^16 down to 2^-14 in full, and small gradients against many keys are below that long before the result is: the
+// backward's 16-bit operands are therefore kept in the middle of the range by powers of two that the way out takes back (bf16 has the range
+// of fp32).  P, at most 1, is held as P 2^15.  dS = P (dP - delta): with dP_ij = do_i.v_j and delta the mean of dP_i under P_i,
+// |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= P (1 - P) 2 |do_i| max|v| <= |do_i| max|v| / 2, so that the largest 2^e with
+// 2^e |do_i| max|v| <= 2^16 keeps it below 2^15 whatever the operands hold, the rounding of delta included.  dQ takes an e for each row;
+// dK and dV add rows up, and take one for all rows of a key head.
+template <typename T> constexpr bool kRanged = kFmt<T> == 0u;
+constexpr int kPShift = 15;
+// e from the product of the squared norms (0: nothing to hold; infinite or NaN: nothing to save)
+__device__ __forceinline__ int range_exponent(float squares) {
+  const int log2 = (int)(__float_as_uint(squares) >> 23) - 127;      // floor; squares >= 0
+  return max(-30, min(60, 15 - (log2 >> 1)));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 // ------------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------------
@@ -526,7 +541,8 @@ struct DqSmem {
   static constexpr uint32_t v = k + k_stages * tile;
   static constexpr uint32_t stage = v + v_stages * tile;          // 32 rows x 64 bytes x HD / 32 a helper warp
   static constexpr uint32_t stats = stage + 4 * (HD / 32) * 2048; // float2 [2][128]: delta and the statistic of a row
-  static constexpr uint32_t bars = stats + 2048;
+  static constexpr uint32_t exps = stats + 2048;                  // int8 [2][128]: kRanged's e of a row
+  static constexpr uint32_t bars = exps + 256;
   static constexpr uint32_t misc = bars + 32 * 8;
   static constexpr uint32_t total = misc + 16;
 };
@@ -578,7 +594,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       mbar_init(bar(Q_S_EMPTY + i), 1);
       mbar_init(bar(Q_DS_FULL + i), 4 * kDqGroups);
       mbar_init(bar(Q_STATS_FULL + i), 4);
-      mbar_init(bar(Q_STATS_EMPTY + i), 4 * kDqGroups);
+      mbar_init(bar(Q_STATS_EMPTY + i), 4 * kDqGroups + (kRanged<T> ? 4 : 0));
     }
     mbar_init(bar(Q_ACC_EMPTY), 4);
     mbar_init(bar(Q_DP_FULL), 1);
@@ -715,6 +731,14 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         continue;
       }
+      float mul = 1.f;                           // bf16: the scale is in dS
+      if (kRanged<T>) {
+        ok = CROSS_WAIT(bar(Q_STATS_FULL + (live_items & 1)), (live_items >> 1) & 1);
+        if (!ok) break;
+        mul = a.scale * power_of_two(-reinterpret_cast<const int8_t*>(sm + Sm::exps)[(live_items & 1) * kRows + quarter * 32 + lane]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Q_STATS_EMPTY + (live_items & 1)));
+      }
       ok = CROSS_WAIT(bar(Q_ACC_FULL), live_items & 1);
       if (!ok) break;
       ++live_items;
@@ -731,6 +755,9 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(Q_ACC_EMPTY));
         }
+        if (kRanged<T>)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) av[i] = __float_as_uint(__uint_as_float(av[i]) * mul);
         // TMA's 64-byte swizzle (pieces xor row / 2); what lies outside the tensor is not written
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -750,7 +777,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   } else if (warp < 12) {
     // delta and the statistics of the next piece's rows while this one is worked on
     const int st = tid - 256;
-    const float log_scale = log2f(a.scale);      // > 0
+    const float log_scale = kRanged<T> ? 0.f : log2f(a.scale);      // > 0
     const long long lp = cross_rows(a.Lq);
     // The rows of the next piece into L2: its loads come when there is room for them, too late to wait for memory.
     auto ask = [&](const void* p, const int64_t(&stride)[3], const DqItem& it) {
@@ -760,6 +787,8 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     };
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       const DqItem it(a, qtiles, heads, item);
+      const long long bhk = (long long)it.b * a.Hkv + group_heads(it.h);
+      const float v_part = kRanged<T> ? a.bounds[bhk * VSA_CROSS_BOUNDS + lane] : 0.f;
       if (item + (int)gridDim.x < items) {
         const DqItem next(a, qtiles, heads, item + gridDim.x);
         ask(a.out, a.out_stride, next);
@@ -770,6 +799,9 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       ok = CROSS_WAIT(bar(Q_STATS_EMPTY + (live_items & 1)), ((live_items >> 1) & 1) ^ 1);
       if (!ok) break;
       float2* to = reinterpret_cast<float2*>(sm + Sm::stats) + (live_items & 1) * kRows;
+      int8_t* to_exp = reinterpret_cast<int8_t*>(sm + Sm::exps) + (live_items & 1) * kRows;
+      const float v_bound = kRanged<T> ? warp_max(v_part) : 0.f;
+      float g_bound = 0.f;                       // max |do|^2 of this thread's rows
       const long long stat = ((long long)it.b * a.H + it.h) * lp + it.row0;
       const T* o = (const T*)a.out + it.b * a.out_stride[0] + it.h * a.out_stride[1] + (long long)it.row0 * a.out_stride[2];
       const T* g = (const T*)a.dout + it.b * a.dout_stride[0] + it.h * a.dout_stride[1] + (long long)it.row0 * a.dout_stride[2];
@@ -785,7 +817,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           y[i] = *reinterpret_cast<const uint4*>(g + rr * a.dout_stride[2] + d);
         }
         const float lse = a.lse2[stat + r];
-        float sum = 0.f;
+        float sum = 0.f, norm = 0.f;
 #pragma unroll
         for (int i = 0; i < HD / 32; ++i) {
           if ((4 * i + (st & 3)) * 8 >= a.D) continue;
@@ -794,15 +826,29 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           for (int e = 0; e < 4; ++e) {
             const float2 u = Elem<T>::unpack(p[e]), w = Elem<T>::unpack(q[e]);
             sum = fmaf(u.x, w.x, fmaf(u.y, w.y, sum));
+            if (kRanged<T>) norm = fmaf(w.x, w.x, fmaf(w.y, w.y, norm));
           }
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        int e = 0;
+        if (kRanged<T>) {
+          norm += __shfl_xor_sync(0xffffffffu, norm, 1);
+          norm += __shfl_xor_sync(0xffffffffu, norm, 2);
+          g_bound = __uint_as_float(max(__float_as_uint(g_bound), __float_as_uint(norm)));      // NaN stays
+          e = range_exponent(norm * v_bound);
+        }
         if ((st & 3) == 0) {
           if (it.row0 + r >= a.Lq) sum = 0.f;
           a.delta[stat + r] = sum;
-          to[r] = make_float2(sum, log_scale - lse);             // 2^(s c - lse) * scale in one exponential
+          // bf16: 2^(s c - lse) * scale in one exponential; fp16: delta of the dP 2^e that the elementwise warps form
+          to[r] = make_float2(kRanged<T> ? sum * power_of_two(e) : sum, log_scale - lse);
+          if (kRanged<T>) to_exp[r] = (int8_t)e;
         }
+      }
+      if (kRanged<T>) {                          // for the dK/dV pass; the order of the rows changes nothing
+        const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(g_bound));
+        if (lane == 0) atomicMax(reinterpret_cast<unsigned*>(a.bounds) + bhk * VSA_CROSS_BOUNDS + VSA_CROSS_BOUNDS - 1, top);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Q_STATS_FULL + (live_items & 1)));
@@ -821,6 +867,8 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       ok = CROSS_WAIT(bar(Q_STATS_FULL + (live_items & 1)), (live_items >> 1) & 1);
       if (!ok) break;
       const float2 row_stats = stats[(live_items & 1) * kRows];
+      float2 f2 = make_float2(1.f, 1.f);
+      if (kRanged<T>) f2.x = f2.y = power_of_two(reinterpret_cast<const int8_t*>(sm + Sm::exps)[(live_items & 1) * kRows + row]);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Q_STATS_EMPTY + (live_items & 1)));
       ++live_items;
@@ -866,7 +914,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float2 y = mul2(pf[h / 2 + i], add2(word_pair(dv + 2 * i), d2));
+            const float2 y = mul2(pf[h / 2 + i], kRanged<T> ? fma2(word_pair(dv + 2 * i), f2, d2) : add2(word_pair(dv + 2 * i), d2));
             pk[h / 2 + i] = Elem<T>::pack(y.x, y.y);
           }
         }
@@ -1013,21 +1061,45 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const uint32_t tmem_dk = tmem + 128 * Sm::bufs, tmem_dv = tmem_dk + HD;
   static_assert(128 * Sm::bufs + 2 * HD <= (int)kTmemCols, "tensor memory of the dK/dV pass");
   bool ok = true;
+  int e = 0;                                      // kRanged: dS is held as dS 2^e, P as P 2^15
+  if (kRanged<T> && (warp == 0 || warp >= 4)) {
+    const float* bounds = a.bounds + (long long)bhk * VSA_CROSS_BOUNDS;      // 32 parts of max |v|^2, then max |do|^2
+    e = range_exponent(warp_max(bounds[lane]) * bounds[VSA_CROSS_BOUNDS - 1]);
+  }
+  const float range = kRanged<T> ? power_of_two(e - kPShift) : 1.f;      // dP and delta take what P has not
 
   if (warp == 0) {       // dO tiles; Q tiles and the statistics of their rows
     int g = (int)(first / qtiles), qt = (int)(first - (long long)g * qtiles);
+    float stats[4];                               // kRanged: of the tile to come, on their way through registers
+    auto fetch = [&]() {
+      const long long stat = ((long long)b * a.H + hk * group_heads + g) * lp + qt * kQTile + lane;
+      stats[0] = a.lse2[stat];
+      stats[1] = a.lse2[stat + 32];
+      stats[2] = a.delta[stat];
+      stats[3] = a.delta[stat + 32];
+    };
+    if (kRanged<T>) fetch();
     for (int p = 0; p < n_tiles; ++p) {
       const int sq = p % Sm::q_stages, sd = p % Sm::do_stages;
       const int h = hk * group_heads + g, row0 = qt * kQTile;
       ok = CROSS_WAIT(bar(K_Q_EMPTY + sq), ((p / Sm::q_stages) & 1) ^ 1) && CROSS_WAIT(bar(K_DO_EMPTY + sd), ((p / Sm::do_stages) & 1) ^ 1);
       if (!ok) break;
-      const uint32_t st = base + Sm::stats + sq * 512 + lane * 4;
-      const long long stat = ((long long)b * a.H + h) * lp + row0 + lane;
-      cp_async4(st, a.lse2 + stat);
-      cp_async4(st + 128, a.lse2 + stat + 32);
-      cp_async4(st + 256, a.delta + stat);
-      cp_async4(st + 384, a.delta + stat + 32);
-      cp_async_arrive_noinc(bar(K_Q_FULL + sq));
+      if (kRanged<T>) {
+        float* st = reinterpret_cast<float*>(sm + Sm::stats + sq * 512) + lane;
+        st[0] = stats[0] - kPShift;
+        st[32] = stats[1] - kPShift;
+        st[64] = stats[2] * range;
+        st[96] = stats[3] * range;
+        mbar_arrive(bar(K_Q_FULL + sq));
+      } else {
+        const uint32_t st = base + Sm::stats + sq * 512 + lane * 4;
+        const long long stat = ((long long)b * a.H + h) * lp + row0 + lane;
+        cp_async4(st, a.lse2 + stat);
+        cp_async4(st + 128, a.lse2 + stat + 32);
+        cp_async4(st + 256, a.delta + stat);
+        cp_async4(st + 384, a.delta + stat + 32);
+        cp_async_arrive_noinc(bar(K_Q_FULL + sq));
+      }
       if (lane == 0) {
         mbar_arrive_expect_tx(bar(K_Q_FULL + sq), Sm::part);
         load_rows<HD>(base + Sm::q + sq * Sm::part, &map_q, row0, h, b, kSlab, bar(K_Q_FULL + sq));
@@ -1035,6 +1107,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         load_rows<HD>(base + Sm::d_o + sd * Sm::part, &map_do, row0, h, b, kSlab, bar(K_DO_FULL + sd));
       }
       if (++qt == qtiles) qt = 0, ++g;
+      if (kRanged<T> && p + 1 < n_tiles) fetch();
     }
     if (!ok && lane == 0) atomicCAS(status, 0, 91);
   } else if (warp == 2) {
@@ -1100,7 +1173,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int row = quarter * 32 + lane, c0 = cg * kDkCols, st = tid - 128;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const bool live = row < live_keys;
-    const float2 c2 = make_float2(-c, -c), m1 = make_float2(-1.f, -1.f);
+    const float2 c2 = make_float2(-c, -c), m1 = make_float2(-1.f, -1.f), mf = make_float2(-range, -range);
     for (int p = 0; p < n_tiles && ok; ++p) {
       const int bf = p % Sm::bufs, sq = p % Sm::q_stages;
       const uint32_t ph = (p / Sm::bufs) & 1;
@@ -1140,8 +1213,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
       for (int i = 0; i < kDkCols / 4; ++i) {
         const float4 d4 = s_lse[16 + i];       // delta: 64 floats behind the statistics
-        const float2 x = mul2(pf[2 * i], fma2(word_pair(dvv + 4 * i), m1, make_float2(d4.x, d4.y)));      // -dS
-        const float2 y = mul2(pf[2 * i + 1], fma2(word_pair(dvv + 4 * i + 2), m1, make_float2(d4.z, d4.w)));
+        const float2 x = mul2(pf[2 * i], fma2(word_pair(dvv + 4 * i), mf, make_float2(d4.x, d4.y)));      // -dS
+        const float2 y = mul2(pf[2 * i + 1], fma2(word_pair(dvv + 4 * i + 2), mf, make_float2(d4.z, d4.w)));
         pk[2 * i] = live ? Elem<T>::pack(x.x, x.y) : 0u;
         pk[2 * i + 1] = live ? Elem<T>::pack(y.x, y.y) : 0u;
       }
@@ -1163,7 +1236,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         uint32_t av[32];
         tmem_ld((is_k ? tmem_dk : tmem_dv) + lane_addr + 32 * jj, av);
         tmem_ld_wait();
-        const float mul = is_k ? -a.scale : 1.f;       // the products summed -dS
+        // the products summed -dS
+        const float mul = is_k ? -a.scale * (kRanged<T> ? power_of_two(-e) : 1.f) : kRanged<T> ? power_of_two(-kPShift) : 1.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) av[i] = live ? __float_as_uint(__uint_as_float(av[i]) * mul) : 0u;
         if (part == nullptr) {
@@ -1194,6 +1268,42 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// max |v|^2 of a key head's live keys in 32 parts, and a zero where dQ will put max |do|^2.  A row is D / 8 lanes of 16 bytes.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) cross_bounds_kernel(const __grid_constant__ VsaCross a) {
+  __shared__ unsigned top[8];
+  constexpr int kParts = VSA_CROSS_BOUNDS - 1;
+  const int piece = blockIdx.x % kParts, bhk = blockIdx.x / kParts, b = bhk / (int)a.Hkv, hk = bhk - b * (int)a.Hkv;
+  const int tid = threadIdx.x, lane = tid % LANES, len = cross_length(a, b);
+  const int per = (len + kParts - 1) / kParts, r1 = (int)min((long long)len, (long long)per * (piece + 1));
+  const T* v = (const T*)a.v + b * a.v_stride[0] + hk * a.v_stride[1] + lane * 8;
+  unsigned most = 0;
+  for (int r0 = piece * per; r0 < r1; r0 += 256 / LANES) {
+    const int r = r0 + tid / LANES;
+    float x = 0.f;
+    if (r < r1 && lane * 8 < a.D) {
+      const uint4 p = *reinterpret_cast<const uint4*>(v + r * a.v_stride[2]);
+      const uint32_t* w = &p.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Elem<T>::unpack(w[i]);
+        x = fmaf(f.x, f.x, fmaf(f.y, f.y, x));
+      }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    most = max(most, __float_as_uint(x));          // non-negative numbers, NaN above them all
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((tid & 31) == 0) top[tid >> 5] = most;
+  __syncthreads();
+  if (tid > 0) return;
+  for (int i = 1; i < 8; ++i) most = max(most, top[i]);
+  float* to = a.bounds + (long long)bhk * VSA_CROSS_BOUNDS;
+  to[piece] = __uint_as_float(most);
+  if (piece == 0) to[kParts] = 0.f;
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
@@ -1253,6 +1363,10 @@ int launch_bwd(const VsaCross& a, int splits, bool parts, float* part, cudaStrea
   const int64_t qtiles = (a.Lq + kRows - 1) / kRows, items = a.B * a.H * qtiles, ktiles = (a.Lkv + kRows - 1) / kRows;
   const int64_t units = a.B * a.Hkv * ktiles * splits;
   if (items > 0x3fffffff || units > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention backward: too many rows");
+  if constexpr (kRanged<T>) {
+    cross_bounds_kernel<T, HD / 8><<<(unsigned)(a.B * a.Hkv * (VSA_CROSS_BOUNDS - 1)), 256, 0, st>>>(a);
+    if ((rc = check_launch("cross_bounds_kernel"))) return rc;
+  }
   const int64_t sms = device_sms();
   cross_dq_umma_kernel<T, HD><<<(unsigned)(items < sms ? items : sms), kDqThreads, DqSmem<HD>::total, st>>>(
       mq, mdo, mk, mv, mdq, a, Divisor((uint32_t)qtiles), Divisor((uint32_t)a.H), Divisor((uint32_t)(a.H / a.Hkv)), (int)items, status);

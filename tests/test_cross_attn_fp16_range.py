@@ -1,0 +1,90 @@
+"""Backward of cross attention in fp16: gradients far from one, many keys, values of any size, against float64.
+
+Softmax weights of many keys and their gradients are far below fp16's smallest normal number, 2^-14, where its steps are an absolute 2^-24;
+what the results may be off is what their own rounding and the relative bound of the other tests allow."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from simple_vsa_b200 import _lib
+from tests.test_cross_attn import DEV, _bound, _exact, _inputs, _live, _run
+
+
+def test_arguments_of_the_c_entry():
+    a = _lib.Cross()
+    assert _lib.Cross.PACK.size == ctypes.sizeof(a)
+    a.B, a.H, a.Hkv, a.Lq, a.Lkv, a.D, a.dtype, a.scale = 1, 1, 1, 4, 4, 64, _lib.VSA_F16, 0.25
+    for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "lse2", "delta", "workspace"):
+        setattr(a, n, 1 << 20)
+    assert _lib.lib.vsa_cross_bwd(a, None) == _lib.ERR_BAD_ARGUMENT and "bounds" in _lib.last_error()      # refused before any launch
+
+
+def _check(got, want, names=("out", "dq", "dk", "dv")):
+    for name, x, y, off in zip(names, got, want, want[4]):
+        assert x.dtype == torch.float16
+        x = x.detach().double().cpu()
+        assert torch.isfinite(x).all(), name
+        err = (x - y).norm().item()
+        # a result below 2^-14 is rounded to the nearest multiple of 2^-24, off by 2^-25 at most
+        allowed = _bound(torch.float16) * y.norm().item() + off + 2.0 ** -25 * math.sqrt(y.numel())
+        assert err <= allowed, (name, err, y.norm().item(), allowed)
+
+
+SHAPES = [  # B, H, Hk, L, T, D
+    (1, 2, 1, 300, 512, 128), (2, 2, 2, 130, 1001, 64), (1, 2, 1, 300, 2048, 128), (1, 1, 1, 200, 2048, 72), (1, 2, 2, 200, 16384, 64),
+    (1, 1, 1, 130, 65536, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4, 300.0])
+@pytest.mark.parametrize("B,H,Hk,L,T,D", SHAPES)
+def test_incoming_gradients_of_any_size(B, H, Hk, L, T, D, size):
+    q, k, v, dout = _inputs(B, H, Hk, L, T, D, torch.float16, T + D)
+    dout = (dout.float() * size).half()
+    _check(_run(q, k, v, dout), _exact(q, k, v, _live(B, T, None, None), 1 / math.sqrt(D), dout))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("values,size", [(1e-3, 1.0), (1e-3, 1000.0), (200.0, 1e-3), (200.0, 10.0), (1000.0, 1e-4)])
+def test_values_of_any_size(values, size):
+    """Peaked and flat rows: p (dp - delta) as large as the bound on it, and small beside it."""
+    B, H, Hk, L, T, D = 1, 2, 1, 300, 700, 128
+    q, k, v, dout = _inputs(B, H, Hk, L, T, D, torch.float16, 31)
+    q[:, :, ::2] *= 3
+    v, dout = (v.float() * values).half(), (dout.float() * size).half()
+    _check(_run(q, k, v, dout), _exact(q, k, v, _live(B, T, None, None), 1 / math.sqrt(D), dout))
+
+
+@pytest.mark.gpu
+def test_rows_and_samples_of_different_sizes():
+    """Rows of the gradient 2^10 apart, a row of zeros, and samples that share nothing: each with lengths, with a mask, and with an
+    encoder state outside them that is infinite."""
+    B, H, Hk, L, T, D = 3, 2, 1, 260, 600, 64
+    q, k, v, dout = _inputs(B, H, Hk, L, T, D, torch.float16, 32)
+    rows = 2.0 ** -(torch.arange(L, device=DEV) % 11).float()
+    dout = (dout.float() * rows[None, None, :, None] * torch.tensor([1.0, 1e-3, 50.0], device=DEV).view(3, 1, 1, 1)).half()
+    dout[:, :, 7] = 0
+    lengths, mask = torch.tensor([T, 333, 0]), torch.rand(B, T, generator=torch.Generator().manual_seed(3)) < 0.5
+    for ln, mk in ((lengths, None), (None, mask)):
+        live = _live(B, T, ln, mk)
+        kk, vv = k.clone(), v.clone()
+        dead = ~live[:, None, :, None].to(DEV).expand_as(kk)
+        kk[dead], vv[dead] = math.nan, math.inf
+        got = _run(q, kk, vv, dout, ln, None if mk is None else mk.to(DEV))
+        want = _exact(q, k, v, live, 1 / math.sqrt(D), dout)
+        for b in range(B):                            # each sample by its own norms
+            if not live[b].any():
+                assert all(not x[b].any() for x in got)
+                continue
+            part = lambda x: x[b:b + 1]
+            _check([part(x) for x in got], [*(part(x) for x in want[:4]), _exact(*(part(x) for x in (q, k, v)), part(live), 1 / math.sqrt(D), part(dout))[4]])
+        assert not got[1][:, :, 7].any()
+        assert all(torch.equal(x, y) for x, y in zip(got, _run(q, kk, vv, dout, ln, None if mk is None else mk.to(DEV))))
+        # a row's dQ does not lose digits to larger rows: each row class by itself
+        for c in range(11):
+            x, y = got[1][0, :, c::11].double().cpu(), want[1][0, :, c::11]
+            e = 2 * torch.finfo(torch.float16).eps * (want[0][0, :, c::11] * dout[0, :, c::11].double().cpu()).norm(dim=-1) / math.sqrt(D)
+            assert (x - y).norm() <= 2 * _bound(torch.float16) * y.norm() + 8 * e.norm() + 2.0 ** -25 * math.sqrt(y.numel())
