@@ -138,8 +138,7 @@ def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
             kv_mask = kv_mask.to(q.device)
             key_bits = _key_bits(kv_mask if T <= 1 or kv_mask.stride(1) == 1 else kv_mask.contiguous(), kv_lengths)
         q, k, v = _usable(q), _usable(k), _usable(v)
-        need_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-        if need_grad:
+        if ops._differentiated(q, k, v):
             return _CrossAttention.apply(q, k, v, kv_lengths, key_bits, scale, raster)
         return _forward(q, k, v, kv_lengths, key_bits, scale, raster)[0]
 

@@ -20,6 +20,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call
@@ -106,6 +107,21 @@ def _like(x: Tensor) -> Tensor:
     two dims of stride 1, and ``empty_like`` may put the other one innermost.)"""
     y = torch.empty_like(x)
     return y if y.stride(3) == 1 or y.shape[3] <= 1 else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+def _has_tangent(x: Tensor) -> bool:
+    # tangents exist inside a dual level only: outside, the question to the tensor (0.3 us) is spared
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
+def _differentiated(*xs: Optional[Tensor]) -> bool:
+    """Whether a call on these tensors has to go through its autograd function: a gradient is recorded, or one of them carries a
+    forward-mode tangent, whether or not it requires a gradient (the function refuses it; past the function it would vanish)."""
+    recorded = torch.is_grad_enabled()
+    for x in xs:
+        if x is not None and (recorded and x.requires_grad or _has_tangent(x)):
+            return True
+    return False
 
 
 def _integers(x: Tensor) -> bool:

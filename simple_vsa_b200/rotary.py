@@ -93,7 +93,7 @@ def _table(rotary: Dict[str, object], head_dim: int, device) -> Tuple[Tensor, Te
         raise ValueError("the rotary table's cos and sin must share the shape [positions, rotary_dim/2]")
     if 2 * cos.shape[1] > head_dim:
         raise ValueError(f"the rotary table turns {2 * cos.shape[1]} dims of a head, the tensors have {head_dim}")
-    if cos.requires_grad or sin.requires_grad:
+    if cos.requires_grad or sin.requires_grad or ops._has_tangent(cos) or ops._has_tangent(sin):
         raise ValueError("the rotary table is a constant: it receives no gradient")
     if cos.device != device or cos.dtype != torch.float32 or sin.device != device or sin.dtype != torch.float32:
         cos, sin = cos.to(device=device, dtype=torch.float32), sin.to(device=device, dtype=torch.float32)
@@ -187,8 +187,7 @@ def _turn(q: Tensor, k: Optional[Tensor], rotary: Dict[str, object], positions: 
     with torch.cuda.device(q.device):
         if positions is not None:
             positions = positions.to(device=q.device, dtype=torch.int32).contiguous()
-        need_grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
-        out_q, out_k = (_Rotary.apply if need_grad else _turned)(q, k, cos, sin, positions, interleaved, raster)
+        out_q, out_k = (_Rotary.apply if ops._differentiated(q, k) else _turned)(q, k, cos, sin, positions, interleaved, raster)
     return out_q if k is None else (out_q, out_k)
 
 
