@@ -736,9 +736,16 @@ int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* 
   return cross_key_bits(mask, mask_stride, kv_lengths, key_bits, B, Lkv, (cudaStream_t)stream);
 }
 
-static bool cross_on_umma(const VsaCross& a, bool backward) { return !scalar_forced() && cross_umma_eligible(a, backward); }
+// Which kernels: the pass over the keys for a forward of few rows, the tcgen05 kernels, or those of the CUDA cores.
+static bool cross_on_rows(const VsaCross& a) { return !scalar_forced() && cross_few_rows(a.H, a.Hkv, a.Lq, a.D, a.dtype) && cross_aligned(a, false); }
+static bool cross_on_umma(const VsaCross& a, bool backward) {
+  return !scalar_forced() && cross_umma_eligible(a, backward) && (backward || !cross_on_rows(a));
+}
 
-int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) { return a != nullptr && cross_on_umma(*a, backward != 0) ? 1 : 0; }
+int vsa_cross_on_tensor_cores(const VsaCross* a, int backward) {
+  if (a == nullptr || !cross_extents_fine(a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D) || a->B == 0 || a->H == 0) return 0;
+  return cross_on_umma(*a, backward != 0) ? 1 : 0;
+}
 
 // The call on compacted keys: dense K and V of which the first counts[b] rows of a sample take part.
 static int compacted(const VsaCross& a, const CrossSpace& s, VsaCross* out, cudaStream_t st) {
@@ -760,7 +767,7 @@ int vsa_cross_fwd(const VsaCross* a, void* stream) {
   const CrossSpace s = cross_space(false, a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D, a->dtype, a->key_bits != nullptr);
   float* part_out = (float*)a->workspace;
   float* part_lse = part_out + (s.splits == 1 ? 0 : s.splits * a->B * a->H * a->Lq * a->D);
-  if (cross_few_rows(a->H, a->Hkv, a->Lq, a->D, a->dtype) && !scalar_forced() && cross_aligned(*a, false)) {
+  if (cross_on_rows(*a)) {
     rc = cross_fwd_rows(*a, s.splits, part_out, part_lse, st);
   } else if (!cross_on_umma(*a, false)) {
     rc = cross_fwd_generic(*a, s.splits, part_out, part_lse, st);
