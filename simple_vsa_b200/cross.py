@@ -35,6 +35,7 @@ def _usable(x: Tensor) -> Tensor:
 _PACK = _lib.Cross.PACK.pack
 _ARGUMENTS = _lib.Cross.from_buffer_copy
 _NO_STRIDES = (0, 0, 0)
+_LARGEST = torch.finfo(torch.float32).max
 
 
 def _steps(x: Optional[Tensor], raster: bool):
@@ -103,6 +104,13 @@ class _CrossAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
+def _scale(sm_scale: Optional[float], dim: int) -> float:
+    scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(dim)
+    if not abs(scale) * math.log2(math.e) <= _LARGEST:           # the kernels' factor of exponents of two, in fp32
+        raise ValueError(f"sm_scale must be finite in fp32 (magnitude up to {_LARGEST * math.log(2):.3g}), got {scale}")
+    return scale
+
+
 def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
     layout = "[batch, seq_len, heads, head_dim]" if raster else "[batch, heads, seq_len, dim]"
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
@@ -125,9 +133,7 @@ def _attend(q, k, v, kv_lengths, kv_mask, sm_scale, raster: bool) -> Tensor:
         raise ValueError(f"kv_lengths must hold {B} integers of a signed type or uint8, one per sample")
     if kv_mask is not None and (kv_mask.dtype != torch.bool or tuple(kv_mask.shape) != (B, T)):
         raise ValueError(f"kv_mask must be a bool tensor of shape [{B}, {T}], True where a key takes part")
-    scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D)
-    if not math.isfinite(scale):
-        raise ValueError("sm_scale must be finite")
+    scale = _scale(sm_scale, D)
     with torch.cuda.device(q.device):
         if kv_lengths is not None:
             if kv_lengths.dtype == torch.int64:
@@ -150,7 +156,7 @@ def video_cross_attn(q: Tensor, k: Tensor, v: Tensor, kv_lengths: Optional[Tenso
     ``heads`` is a multiple of ``kv_heads``; neighbouring query heads share a key head.  Key j of sample b takes part where
     ``j < kv_lengths[b]`` (None: all; lengths beyond kv_len are kv_len) and ``kv_mask[b, j]`` (bool, None: all).  What stands in
     the other keys and values does not matter, NaN included; a sample without a key that takes part gives zeros and zero
-    gradients.  Scale ``1/sqrt(dim)`` unless ``sm_scale`` says otherwise.  bf16, fp16 or fp32; head dims up to 256, in 16-bit types
+    gradients.  Scale ``1/sqrt(dim)`` unless ``sm_scale`` says otherwise (finite in fp32; above 0 on the tensor cores).  bf16, fp16 or fp32; head dims up to 256, in 16-bit types
     multiples of 8 up to 128 on the tensor cores.  Differentiable in q, k and v."""
     return _attend(q, k, v, kv_lengths, kv_mask, sm_scale, False)
 

@@ -1,6 +1,7 @@
 // extern "C" boundary of the library: argument checks, dispatch between the
 // tensor-core and the scalar kernels, error text.  No allocation, no host sync.
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 
@@ -715,6 +716,7 @@ static int check_cross(const VsaCross* a, bool backward, const char* what) {
   VSA_REQUIRE(a->B >= 0 && a->Lq >= 0 && a->Lkv >= 0 && a->D >= 1, "%s: negative extent", what);
   if (!cross_extents_fine(a->B, a->H, a->Hkv, a->Lq, a->Lkv, a->D))
     return fail(VSA_ERR_UNSUPPORTED, "%s: head dims up to 256, batches and heads up to 65535, 2^30 tokens", what);
+  VSA_REQUIRE(std::isfinite(a->scale * kLog2e), "%s: the scale, as a factor of exponents of two, is not finite", what);
   if (a->B == 0 || a->Hkv == 0) return VSA_OK;
   const bool rows = a->H > 0 && a->Lq > 0, keys = a->Lkv > 0;
   VSA_REQUIRE(!rows || (a->q && a->out && a->lse2), "%s: null pointer", what);

@@ -1,5 +1,7 @@
 """Which kernels a call of cross attention runs on, as the library says."""
 
+import math
+
 import pytest
 
 from simple_vsa_b200 import _lib
@@ -37,3 +39,16 @@ def test_which_calls_run_on_the_tensor_cores(args, forward, backward):
 
 def test_no_call_no_tensor_cores():
     assert _lib.lib.vsa_cross_on_tensor_cores(None, 0) == 0
+
+
+def test_a_scale_that_fp32_does_not_hold_is_refused():
+    from simple_vsa_b200 import cross
+    assert cross._scale(None, 64) == 0.125 and cross._scale(-2e38, 64) == -2e38 and cross._scale(1e-60, 64) == 1e-60
+    for scale in (1e39, -1e300, 3e38, math.inf, math.nan):
+        with pytest.raises(ValueError, match="finite"):
+            cross._scale(scale, 64)
+    a = call_of(1, 2, 2, 100, 100, 64)
+    for scale in (3e38, -3e38, math.inf, math.nan):
+        a.scale = scale
+        for f in (_lib.lib.vsa_cross_fwd, _lib.lib.vsa_cross_bwd):
+            assert f(a, None) == _lib.ERR_BAD_ARGUMENT and "scale" in _lib.last_error()      # refused before any launch
