@@ -634,12 +634,12 @@ int vsa_combine_bwd(const void* dout, const void* gate, const void* out_c, void*
 
 // ---- cross attention ----------------------------------------------------------------------------------------
 // Parts that a pass is cut into: `units` blocks of work of `steps` steps each; a part more costs a block's set-up, taken as
-// `setup` steps.  The smallest time of whole waves over the SMs wins, the fewest parts among equals.
-static int cross_parts(int64_t units, int64_t steps, int64_t setup, int64_t most) {
-  const int64_t sms = 148;
-  int best = 1;
+// `setup` steps.  The smallest time of whole waves over the SMs wins, the fewest parts among equals; none of more than `longest` steps.
+static int cross_parts(int64_t units, int64_t steps, int64_t setup, int64_t most, int64_t longest = INT64_MAX) {
+  const int64_t sms = 148, least = steps <= longest ? 1 : (steps - 1) / longest + 1;
+  int best = (int)least;
   int64_t best_time = -1;
-  for (int64_t s = 1; s <= steps && s <= most; ++s) {
+  for (int64_t s = least; s <= steps && s <= most; ++s) {
     const int64_t per = (steps + s - 1) / s;
     if ((steps + per - 1) / per != s) continue;      // the same cut as with fewer parts
     const int64_t time = (units * s + sms - 1) / sms * (per + setup);
@@ -656,13 +656,13 @@ static int cross_fwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64
     const int64_t s = units >= 148 ? 1 : most < steps ? most : steps;
     return (int)(s < 64 ? s : 64);
   }
-  if (cross_umma_shape(D, dtype)) return cross_parts(B * H * ((Lq + 255) / 256), (Lkv + 127) / 128, 4, 64);
+  if (cross_umma_shape(D, dtype)) return cross_parts(B * H * ((Lq + 255) / 256), (Lkv + 127) / 128, 4, 64, cross_umma_sum(dtype) / 128);
   const CrossTile tile = cross_generic_fwd_tile(B, H, Lq, Lkv, D);
   return cross_parts(B * H * ((Lq + tile.rows - 1) / tile.rows), (Lkv + tile.cols - 1) / tile.cols, 2, 64);
 }
 static int cross_bwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
   // a step of the tensor path is 64 query rows; a CTA's set-up and epilogue and its share of the sum weigh about ten
-  if (cross_umma_shape(D, dtype)) return cross_parts(B * Hkv * ((Lkv + 127) / 128), (H / Hkv) * ((Lq + 63) / 64), 10, 64);
+  if (cross_umma_shape(D, dtype)) return cross_parts(B * Hkv * ((Lkv + 127) / 128), (H / Hkv) * ((Lq + 63) / 64), 10, 64, cross_umma_sum(dtype) / 64);
   const CrossTile tile = cross_generic_bwd_tile(B, H, Hkv, Lq, Lkv, D);
   return cross_parts(B * Hkv * ((Lkv + tile.rows - 1) / tile.rows), (H / Hkv) * ((Lq + tile.cols - 1) / tile.cols), 2, 64);
 }
@@ -687,7 +687,7 @@ struct CrossSpace {
 static CrossSpace cross_space(bool backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype, bool mask) {
   CrossSpace s{1, 1, 0, 0, 0, 0, 0, 0};
   if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return s;
-  const bool compact = mask && cross_umma_shape(D, dtype) && (backward || !cross_few_rows(H, Hkv, Lq, D, dtype));
+  const bool compact = mask && cross_umma_shape(D, dtype) && (backward ? Lkv <= cross_umma_sum(dtype) : !cross_few_rows(H, Hkv, Lq, D, dtype));
   s.splits = backward ? cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype) : cross_fwd_splits(B, H, Hkv, Lq, Lkv, D, dtype);
   if (!backward) s.parts = s.splits == 1 ? 0 : s.splits * B * H * Lq * (int64_t)(D + 1) * 4;
   else s.parts = s.splits == 1 && !compact ? 0 : s.splits * 2 * B * Hkv * Lkv * (int64_t)D * 4;

@@ -1387,7 +1387,9 @@ bool aligned(const void* p, const int64_t (&s)[3], int64_t heads, int64_t rows, 
 
 bool cross_umma_shape(int D, int dtype) { return (dtype == VSA_BF16 || dtype == VSA_F16) && D % 8 == 0 && D >= 8 && D <= 128; }
 
-bool cross_umma_eligible(const VsaCross& a, bool backward) { return a.scale > 0.f && cross_aligned(a, backward); }
+bool cross_umma_eligible(const VsaCross& a, bool backward) {
+  return a.scale > 0.f && !(backward && a.Lkv > cross_umma_sum(a.dtype)) && cross_aligned(a, backward);
+}
 
 bool cross_aligned(const VsaCross& a, bool backward) {
   if (!cross_umma_shape(a.D, a.dtype) || a.Lkv < 1 || a.Lq < 1) return false;

@@ -83,8 +83,14 @@ CrossTile cross_generic_dq_tile(int64_t B, int64_t H, int64_t Lq, int D);
 CrossTile cross_generic_bwd_tile(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D);
 // tensor path (cross_umma.cu), lengths only (key_bits is not looked at): by head dim and type; with pointers and strides
 bool cross_umma_shape(int D, int dtype);
+// Terms of a sum that one accumulator of the tensor cores may take.  They drop what a product has below a quarter of the accumulator's last
+// place: a sum of n terms of one sign comes out 2^-27 n too small on average (a forward of 2^20 keys of one value: -6.4e-3, of 2^22: -4e-2, both
+// as this rule says for that value).  n 2^-27 stays within a half step of the type; longer sums are cut into parts, which are added in
+// fp32.  dQ's sums over the keys are not cut: more keys are not for the tensor cores.  A piece of work also ends within a
+// wait of one role of a persistent CTA for another this way (14 million cycles of the 500 million after which it gives up).
+VSA_HD int64_t cross_umma_sum(int dtype) { return dtype == VSA_F16 ? 1 << 16 : 1 << 19; }
 bool cross_aligned(const VsaCross& a, bool backward);
-bool cross_umma_eligible(const VsaCross& a, bool backward);      // and a positive scale
+bool cross_umma_eligible(const VsaCross& a, bool backward);      // and a positive scale; backward: keys for one sum
 // at most eight rows of queries a key head (cross_rows.cu), any positive or negative scale, key_bits looked at; shapes and alignment as above
 int cross_fwd_rows(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
