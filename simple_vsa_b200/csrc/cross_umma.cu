@@ -1275,35 +1275,39 @@ template <typename T, int LANES>
 __global__ void __launch_bounds__(256) cross_bounds_kernel(const __grid_constant__ VsaCross a) {
   __shared__ unsigned top[8];
   constexpr int kParts = VSA_CROSS_BOUNDS - 1;
-  const int piece = blockIdx.x % kParts, bhk = blockIdx.x / kParts, b = bhk / (int)a.Hkv, hk = bhk - b * (int)a.Hkv;
-  const int tid = threadIdx.x, lane = tid % LANES, len = cross_length(a, b);
-  const int per = (len + kParts - 1) / kParts, r1 = (int)min((long long)len, (long long)per * (piece + 1));
-  const T* v = (const T*)a.v + b * a.v_stride[0] + hk * a.v_stride[1] + lane * 8;
-  unsigned most = 0;
-  for (int r0 = piece * per; r0 < r1; r0 += 256 / LANES) {
-    const int r = r0 + tid / LANES;
-    float x = 0.f;
-    if (r < r1 && lane * 8 < a.D) {
-      const uint4 p = *reinterpret_cast<const uint4*>(v + r * a.v_stride[2]);
-      const uint32_t* w = &p.x;
+  const int piece = blockIdx.x, tid = threadIdx.x, lane = tid % LANES;
+  for (long long bhk = blockIdx.y; bhk < a.B * a.Hkv; bhk += gridDim.y) {
+    const int b = (int)(bhk / a.Hkv), hk = (int)(bhk - b * a.Hkv), len = cross_length(a, b);
+    const int per = (len + kParts - 1) / kParts, r1 = (int)min((long long)len, (long long)per * (piece + 1));
+    const T* v = (const T*)a.v + b * a.v_stride[0] + hk * a.v_stride[1] + lane * 8;
+    unsigned most = 0;
+    for (int r0 = piece * per; r0 < r1; r0 += 256 / LANES) {
+      const int r = r0 + tid / LANES;
+      float x = 0.f;
+      if (r < r1 && lane * 8 < a.D) {
+        const uint4 p = *reinterpret_cast<const uint4*>(v + r * a.v_stride[2]);
+        const uint32_t* w = &p.x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = Elem<T>::unpack(w[i]);
-        x = fmaf(f.x, f.x, fmaf(f.y, f.y, x));
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = Elem<T>::unpack(w[i]);
+          x = fmaf(f.x, f.x, fmaf(f.y, f.y, x));
+        }
       }
-    }
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    most = max(most, __float_as_uint(x));          // non-negative numbers, NaN above them all
+      for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      most = max(most, __float_as_uint(x));        // non-negative numbers, NaN above them all
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((tid & 31) == 0) top[tid >> 5] = most;
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 1; i < 8; ++i) most = max(most, top[i]);
+      float* to = a.bounds + bhk * VSA_CROSS_BOUNDS;
+      to[piece] = __uint_as_float(most);
+      if (piece == 0) to[kParts] = 0.f;
+    }
+    __syncthreads();
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  if ((tid & 31) == 0) top[tid >> 5] = most;
-  __syncthreads();
-  if (tid > 0) return;
-  for (int i = 1; i < 8; ++i) most = max(most, top[i]);
-  float* to = a.bounds + (long long)bhk * VSA_CROSS_BOUNDS;
-  to[piece] = __uint_as_float(most);
-  if (piece == 0) to[kParts] = 0.f;
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
@@ -1364,7 +1368,8 @@ int launch_bwd(const VsaCross& a, int splits, bool parts, float* part, cudaStrea
   const int64_t units = a.B * a.Hkv * ktiles * splits;
   if (items > 0x3fffffff || units > 0x3fffffff) return fail(VSA_ERR_UNSUPPORTED, "cross attention backward: too many rows");
   if constexpr (kRanged<T>) {
-    cross_bounds_kernel<T, HD / 8><<<(unsigned)(a.B * a.Hkv * (VSA_CROSS_BOUNDS - 1)), 256, 0, st>>>(a);
+    const int64_t heads = a.B * a.Hkv;
+    cross_bounds_kernel<T, HD / 8><<<dim3(VSA_CROSS_BOUNDS - 1, (unsigned)(heads < 65535 ? heads : 65535)), 256, 0, st>>>(a);
     if ((rc = check_launch("cross_bounds_kernel"))) return rc;
   }
   const int64_t sms = device_sms();

@@ -88,3 +88,17 @@ def test_rows_and_samples_of_different_sizes():
             x, y = got[1][0, :, c::11].double().cpu(), want[1][0, :, c::11]
             e = 2 * torch.finfo(torch.float16).eps * (want[0][0, :, c::11] * dout[0, :, c::11].double().cpu()).norm(dim=-1) / math.sqrt(D)
             assert (x - y).norm() <= 2 * _bound(torch.float16) * y.norm() + 8 * e.norm() + 2.0 ** -25 * math.sqrt(y.numel())
+
+
+@pytest.mark.gpu
+def test_more_key_heads_than_a_grid_has_rows():
+    B, H, L, T, D = 700, 100, 9, 3, 8                   # 70,000 slices
+    q, k, v, dout = _inputs(B, H, H, L, T, D, torch.float16, 33)
+    dout = (dout.float() * 1e-3).half()
+    got = _run(q, k, v, dout)
+    p = torch.softmax(q.double() @ k.double().transpose(2, 3) / math.sqrt(D), dim=-1)
+    o, dp = p @ v.double(), dout.double() @ v.double().transpose(2, 3)
+    ds = p * (dp - (dout.double() * o).sum(-1, keepdim=True)) / math.sqrt(D)
+    for x, y in zip(got, (o, ds @ k.double(), ds.transpose(2, 3) @ q.double(), p.transpose(2, 3) @ dout.double())):
+        # delta from the rounded output: with three keys dP - delta is a third of dP and more, so that 2 u of delta are within another bound
+        assert (x.double() - y).norm() <= 2 * _bound(torch.float16) * y.norm() + 2.0 ** -25 * math.sqrt(y.numel())
