@@ -485,9 +485,11 @@ int vsa_rotary(const VsaRotary* a, void* stream);
  *   workspace vsa_cross_workspace_bytes(backward, ..., key_bits != NULL) bytes (0: may be NULL), 16-byte aligned, free again after the
  *             call
  * bf16 and fp16 with head dims that are multiples of 8 up to 128, 16-byte aligned pointers, strides of multiples of 8 and a positive
- * scale run on tcgen05 kernels, but for a forward of up to eight query rows a key head (H / Hkv * Lq), which is a pass over the keys, and
- * a backward of more than 2^19 keys in bf16, 2^16 in fp16; everything else up to head dim 256 runs on CUDA cores in fp32.  vsa_cross_on_tensor_cores says whether a call runs on tcgen05.  Results do not
- * depend on the order in which blocks run.  No reference counterpart (its operator is self-attention over one token grid). */
+ * scale run on tcgen05 kernels.  Not so a forward of one or two query rows a key head (H / Hkv * Lq) against up to 2048 keys, or of three or
+ * four against up to 512 where B * Hkv < 148, which is a pass over the keys, and a backward of more than 2^19 keys in bf16, 2^16 in
+ * fp16, which with everything else up to head dim 256 runs on CUDA cores in fp32.  vsa_cross_on_tensor_cores says whether a call runs on
+ * tcgen05.  Results do not depend on the order in which blocks run.  No reference counterpart (its operator is self-attention over one
+ * token grid). */
 #define VSA_CROSS_BOUNDS 33
 typedef struct VsaCross {
   const void *q, *k, *v, *dout;

@@ -648,10 +648,21 @@ static int cross_parts(int64_t units, int64_t steps, int64_t setup, int64_t most
   }
   return best;
 }
-static bool cross_few_rows(int64_t H, int64_t Hkv, int64_t Lq, int D, int dtype) { return cross_umma_shape(D, dtype) && H / Hkv * Lq <= 8; }
+// A forward of few rows a key head: a pass over the keys reads them once, where a tile of 128 rows works on rows that do not exist and a
+// mask costs it the gathering of the keys first.  The pass's arithmetic grows with the rows, and where its CTAs fill the GPU it is what takes
+// the time from three rows on; long keys are cut better for the tiles.  us of the pass and of the tiles, bf16, at 1, 2, 4 and 8 rows:
+//   [8, 40] heads, D = 128, 512 keys   22/25   26/25   53/25   80/25      40 heads, D = 128, 256 keys   7.8/13.8  9.3/13.3  11.8/13.2  17.8/13.2
+//                           2048       63/70   81/70  167/70  247/71                           512     13.4/15.5 14.5/15.1  16.9/14.9  22.9/15.0
+//                  D = 64, 512         13/21   16/21   31/21   48/21                          2048     28/23     30/22      46/22      63/22
+//   8 heads, D = 128, 512              11/13   12/12   14/12   20/12      8 heads, D = 128, 8192       53/37     55/37      65/37      76/37
+// with a mask at 4 and 8 rows: [8, 40], D = 128, 512 keys 54/51, 81/52; 40 heads, 256 13/20, 19/20, 512 18/22, 24/22; D = 64, 256 8/16, 12/16.
+static bool cross_few_rows(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
+  const int64_t rows = H / Hkv * Lq;
+  return cross_umma_shape(D, dtype) && ((rows <= 2 && Lkv <= 2048) || (rows <= 4 && Lkv <= 512 && B * Hkv < 148));
+}
 static int cross_fwd_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype) {
   // a CTA of few rows takes 256 keys or 128 at a time; three of them on an SM hide its latencies, a cut costs the join's launch
-  if (cross_few_rows(H, Hkv, Lq, D, dtype)) {
+  if (cross_few_rows(B, H, Hkv, Lq, Lkv, D, dtype)) {
     const int64_t units = B * Hkv, steps = (Lkv + 255) / 256, most = (148 * 3 + units - 1) / units;
     const int64_t s = units >= 148 ? 1 : most < steps ? most : steps;
     return (int)(s < 64 ? s : 64);
@@ -687,7 +698,7 @@ struct CrossSpace {
 static CrossSpace cross_space(bool backward, int64_t B, int64_t H, int64_t Hkv, int64_t Lq, int64_t Lkv, int D, int dtype, bool mask) {
   CrossSpace s{1, 1, 0, 0, 0, 0, 0, 0};
   if (B == 0 || H == 0 || Lq == 0 || Lkv == 0) return s;
-  const bool compact = mask && cross_umma_shape(D, dtype) && (backward ? Lkv <= cross_umma_sum(dtype) : !cross_few_rows(H, Hkv, Lq, D, dtype));
+  const bool compact = mask && cross_umma_shape(D, dtype) && (backward ? Lkv <= cross_umma_sum(dtype) : !cross_few_rows(B, H, Hkv, Lq, Lkv, D, dtype));
   s.splits = backward ? cross_bwd_splits(B, H, Hkv, Lq, Lkv, D, dtype) : cross_fwd_splits(B, H, Hkv, Lq, Lkv, D, dtype);
   if (!backward) s.parts = s.splits == 1 ? 0 : s.splits * B * H * Lq * (int64_t)(D + 1) * 4;
   else s.parts = s.splits == 1 && !compact ? 0 : s.splits * 2 * B * Hkv * Lkv * (int64_t)D * 4;
@@ -739,7 +750,7 @@ int vsa_cross_key_bits(const uint8_t* mask, int64_t mask_stride, const int32_t* 
 }
 
 // Which kernels: the pass over the keys for a forward of few rows, the tcgen05 kernels, or those of the CUDA cores.
-static bool cross_on_rows(const VsaCross& a) { return !scalar_forced() && cross_few_rows(a.H, a.Hkv, a.Lq, a.D, a.dtype) && cross_aligned(a, false); }
+static bool cross_on_rows(const VsaCross& a) { return !scalar_forced() && cross_few_rows(a.B, a.H, a.Hkv, a.Lq, a.Lkv, a.D, a.dtype) && cross_aligned(a, false); }
 static bool cross_on_umma(const VsaCross& a, bool backward) {
   return !scalar_forced() && cross_umma_eligible(a, backward) && (backward || !cross_on_rows(a));
 }

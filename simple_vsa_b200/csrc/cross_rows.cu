@@ -1,6 +1,6 @@
-// Cross attention for a few query rows: bf16 and fp16, at most eight rows (the tokens of all query heads of a key head together), the
-// decoding form.  Bound by HBM: every key and value is read once for two flops per byte and row, so there is nothing for the tensor
-// cores to do, and a tile of 128 rows spends its time on rows that do not exist.
+// Cross attention for up to four query rows (the tokens of all query heads of a key head together): bf16 and fp16, the decoding form.
+// Bound by HBM: every key and value is read once for two flops per byte and row, so there is nothing for the tensor cores to do, and a
+// tile of 128 rows spends its time on rows that do not exist.
 //
 // A key is D / 8 neighbouring lanes with 16 bytes of it each; a group of lanes walks keys of its own with its own running maximum, sum
 // and output, four keys (K and V) in flight, and the groups of a CTA are joined through shared memory.  fp32 throughout, one
@@ -154,8 +154,7 @@ int by_rows(const VsaCross& a, int splits, float* part_out, float* part_lse, cud
   const int64_t rows = a.H / a.Hkv * a.Lq;
   if (rows <= 1) cross_rows_kernel<T, 1, LANES><<<grid, kThreads, 0, st>>>(a, splits, part_out, part_lse);
   else if (rows <= 2) cross_rows_kernel<T, 2, LANES><<<grid, kThreads, 0, st>>>(a, splits, part_out, part_lse);
-  else if (rows <= 4) cross_rows_kernel<T, 4, LANES><<<grid, kThreads, 0, st>>>(a, splits, part_out, part_lse);
-  else cross_rows_kernel<T, 8, LANES><<<grid, kThreads, 0, st>>>(a, splits, part_out, part_lse);
+  else cross_rows_kernel<T, 4, LANES><<<grid, kThreads, 0, st>>>(a, splits, part_out, part_lse);
   return check_launch("cross_rows_kernel");
 }
 

@@ -91,7 +91,7 @@ bool cross_umma_shape(int D, int dtype);
 VSA_HD int64_t cross_umma_sum(int dtype) { return dtype == VSA_F16 ? 1 << 16 : 1 << 19; }
 bool cross_aligned(const VsaCross& a, bool backward);
 bool cross_umma_eligible(const VsaCross& a, bool backward);      // and a positive scale; backward: keys for one sum
-// at most eight rows of queries a key head (cross_rows.cu), any positive or negative scale, key_bits looked at; shapes and alignment as above
+// up to four rows of queries a key head (cross_rows.cu), any positive or negative scale, key_bits looked at; shapes and alignment as above
 int cross_fwd_rows(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 int cross_fwd_umma(const VsaCross& a, int splits, float* part_out, float* part_lse, cudaStream_t st);
 // parts: dK and dV go to `part` in fp32 (always with more than one split)

@@ -26,7 +26,10 @@ def on_tensor_cores(a, backward):
 @pytest.mark.parametrize("args,forward,backward", [
     ((1, 40, 40, 92160, 512, 128), 1, 1), ((2, 12, 4, 8190, 1001, 64, _lib.VSA_F16), 1, 1), ((1, 2, 2, 9, 7, 8), 1, 1),
     ((8, 40, 40, 1, 512, 128), 0, 1),            # a row each: a pass over the keys, without tensor cores; its gradient is theirs
-    ((8, 40, 8, 1, 512, 128), 0, 1), ((1, 4, 2, 4, 300, 64), 0, 1), ((1, 4, 2, 5, 300, 64), 1, 1),
+    ((1, 4, 2, 1, 300, 64), 0, 1), ((1, 4, 4, 2, 2048, 72), 0, 1), ((1, 4, 2, 1, 2049, 64), 1, 1),
+    # from five rows on the tiles are faster, up to three times at eight; from three on where the pass over the keys fills the GPU
+    ((8, 40, 8, 1, 512, 128), 1, 1), ((1, 4, 4, 3, 512, 64), 0, 1), ((1, 4, 2, 2, 513, 64), 1, 1), ((4, 80, 40, 2, 300, 64), 1, 1),
+    ((4, 40, 40, 2, 300, 64), 0, 1), ((1, 4, 4, 5, 100, 64), 1, 1),
     ((1, 2, 2, 100, 100, 128, _lib.VSA_F32), 0, 0), ((1, 2, 2, 100, 100, 136), 0, 0), ((1, 2, 2, 100, 100, 20), 0, 0),
     ((1, 2, 2, 100, 100, 64, _lib.VSA_BF16, -1.0), 0, 0), ((1, 2, 2, 1, 100, 64, _lib.VSA_BF16, 0.0), 0, 0),
     ((1, 0, 0, 100, 100, 64), 0, 0), ((0, 2, 2, 100, 100, 64), 0, 0), ((1, 2, 2, 0, 100, 64), 0, 0), ((1, 2, 2, 100, 0, 64), 0, 0),
