@@ -156,8 +156,10 @@ def video_cross_attn(q: Tensor, k: Tensor, v: Tensor, kv_lengths: Optional[Tenso
     ``heads`` is a multiple of ``kv_heads``; neighbouring query heads share a key head.  Key j of sample b takes part where
     ``j < kv_lengths[b]`` (None: all; lengths beyond kv_len are kv_len) and ``kv_mask[b, j]`` (bool, None: all).  What stands in
     the other keys and values does not matter, NaN included; a sample without a key that takes part gives zeros and zero
-    gradients.  Scale ``1/sqrt(dim)`` unless ``sm_scale`` says otherwise (finite in fp32; above 0 on the tensor cores).  bf16, fp16 or fp32; head dims up to 256, in 16-bit types
-    multiples of 8 up to 128 on the tensor cores.  Differentiable in q, k and v."""
+    gradients.  Scale ``1/sqrt(dim)`` unless ``sm_scale`` says otherwise (finite in fp32).  bf16, fp16 or fp32; head dims up to 256.  In
+    16-bit types with head dims that are multiples of 8 up to 128 and a positive scale the tensor cores do the work (a backward up to
+    2^19 keys in bf16, 2^16 in fp16); the rest runs on CUDA cores in fp32, many times slower per FLOP.  Differentiable in q, k and v;
+    forward-mode derivatives are refused."""
     return _attend(q, k, v, kv_lengths, kv_mask, sm_scale, False)
 
 

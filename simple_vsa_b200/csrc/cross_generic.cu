@@ -5,9 +5,9 @@
 // Tiles of 128 query rows x 64 keys, 64 x 64 where there are few (64 x 64 and 32 x 32 above head dim 128; dK/dV up to 128 keys x 64 query
 // rows), 256 threads, a patch of 8 x 4 scores each, everything in fp32 and one rounding at the end.  Bound by the FP32 pipe and the
 // shared-memory reads that feed it (12 of 16 bytes for 128 multiply-adds in the scores, 16 for 256 in the products): at
-// [1, 12, 4096, 128] x 2048 the forward takes 1386 us (37 of 72 TFLOP/s; pipe 64 % busy, reads 50 %), the backward 4470 (its seven products at
-// 40).  8 x 8 scores a thread spill (1448 us); chains without pairs are slower in the backward (4954), two CTAs an SM at head dim 64
-// spill too (874 us for 830).  With few query rows a pass is cut over the keys, with few keys dK/dV is over the query rows.
+// [1, 12, 4096, 128] x 2048 the forward takes 1433 us (36 of 72 TFLOP/s; pipe 62 % busy, reads 47 %), the backward 4475 (its seven products at
+// 40; 65 and 67 %, 51 and 61 %).  8 x 8 scores a thread spill (4 % slower); chains without pairs are 11 % slower in the backward, two CTAs
+// an SM at head dim 64 spill too (5 %).  With few query rows a pass is cut over the keys, with few keys dK/dV is over the query rows.
 #include <atomic>
 
 #include "common.cuh"

@@ -150,10 +150,11 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 // The softmax keeps a running maximum, but moves the accumulated row only when the maximum has grown by more than 2^8: P stays below
 // 2^8 (fp16 holds 2^16, the sums are fp32), and moving O through registers is rare.
 //
-// [1, 40, 92160, 128] x 512 keys, bf16: 835 us, 1157 TFLOP/s (994 in a long loop, power limit); [2, 12 + 4, 8190, 64] x 801 of 1001: 75 us.
-// Per 256 x 64 scores at D = 128, of some 1650 cycles: 1280 of MMAs (an M128 x N64 x K16 product takes 48 cycles of the 32 that its size
-// asks for), 1250 of shared-memory traffic (160 KB at 128 B/clk), 1024 of exponentials before a quarter of them moved to the FMA pipe;
-// what bounds it is a softmax group's chain (scores from tensor memory, maximum, exponentials, P back), which two groups overlap.
+// [1, 40, 92160, 128] x 512 keys, bf16: 867 us, 1115 TFLOP/s (959 in a long loop, power limit); [2, 12 + 4, 8190, 64] x 801 of 1001: 80 us.
+// Counters at [1, 8, 92160, 128]: 1705 cycles per 256 x 64 scores, set-up and ends included; tensor pipe active for 60 % of them, its operand
+// reads 54 % of what shared memory gives (128 KB, and 32 KB more arrive by TMA), exponentials 45 % with a quarter of them on the FMA pipe,
+// instruction issue 53 %.  No pipe is full: what bounds it is a softmax group's chain (scores from tensor memory, maximum, exponentials, P
+// back), which two groups overlap, and MMAs of 64 keys, which take 48 cycles of the 32 that their size asks for.
 // More warps were slower: eight a tile sharing its rows, and four groups on alternating steps with the maximum handed on (982 for
 // 860 us).  A piece's end (O out, the next piece's set-up) is some 3000 of 16000 cycles at 512 keys, but the other tile's group works
 // under it: four warps that write O while both groups go on brought nothing (880 -> 891 us, at eight heads 181 -> 188).
@@ -523,10 +524,11 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // form delta = rowsum(out * dout) and the statistics of the next piece's rows from memory, into two buffers, and ask L2 for the rows
 // of the piece after it; four more write a finished dQ while the elementwise warps are at the next piece.
 //
-// [1, 8, 92160, 128] x 512 keys: 236 us, 1230 TFLOP/s (where dK/dV takes 257).  A piece of four key tiles takes some 8800 cycles: 1700 to
-// 1800 a tile (1536 of MMAs, 1024 of exponentials before three of eight moved to the FMA pipe), then the elementwise warps wait 500 to
-// 800 for the delta warps, whose 8800 cycles are loads of 64 KB.  With delta and dQ done by the elementwise warps the tiles' 7000 cycles had
-// 5000 of them around (268 us).  Loads of two delta rows in flight, and Q and dO on barriers of their own, changed nothing.
+// [1, 8, 92160, 128] x 512 keys: 265 us, 1094 TFLOP/s.  9770 cycles a piece of four key tiles, set-up and ends included; tensor pipe active for
+// 63 % of them, issue 55 %, operand reads 49 %.  By clock readings in the roles a tile takes 1700 to 1800 (1536 of MMAs, 1024 of exponentials
+// before three of eight moved to the FMA pipe), and a piece's elementwise warps wait 500 to 800 more for the delta warps, which are at loads
+// of 64 KB all the time.  With delta and dQ done by the elementwise warps it took an eighth longer (268 us for 236, on a faster board).
+// Loads of two delta rows in flight, and Q and dO on barriers of their own, changed nothing.
 constexpr int kDqCols = 32;
 constexpr int kDqGroups = kRows / kDqCols;
 constexpr int kDqPoly = 3;                 // of eight pairs of exponentials, on the FMA pipe
@@ -943,9 +945,10 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 // dK / dV: lanes = 128 key rows, columns = 64 query rows of a streamed tile
 // ------------------------------------------------------------------------------------------------------
 // A CTA owns 128 keys of one key head and walks a range of the query tiles of all heads that share it; K and V stay in shared memory,
-// dK and dV in tensor memory.  S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q: 2560 tensor cycles per 128 x 128 scores, which is
-// what bounds it at D = 128: [1, 8, 92160, 128] x 512 keys 257 us, 1500 TFLOP/s.  At D = 64 a step's chain does (139 us at
-// [2, 12 + 4, 8190, 64] x 801 of 1001 keys; with two buffers and all exponentials on the MUFU 155).  The range is cut so that the CTAs
+// dK and dV in tensor memory.  S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q: 2560 cycles of MMAs per 128 x 128 scores, of 2700, which
+// is what bounds it at D = 128: [1, 8, 92160, 128] x 512 keys 287 us, 1350 TFLOP/s (tensor pipe active for 76 %, operand reads 71 %).  At
+// D = 64 a step's chain does (159 us at [2, 12 + 4, 8190, 64] x 801 of 1001 keys, fp16, 153 before its operands were kept in range; tensor
+// pipe 38 %, issue 43 %; with two buffers and all exponentials on the MUFU a tenth longer).  The range is cut so that the CTAs
 // fill whole waves of SMs; parts are added by a kernel of their own, in the order of the cuts.
 constexpr int kQTile = 64;
 constexpr int kSlab = kQTile * 128;

@@ -146,7 +146,9 @@ class _RasterVideoSparseAttention(torch.autograd.Function):
                  lse.data_ptr(), delta.data_ptr(), counts.data_ptr(), offsets.data_ptr(), inverse.data_ptr(),
                  sizes.data_ptr(), dk.data_ptr(), dv.data_ptr(), dkc.data_ptr(), dvc.data_ptr(), tile_map.data_ptr(),
                  S, H, B * H, L, L, D, be, tk, scale, dt, st)
-            if ctx.interleaved is not None:        # the kernels' gradients are those of the turned q and k: turn them back
+            # The kernels' gradients are those of the turned q and k: turn them back.  They are rounded to the operands' type on the way, half a
+            # step more on dq and dk, as they are where the rotation is a call of its own; in fp32 they would be twice the memory and traffic.
+            if ctx.interleaved is not None:
                 turned, (dq, dk) = (dq, dk), (torch.empty_like(dq), torch.empty_like(dk))
                 rot.rotate(turned, (dq, dk), saved[-2], saved[-1], ctx.interleaved, True, x_raster=True, y_raster=True)
         return dq, dk, dv, dgate, None, None, None, None, None, None, None, None
