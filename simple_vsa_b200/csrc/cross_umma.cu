@@ -44,6 +44,18 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
 }
 #define CROSS_WAIT(bar_, parity_) wait_for((bar_), (parity_))
 
+// The end of every role: a __syncthreads, and where a wait of any thread has run out, time for copies and products that are still in flight
+// to land (a millisecond; they take microseconds) before the CTA gives its shared and tensor memory back.
+constexpr uint32_t kSettleCycles = 2u * 1000u * 1000u;
+__device__ __forceinline__ void settle(bool ok) {
+  if (__syncthreads_or(!ok)) {
+    const uint32_t t0 = sm_clock();
+#pragma unroll 1
+    while (sm_clock() - t0 < kSettleCycles) {
+    }
+  }
+}
+
 // Division of n < 2^31 by a number known on the host: (n + umulhi(n, mul)) >> shift.
 struct Divisor {
   uint32_t by, mul, shift;
@@ -512,7 +524,7 @@ cross_fwd_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
   }
   tc_fence_before();
-  __syncthreads();
+  settle(ok);
   if (warp == 5) tmem_dealloc(tmem, kTmemCols);
 }
 
@@ -937,7 +949,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     if (!ok && lane == 0) atomicCAS(status, 0, 85);
   }
   tc_fence_before();
-  __syncthreads();
+  settle(ok);
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
@@ -1269,7 +1281,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     }
   }
   tc_fence_before();
-  __syncthreads();
+  settle(ok);
   if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 

@@ -37,3 +37,10 @@ def test_the_search_finds_a_barrier_that_some_warps_may_miss():
 @pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
 def test_no_named_barrier_depends_on_a_warps_own_wait(path):
     assert _under_a_wait(open(path).read()) == []
+
+
+def test_memory_in_flight_settles_before_a_cross_attention_cta_ends():
+    """Every CTA gives its tensor memory back behind ``settle``, which waits for what is in flight after a wait that ran out."""
+    text = open(os.path.join(CSRC, "cross_umma.cu")).read()
+    ends = re.findall(r"([^;]*);\s*if \(warp == \d\) tmem_dealloc", text)
+    assert len(ends) == len(re.findall(r"tmem_alloc\(", text)) == 3 and all(e.strip() == "settle(ok)" for e in ends)
