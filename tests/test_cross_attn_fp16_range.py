@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from simple_vsa_b200 import _lib
+from simple_vsa_b200 import _lib, video_cross_attn
 from tests.test_cross_attn import DEV, _bound, _exact, _inputs, _live, _run
 
 
@@ -102,3 +102,54 @@ def test_more_key_heads_than_a_grid_has_rows():
     for x, y in zip(got, (o, ds @ k.double(), ds.transpose(2, 3) @ q.double(), p.transpose(2, 3) @ dout.double())):
         # delta from the rounded output: with three keys dP - delta is a third of dP and more, so that 2 u of delta are within another bound
         assert (x.double() - y).norm() <= 2 * _bound(torch.float16) * y.norm() + 2.0 ** -25 * math.sqrt(y.numel())
+
+
+@pytest.mark.gpu
+def test_captured_steps_and_side_streams():
+    """Two captured steps replayed in turn on gradients of new sizes, and two calls at once on streams of their own: the norms are each
+    call's."""
+    steps = []
+    for L, T in ((300, 200), (140, 3000)):
+        q, k, v, dout = _inputs(2, 2, 1, L, T, 64, torch.float16, L)
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+
+        def step(leaves=leaves, dout=dout):
+            out = video_cross_attn(*leaves)
+            return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step()
+        steps.append((graph, res, leaves, dout, step, side))
+    for size in (1e-3, 100.0, 1e-4, 1.0):
+        for graph, res, leaves, dout, _, _ in steps:
+            with torch.no_grad():
+                dout.copy_(torch.randn(dout.shape, device=DEV) * size)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(res, _run(*leaves, dout)))
+    steps[0][3].mul_(1e-3)
+    torch.cuda.synchronize()
+    together = []
+    for _, _, _, _, step, side in steps:
+        with torch.cuda.stream(side):
+            together.append(step())
+    torch.cuda.synchronize()
+    for got, (_, _, leaves, dout, _, _) in zip(together, steps):
+        assert all(torch.equal(a, b) for a, b in zip(got, _run(*leaves, dout)))
+
+
+@pytest.mark.gpu
+def test_gradients_of_some_operands_only():
+    q, k, v, dout = _inputs(2, 4, 2, 130, 900, 64, torch.float16, 35)
+    dout = (dout.float() * 1e-3).half()
+    want = _run(q, k, v, dout)[1:]
+    for need in ((0,), (1,), (2,), (0, 2)):
+        xs = [x.clone().requires_grad_(i in need) for i, x in enumerate((q, k, v))]
+        got = torch.autograd.grad(video_cross_attn(*xs), [xs[i] for i in need], dout)
+        assert all(torch.equal(g, want[i]) for g, i in zip(got, need))
