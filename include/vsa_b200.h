@@ -477,7 +477,8 @@ int vsa_rotary(const VsaRotary* a, void* stream);
  * looked at (they may hold anything) and receive zeros.  Strides in elements: batch, head, token; head dims contiguous.
  *   key_bits  [B, vsa_cross_words(Lkv)] from vsa_cross_key_bits (which folds kv_lengths in), or NULL
  *   lse2      [B * H, Lq rounded up to 128] fp32: base-2 log-sum-exp of the scaled scores, +inf for rows without a live key and
- *             for the padding; written by the forward, read by the backward
+ *             for the padding; written by the forward, read by the backward, whose weights are off by what its rounding costs: up to 2^-8
+ *             of themselves where it is 2^16, a fifth at 2^22, powers of two beyond
  *   delta     the same shape, scratch of the backward
  *   bounds    [B * Hkv, VSA_CROSS_BOUNDS] fp32, scratch of the backward in fp16 with head dims that are multiples of 8 up to 128, else
  *             not looked at: norms that keep its 16-bit operands within the type's range

@@ -138,16 +138,28 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, bool poly) {
 
 // fp16 holds numbers from 2^16 down to 2^-14 in full, and small gradients against many keys are below that long before the result is: the
 // backward's 16-bit operands are therefore kept in the middle of the range by powers of two that the way out takes back (bf16 has the range
-// of fp32).  P, at most 1, is held as P 2^15.  dS = P (dP - delta): with dP_ij = do_i.v_j and delta the mean of dP_i under P_i,
+// of fp32).  P, at most 1, is held as P 2^14.  dS = P (dP - delta): with dP_ij = do_i.v_j and delta the mean of dP_i under P_i,
 // |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= P (1 - P) 2 |do_i| max|v| <= |do_i| max|v| / 2, so that the largest 2^e with
-// 2^e |do_i| max|v| <= 2^16 keeps it below 2^15 whatever the operands hold, the rounding of delta included.  dQ takes an e for each row;
-// dK and dV add rows up, and take one for all rows of a key head.
+// 2^e |do_i| max|v| <= 2^15 keeps it within 2^14 whatever the operands hold.  The factor of four to the type's end is for the roundings of
+// delta and of exponents of many thousands.  dQ takes an e for each row; dK and dV add rows up, and take one for all rows of a key head.
 template <typename T> constexpr bool kRanged = kFmt<T> == 0u;
-constexpr int kPShift = 15;
+constexpr int kPShift = 14;
 // e from the product of the squared norms (0: nothing to hold; infinite or NaN: nothing to save)
 __device__ __forceinline__ int range_exponent(float squares) {
   const int log2 = (int)(__float_as_uint(squares) >> 23) - 127;      // floor; squares >= 0
-  return max(-30, min(60, 15 - (log2 >> 1)));
+  return max(-30, min(60, 14 - (log2 >> 1)));
+}
+// P and dS of the backward, to 16 bits.  In fp16 never to infinity: where the scores are so large that the last place of their fp32 statistic is
+// several units (from 2^25 on), the weights formed with it may come out above four.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  if constexpr (!kRanged<T>) {
+    return Elem<T>::pack(lo, hi);
+  } else {
+    uint32_t w;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+  }
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -929,7 +941,7 @@ cross_dq_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float2 y = mul2(pf[h / 2 + i], kRanged<T> ? fma2(word_pair(dv + 2 * i), f2, d2) : add2(word_pair(dv + 2 * i), d2));
-            pk[h / 2 + i] = Elem<T>::pack(y.x, y.y);
+            pk[h / 2 + i] = pack_weights<T>(y.x, y.y);
           }
         }
         if (c0 + kDqCols > live) {               // what stands in a key that takes no part may be anything
@@ -1076,7 +1088,7 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
   const uint32_t tmem_dk = tmem + 128 * Sm::bufs, tmem_dv = tmem_dk + HD;
   static_assert(128 * Sm::bufs + 2 * HD <= (int)kTmemCols, "tensor memory of the dK/dV pass");
   bool ok = true;
-  int e = 0;                                      // kRanged: dS is held as dS 2^e, P as P 2^15
+  int e = 0;                                      // kRanged: dS is held as dS 2^e, P as P 2^kPShift
   if (kRanged<T> && (warp == 0 || warp >= 4)) {
     const float* bounds = a.bounds + (long long)bhk * VSA_CROSS_BOUNDS;      // 32 parts of max |v|^2, then max |do|^2
     e = range_exponent(warp_max(bounds[lane]) * bounds[VSA_CROSS_BOUNDS - 1]);
@@ -1211,8 +1223,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         pf[2 * i] = kDkPoly<HD> > 2 * i % 8 ? poly_exp2<T>(mul2(x, m1)) : make_float2(fast_exp2(-x.x), fast_exp2(-x.y));
         pf[2 * i + 1] = kDkPoly<HD> > (2 * i + 1) % 8 ? poly_exp2<T>(mul2(y, m1)) : make_float2(fast_exp2(-y.x), fast_exp2(-y.y));
         // a key that takes no part: its scores come from whatever sits in K there
-        pk[2 * i] = live ? Elem<T>::pack(pf[2 * i].x, pf[2 * i].y) : 0u;
-        pk[2 * i + 1] = live ? Elem<T>::pack(pf[2 * i + 1].x, pf[2 * i + 1].y) : 0u;
+        pk[2 * i] = live ? pack_weights<T>(pf[2 * i].x, pf[2 * i].y) : 0u;
+        pk[2 * i + 1] = live ? pack_weights<T>(pf[2 * i + 1].x, pf[2 * i + 1].y) : 0u;
       }
       tmem_st(s_addr, pk);
       tmem_st_wait();
@@ -1230,8 +1242,8 @@ cross_dkdv_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const float4 d4 = s_lse[16 + i];       // delta: 64 floats behind the statistics
         const float2 x = mul2(pf[2 * i], fma2(word_pair(dvv + 4 * i), mf, make_float2(d4.x, d4.y)));      // -dS
         const float2 y = mul2(pf[2 * i + 1], fma2(word_pair(dvv + 4 * i + 2), mf, make_float2(d4.z, d4.w)));
-        pk[2 * i] = live ? Elem<T>::pack(x.x, x.y) : 0u;
-        pk[2 * i + 1] = live ? Elem<T>::pack(y.x, y.y) : 0u;
+        pk[2 * i] = live ? pack_weights<T>(x.x, x.y) : 0u;
+        pk[2 * i + 1] = live ? pack_weights<T>(y.x, y.y) : 0u;
       }
       tmem_st(s_addr + 64, pk);
       tmem_st_wait();

@@ -153,3 +153,16 @@ def test_gradients_of_some_operands_only():
         xs = [x.clone().requires_grad_(i in need) for i, x in enumerate((q, k, v))]
         got = torch.autograd.grad(video_cross_attn(*xs), [xs[i] for i in need], dout)
         assert all(torch.equal(g, want[i]) for g, i in zip(got, need))
+
+
+@pytest.mark.gpu
+def test_scores_of_many_thousands():
+    """Exponents whose fp32 steps are no longer small beside one: weights may be off by a factor, and stay finite on their way through fp16."""
+    q, k, v, dout = _inputs(1, 2, 1, 130, 300, 128, torch.float16, 36)
+    for size in (100.0, 1000.0, 4000.0):
+        got = _run((q.float() * size).half(), (k.float() * size).half(), v, dout)
+        assert all(torch.isfinite(x).all() for x in (got[0], got[3]))
+        # At the largest size scores are 1.6e7 apart and more, one key has a row's weight, and exponents of 2^25 and more have steps of 4 and
+        # more: the statistic's rounding makes that weight any power of two.  It is held up to 65504 / 2^14 < 4, so that what the values'
+        # gradient sums to over the keys is at most four times dout's.
+        assert (got[3].double().sum((1, 2)).abs() <= 4 * dout.double().abs().sum((1, 2)) + 1).all()
